@@ -69,7 +69,7 @@ const char* ngdn_last_error(void);
  * 0.5.0 took W and U out of ngdn_l0_bwd; 0.6.0 moved the upper levels'
  * lower-state gradients from ngdn_probe_bwd's d_below to an injection that
  * ngdn_upper_scan_bwd adds. */
-#define NGDN_VERSION 1100
+#define NGDN_VERSION 1200
 int32_t ngdn_version(void);
 /* Offload architecture the library was built for ("gfx950"). */
 const char* ngdn_arch(void);
@@ -584,6 +584,70 @@ int32_t ngdn_scale(int32_t x_dtype, int32_t out_dtype, int64_t n, const void* x,
 int32_t ngdn_cross_entropy(int32_t dtype, int64_t rows, int32_t V, int32_t ignore_index,
                            void* logits, const int64_t* labels, const int64_t* n_valid,
                            float* row_loss, int32_t grad, void* stream);
+
+/* ---- The embedding. No counterpart kernel in the reference, which uses
+ * torch's nn.Embedding (models/modeling_nested_gdn2.py:97,122). */
+
+/* y[n,:] = scale w[ids[n],:] rounded to y_dtype. ids int64 [N], w [V,D] in
+ * w_dtype, y [N,D]; both types NGDN_F32 or NGDN_BF16, any N, D >= 1 and V >= 1.
+ * An id outside [0, V) is not read and gives a row of NaN. */
+int32_t ngdn_embedding_fwd(int32_t w_dtype, int32_t y_dtype, int64_t N, int64_t V, int32_t D,
+                           float scale, const int64_t* ids, const void* w, void* y, void* stream);
+/* Its gradient: dw[v,:] = scale sum of dy[n,:] over the n with ids[n] == v, in
+ * fp32 and in an order that the ids alone fix, rounded once to w_dtype; every
+ * row of dw [V,D] is written (zeros where no id points, and on row
+ * padding_idx; negative: no such row). Ids outside [0, V) add nothing. ws:
+ * ngdn_embedding_ws(N, V, D) int32, no initial contents. */
+int32_t ngdn_embedding_bwd(int32_t dy_dtype, int32_t w_dtype, int64_t N, int64_t V, int32_t D,
+                           float scale, int64_t padding_idx, const int64_t* ids, const void* dy,
+                           void* dw, int32_t* ws, void* stream);
+int64_t ngdn_embedding_ws(int64_t N, int64_t V, int32_t D);
+
+/* ---- A gated linear recurrence with a vector state, beside the op's matrix
+ * state (no counterpart in the reference). Per token t and channel d of head
+ * h = d / (D / H):
+ *   g = -exp(A_log[h]) softplus(f + dt_bias[d]), a = e^g,
+ *   s_t = a s_(t-1) + sqrt(1 - a^2) sigmoid(wz) x,  y_t = s_t
+ * the decay with the layer's parameters (as ngdn_gate_prep_fwd's g0).
+ * x, f, wz in dtype, D consecutive values a token, token t of row b at
+ * b *_b + t *_t elements (column slices of a joint projection are taken as
+ * they are); y [B,T,D] in dtype; A_log [H], dt_bias [D], states fp32.
+ *   cu NULL: B rows of T tokens; h0, final_state, dfinal, dh0 [B,D].
+ *   cu int32 [S+1], B = 1: S sequences, tokens [cu[s], cu[s+1]) of the row;
+ *   h0, final_state, dfinal, dh0 [S,D]. cu holds 0 <= cu[0] <= ... <= cu[S]
+ *   <= T; it is read on the device, so it is not checked (values that are not
+ *   so give wrong results, no access outside the arrays). A sequence without
+ *   tokens keeps its state. Tokens in no sequence: y and gradients 0, their
+ *   inputs have no effect.
+ * h0 and dfinal may be NULL (zeros), final_state and dh0 NULL (not written).
+ * The forward with hs set ([B, ceil(T / NGDN_REC_RUN), D] fp32; the state
+ * entering each run of NGDN_REC_RUN tokens) leaves there what the backward
+ * reads; hs is required in both. The backward takes the forward's inputs, hs,
+ * dy (strides dy_b, dy_t) and dfinal, and writes dx, df, dwz [B,T,D] in dtype
+ * and, fp32, ddt_bias [D], dA_log [H] and dh0. ws: ngdn_recurrence_ws(...)
+ * fp32, no initial contents. Sums over tokens are in a fixed order: the same
+ * inputs give the same bits. */
+#define NGDN_REC_RUN 16
+typedef struct ngdn_recurrence_args {
+  int32_t B, T, D, H, S;
+  int64_t x_b, x_t, f_b, f_t, w_b, w_t, dy_b, dy_t;
+  const void *x, *f, *wz;
+  const float *A_log, *dt_bias, *h0;
+  const int32_t* cu;
+  void* y;
+  float *final_state, *hs;
+  const void* dy;
+  const float* dfinal;
+  void *dx, *df, *dwz;
+  float *dA_log, *ddt_bias, *dh0, *ws;
+} ngdn_recurrence_args;
+int32_t ngdn_recurrence_fwd(int32_t dtype, const ngdn_recurrence_args* r, void* stream);
+int32_t ngdn_recurrence_bwd(int32_t dtype, const ngdn_recurrence_args* r, void* stream);
+/* fp32 values of ws for a forward (backward 0) or a backward (1). */
+int64_t ngdn_recurrence_ws(int32_t B, int32_t T, int32_t D, int32_t backward);
+/* One token of B sequences: the state h0 [B,D] in, final_state [B,D] out (may be
+ * the same array), y [B,D]; T, S, cu and the token strides are not read. */
+int32_t ngdn_recurrence_step(int32_t dtype, const ngdn_recurrence_args* r, void* stream);
 
 #ifdef __cplusplus
 }

@@ -20,7 +20,7 @@ NGDN_BF16 = 1
 # NGDN_VERSION of include/ngdn.h: the interface the signatures below describe.
 # The loader refuses a library of another version (working-tensor layouts and
 # argument meanings changed between versions under unchanged signatures).
-VERSION = 1100
+VERSION = 1200
 
 
 class Dims(ctypes.Structure):
@@ -34,6 +34,7 @@ P = ctypes.c_void_p
 I32 = ctypes.c_int32
 I64 = ctypes.c_int64
 WPARTS = 1024         # NGDN_WPARTS: rows of partial weight-gradient sums in the ws arguments
+REC_RUN = 16          # NGDN_REC_RUN: tokens a run of the gated recurrence's saved states
 PARAM_SPLIT = 16      # NGDN_PARAM_SPLIT: slices of firings per head in ngdn_param_grads
 PD = ctypes.POINTER(Dims)
 
@@ -82,8 +83,16 @@ SIGNATURES = {
     "ngdn_sum_f32": [I32, I32, P, I64, P, P],
     "ngdn_scale": [I32, I32, I64, P, P, P, P],
     "ngdn_cross_entropy": [I32, I64, I32, I32, P, P, P, P, I32, P],
+    "ngdn_embedding_fwd": [I32, I32, I64, I64, I32, ctypes.c_float, P, P, P, P],
+    "ngdn_embedding_bwd": [I32, I32, I64, I64, I32, ctypes.c_float, I64, P, P, P, P, P],
+    "ngdn_embedding_ws": [I64, I64, I32],
+    "ngdn_recurrence_fwd": [I32, P, P],
+    "ngdn_recurrence_bwd": [I32, P, P],
+    "ngdn_recurrence_step": [I32, P, P],
+    "ngdn_recurrence_ws": [I32, I32, I32, I32],
 }
-_RESTYPES = {"ngdn_last_error": ctypes.c_char_p, "ngdn_arch": ctypes.c_char_p}
+_RESTYPES = {"ngdn_last_error": ctypes.c_char_p, "ngdn_arch": ctypes.c_char_p,
+             "ngdn_embedding_ws": ctypes.c_int64, "ngdn_recurrence_ws": ctypes.c_int64}
 
 _lib = None
 _fns = {}             # entry point name -> the loaded library's function
@@ -170,6 +179,16 @@ class GateArgs(ctypes.Structure):
                     "q", "k", "f", "bz", "wz", "ml", "A_log", "dt_bias", "qn", "kn", "g0", "b0",
                     "w0", "mix", "dqn", "dkn", "dg0", "db0", "dw0", "dmix", "dq", "dk", "df",
                     "dbz", "dwz", "dml", "dpar", "ws")])
+
+
+class RecurrenceArgs(ctypes.Structure):
+    """ngdn_recurrence_args (include/ngdn.h)."""
+    _fields_ = ([(n, ctypes.c_int32) for n in ("B", "T", "D", "H", "S")] +
+                [(n, ctypes.c_int64) for n in ("x_b", "x_t", "f_b", "f_t", "w_b", "w_t", "dy_b",
+                                               "dy_t")] +
+                [(n, ctypes.c_void_p) for n in (
+                    "x", "f", "wz", "A_log", "dt_bias", "h0", "cu", "y", "final_state", "hs", "dy",
+                    "dfinal", "dx", "df", "dwz", "dA_log", "ddt_bias", "dh0", "ws")])
 
 
 def dims(B, T, H, L, K, V, dtype_code, scale, hold_partial=False):

@@ -1095,4 +1095,98 @@ int32_t ngdn_cross_entropy(int32_t dtype, int64_t rows, int32_t V, int32_t ignor
   return launched(ngdn::cross_entropy(a, dtype, (hipStream_t)stream), "ngdn_cross_entropy");
 }
 
+namespace {
+
+int32_t embed_sizes(int32_t d0, int32_t d1, int64_t N, int64_t V, int32_t D, const char* what) {
+  for (int32_t d : {d0, d1})
+    if (d != NGDN_F32 && d != NGDN_BF16) return fail(NGDN_EINVAL, "%s: dtype %d", what, d);
+  // positions and ids are kept in 32 bits; grids have a workgroup for at most 4 rows
+  if (N < 0 || V < 1 || D < 1 || N > (1LL << 24) || V > (1LL << 24) - 1 || D > (1 << 20))
+    return fail(NGDN_EINVAL, "%s: N=%lld V=%lld D=%d (0 <= N <= 2^24, 1 <= V < 2^24, 1 <= D <= 2^20)",
+                what, (long long)N, (long long)V, D);
+  return NGDN_OK;
+}
+
+int32_t rec_check(int32_t dtype, const ngdn_recurrence_args* r, const char* what) {
+  if (!r) return fail(NGDN_EINVAL, "%s: args is NULL", what);
+  if (dtype != NGDN_F32 && dtype != NGDN_BF16) return fail(NGDN_EINVAL, "%s: dtype %d", what, dtype);
+  if (r->B < 1 || r->D < 1 || r->H < 1 || r->D % r->H)
+    return fail(NGDN_EINVAL, "%s: B=%d D=%d H=%d (each >= 1, D a multiple of H)", what, r->B, r->D, r->H);
+  if (!r->x || !r->f || !r->wz || !r->A_log || !r->dt_bias)
+    return fail(NGDN_EINVAL, "%s: NULL tensor", what);
+  if ((long long)r->B * r->D > (1LL << 31) - 1)
+    return fail(NGDN_EINVAL, "%s: B*D = %lld exceeds 2^31 - 1", what, (long long)r->B * r->D);
+  return NGDN_OK;
+}
+
+int32_t rec_rows(const ngdn_recurrence_args* r, const char* what) {
+  if (r->T < 1) return fail(NGDN_EINVAL, "%s: T=%d", what, r->T);
+  if (!r->cu != !r->S || r->S < 0 || (r->cu && r->B != 1))
+    return fail(NGDN_EINVAL, "%s: S=%d B=%d (packed rows: cu, S >= 1 and B = 1; else S = 0)", what,
+                r->S, r->B);
+  if ((long long)r->S * r->D > (1LL << 31) - 1)
+    return fail(NGDN_EINVAL, "%s: S*D = %lld exceeds 2^31 - 1", what, (long long)r->S * r->D);
+  // the largest grid: 256 work-items for 4 runs of 64 channels
+  const long long groups = (r->D + 63) / 64 * ((((long long)r->T + NGDN_REC_RUN - 1) / NGDN_REC_RUN + 3) / 4) * r->B;
+  if (groups > (1LL << 24) - 1)
+    return fail(NGDN_EINVAL, "%s: %lld workgroups exceed %lld (B*T*D is too large)", what, groups,
+                (1LL << 24) - 1);
+  return NGDN_OK;
+}
+
+}  // namespace
+
+int32_t ngdn_embedding_fwd(int32_t w_dtype, int32_t y_dtype, int64_t N, int64_t V, int32_t D,
+                           float scale, const int64_t* ids, const void* w, void* y, void* stream) {
+  g_err[0] = 0;
+  if (int32_t r = embed_sizes(w_dtype, y_dtype, N, V, D, "ngdn_embedding_fwd")) return r;
+  if (N > 0 && (!ids || !w || !y)) return fail(NGDN_EINVAL, "ngdn_embedding_fwd: NULL tensor");
+  ngdn::EmbedArgs a{};
+  a.ids = reinterpret_cast<const long long*>(ids); a.w = w; a.y = y;
+  a.N = N; a.V = V; a.D = D; a.scale = scale;
+  return launched(ngdn::embed_fwd(a, w_dtype, y_dtype, (hipStream_t)stream), "ngdn_embedding_fwd");
+}
+
+int64_t ngdn_embedding_ws(int64_t N, int64_t V, int32_t D) { return ngdn::embed_ws(N, V, D); }
+
+int32_t ngdn_embedding_bwd(int32_t dy_dtype, int32_t w_dtype, int64_t N, int64_t V, int32_t D,
+                           float scale, int64_t padding_idx, const int64_t* ids, const void* dy,
+                           void* dw, int32_t* ws, void* stream) {
+  g_err[0] = 0;
+  if (int32_t r = embed_sizes(dy_dtype, w_dtype, N, V, D, "ngdn_embedding_bwd")) return r;
+  if (!dw || (N > 0 && (!ids || !dy || !ws))) return fail(NGDN_EINVAL, "ngdn_embedding_bwd: NULL tensor");
+  ngdn::EmbedArgs a{};
+  a.ids = reinterpret_cast<const long long*>(ids); a.dy = dy; a.dw = dw; a.ws = ws;
+  a.N = N; a.V = V; a.D = D; a.scale = scale; a.padding_idx = padding_idx;
+  return launched(ngdn::embed_bwd(a, dy_dtype, w_dtype, (hipStream_t)stream), "ngdn_embedding_bwd");
+}
+
+int64_t ngdn_recurrence_ws(int32_t B, int32_t T, int32_t D, int32_t backward) {
+  return ngdn::rec_ws(B, T, D, backward != 0);
+}
+
+int32_t ngdn_recurrence_fwd(int32_t dtype, const ngdn_recurrence_args* r, void* stream) {
+  g_err[0] = 0;
+  if (int32_t e = rec_check(dtype, r, "ngdn_recurrence_fwd")) return e;
+  if (int32_t e = rec_rows(r, "ngdn_recurrence_fwd")) return e;
+  if (!r->y || !r->hs || !r->ws) return fail(NGDN_EINVAL, "ngdn_recurrence_fwd: NULL tensor");
+  return launched(ngdn::rec_fwd(*r, dtype, (hipStream_t)stream), "ngdn_recurrence_fwd");
+}
+
+int32_t ngdn_recurrence_bwd(int32_t dtype, const ngdn_recurrence_args* r, void* stream) {
+  g_err[0] = 0;
+  if (int32_t e = rec_check(dtype, r, "ngdn_recurrence_bwd")) return e;
+  if (int32_t e = rec_rows(r, "ngdn_recurrence_bwd")) return e;
+  if (!r->hs || !r->ws || !r->dy || !r->dx || !r->df || !r->dwz || !r->dA_log || !r->ddt_bias)
+    return fail(NGDN_EINVAL, "ngdn_recurrence_bwd: NULL tensor");
+  return launched(ngdn::rec_bwd(*r, dtype, (hipStream_t)stream), "ngdn_recurrence_bwd");
+}
+
+int32_t ngdn_recurrence_step(int32_t dtype, const ngdn_recurrence_args* r, void* stream) {
+  g_err[0] = 0;
+  if (int32_t e = rec_check(dtype, r, "ngdn_recurrence_step")) return e;
+  if (!r->y || !r->h0 || !r->final_state) return fail(NGDN_EINVAL, "ngdn_recurrence_step: NULL tensor");
+  return launched(ngdn::rec_step(*r, dtype, (hipStream_t)stream), "ngdn_recurrence_step");
+}
+
 }  // extern "C"

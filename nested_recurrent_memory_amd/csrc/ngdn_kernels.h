@@ -491,4 +491,29 @@ struct L0BwdIntraArgs {
 hipError_t l0_bwd_intra(const L0BwdIntraArgs& a, int dtype, int K, int V, hipStream_t st);
 hipError_t l0_bwd_fused(const L0BwdIntraArgs& a, int dtype, int K, int V, hipStream_t st);
 
+// The gated linear recurrence (recurrence.hip); what each field holds is at
+// ngdn_recurrence_args in ngdn.h. Runs of REC_SEG tokens; the parameter
+// gradients' sums over runs are cut into REC_SLICES.
+using RecArgs = ngdn_recurrence_args;
+constexpr int REC_SEG = NGDN_REC_RUN;
+constexpr int REC_SLICES = 32;
+int64_t rec_ws(int64_t B, int64_t T, int64_t D, bool backward);
+hipError_t rec_fwd(const RecArgs& a, int dtype, hipStream_t st);
+hipError_t rec_bwd(const RecArgs& a, int dtype, hipStream_t st);
+hipError_t rec_step(const RecArgs& a, int dtype, hipStream_t st);
+
+// Embedding (embedding.hip): rows of a [V,D] table by id, times a scale, and
+// the table's gradient. Ids outside [0, V): a row of NaN, no gradient.
+struct EmbedArgs {
+  const long long* ids; const void* w; void* y;
+  const void* dy; void* dw; int* ws;
+  long long N, V;
+  int D;
+  float scale;
+  long long padding_idx;    // its row gets no gradient (negative: none)
+};
+int64_t embed_ws(int64_t N, int64_t V, int64_t D);
+hipError_t embed_fwd(const EmbedArgs& a, int w_dtype, int y_dtype, hipStream_t st);
+hipError_t embed_bwd(const EmbedArgs& a, int dy_dtype, int w_dtype, hipStream_t st);
+
 }  // namespace ngdn

@@ -1,6 +1,7 @@
-"""The three modules NestedGDN2ForCausalLM takes from fla
-(nested_gdn2/models/modeling_nested_gdn2.py:15-17), on the HIP kernels of
-libngdn.so (csrc/model_ops.hip, entry points in include/ngdn.h):
+"""The modules NestedGDN2ForCausalLM takes from fla
+(nested_gdn2/models/modeling_nested_gdn2.py:15-17) and its embedding, on the
+HIP kernels of libngdn.so (csrc/model_ops.hip, csrc/embedding.hip, entry
+points in include/ngdn.h):
 
 * ``RMSNorm``: y = x / sqrt(mean(x^2) + eps) * weight over the last dimension.
 * ``GatedMLP``: down_proj(silu(gate_proj x) * up_proj x), the SwiGLU on a
@@ -11,6 +12,8 @@ libngdn.so (csrc/model_ops.hip, entry points in include/ngdn.h):
   logits a block of rows at a time, the cross-entropy kernel turns them into
   their gradient in place, and dx, dW (and db) are formed right there; the
   backward only scales them by the incoming gradient.
+* ``Embedding``: torch's nn.Embedding with the lookup and its gradient on
+  kernels (``embedding``, which also takes a scale and an output type).
 
 Under autocast the GEMMs run in the autocast dtype (bfloat16), as
 nn.Linear's would; the kernels compute in fp32. There is no fallback: without
@@ -23,12 +26,13 @@ import contextlib
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from .layer_ops import fanout
 
-__all__ = ["RMSNorm", "GatedMLP", "FusedLinearCrossEntropyLoss", "rms_norm", "add_rms_norm",
-           "swiglu", "fused_linear_cross_entropy"]
+__all__ = ["RMSNorm", "GatedMLP", "FusedLinearCrossEntropyLoss", "Embedding", "rms_norm",
+           "add_rms_norm", "swiglu", "fused_linear_cross_entropy", "embedding"]
 
 
 def _code(t):
@@ -51,6 +55,115 @@ def _compute_dtype(x):
     if torch.is_autocast_enabled("cuda"):
         return torch.get_autocast_dtype("cuda")
     return x.dtype
+
+
+# ---------------------------------------------------------------- embedding
+
+_EMBED = (torch.bfloat16, torch.float32)                     # the kernels' types
+_TABLES = (torch.bfloat16, torch.float16, torch.float32)     # fp16 runs in fp32
+_EMBED_MOST = 1 << 24                                        # ids, and rows of the table
+
+
+def _embed_call(name, t, *args):
+    # on t's device, whichever is current: a launch needs its stream's device
+    if t.device.index == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream_of(t))
+    else:
+        with torch.cuda.device(t.device):
+            _lib.call(name, *args, _lib.stream_of(t))
+
+
+def _lookup(ids, weight, scale, ydt):
+    w = _work(weight).contiguous()
+    y = torch.empty(*ids.shape, w.shape[1], device=w.device, dtype=ydt if ydt in _EMBED else torch.float32)
+    if y.numel():
+        _embed_call("ngdn_embedding_fwd", w, _code(w), _code(y), ids.numel(), w.shape[0], w.shape[1],
+                    scale, _lib.ptr(ids), _lib.ptr(w), _lib.ptr(y))
+    return y.to(ydt)
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    """Linear in the table: the gradient is _EmbeddingGradFn, whose own is this."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx, ydt):
+        ctx.save_for_backward(ids)
+        ctx.cfg = (scale, padding_idx, weight.shape[0], weight.dtype)
+        return _lookup(ids, weight, scale, ydt)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        return None, _EmbeddingGradFn.apply(ids, dy, *ctx.cfg), None, None, None
+
+
+class _EmbeddingGradFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, dy, scale, padding_idx, V, wdt):
+        ctx.save_for_backward(ids)
+        ctx.cfg = (scale, padding_idx, dy.dtype)
+        g = _work(dy).contiguous()
+        N, D = ids.numel(), dy.shape[-1]
+        dw = torch.empty(V, D, device=g.device, dtype=wdt if wdt in _EMBED else torch.float32)
+        ws = torch.empty(_lib.lib().ngdn_embedding_ws(N, V, D), device=g.device, dtype=torch.int32)
+        _embed_call("ngdn_embedding_bwd", g, _code(g), _code(dw), N, V, D, scale,
+                    -1 if padding_idx is None else padding_idx, _lib.ptr(ids), _lib.ptr(g),
+                    _lib.ptr(dw), _lib.ptr(ws))
+        return dw.to(wdt)
+
+    @staticmethod
+    def backward(ctx, ddw):
+        ids, = ctx.saved_tensors
+        scale, padding_idx, gdt = ctx.cfg
+        if padding_idx is not None:
+            ddw = ddw.clone()
+            ddw[padding_idx] = 0
+        return None, _EmbeddingFn.apply(ids, ddw, scale, padding_idx, gdt), None, None, None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
+    """scale * weight[ids]: ids (int32 or int64, any shape) into the rows of
+    weight [V,D]; y [*ids.shape, D] in out_dtype (weight's own if None), one
+    rounding from fp32. An id outside [0, V) gives a row of NaN and no
+    gradient. The gradient for weight is dense, its sums in fp32 and in an
+    order that the ids fix; row ``padding_idx`` gets none."""
+    if (weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1
+            or weight.dtype not in _TABLES):
+        raise ValueError(f"embedding: weight {weight.dtype} {tuple(weight.shape)} (bf16, fp16 or "
+                         "fp32, [V,D])")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"embedding: ids are {ids.dtype} (int32 or int64)")
+    V = weight.shape[0]
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"embedding: padding_idx {padding_idx} outside the {V} rows of weight")
+        padding_idx %= V
+    ydt = weight.dtype if out_dtype is None else out_dtype
+    if ydt not in _TABLES:
+        raise ValueError(f"embedding: out_dtype {ydt} (bf16, fp16 or fp32)")
+    _on_gpu("embedding", weight, ids)
+    return _EmbeddingFn.apply(ids.to(torch.int64).contiguous(), weight, float(scale), padding_idx, ydt)
+
+
+class Embedding(nn.Embedding):
+    """nn.Embedding whose lookup on the GPU and its gradient are kernels of the
+    library. With max_norm, scale_grad_by_freq or sparse, off the GPU, for
+    tensor subclasses and under functorch, forward-mode differentiation or
+    tracing it is nn.Embedding's own."""
+
+    def forward(self, ids):
+        w = self.weight
+        plain = (w.is_cuda and ids.device == w.device and w.dim() == 2 and w.dtype in _TABLES
+                 and ids.dtype in (torch.int32, torch.int64) and type(ids) is torch.Tensor
+                 and type(w) in (torch.Tensor, nn.Parameter)
+                 and w.shape[0] < _EMBED_MOST and ids.numel() <= _EMBED_MOST
+                 and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse)
+        if (not plain or torch.compiler.is_compiling() or torch.jit.is_tracing()
+                or forward_ad._current_level >= 0
+                or torch._C._functorch.is_functorch_wrapped_tensor(w)
+                or torch._C._functorch.is_functorch_wrapped_tensor(ids)):
+            return super().forward(ids)
+        return embedding(ids, w, padding_idx=self.padding_idx)
 
 
 # ---------------------------------------------------------------- RMSNorm

@@ -1,0 +1,278 @@
+"""The embedding and its gradient against float64: the lookup is one product
+and one rounding, a row of the gradient a sum of m terms in fp32 (at most
+m + 2 roundings) rounded once."""
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import ngdn_recurrence_oracle as oracle
+from nested_recurrent_memory_amd import gated_recurrence, step_gated_recurrence
+from nested_recurrent_memory_amd.model_ops import Embedding, embedding, fused_linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def make(N, V, D, wdt, ydt, seed=0, zipf=False):
+    g = torch.Generator().manual_seed(seed * 31 + N * 101 + V * 7 + D)
+    if zipf:
+        p = 1.0 / torch.arange(1, V + 1)
+        ids = torch.multinomial(p, N, replacement=True, generator=g) if N else torch.zeros(0, dtype=torch.long)
+    else:
+        ids = torch.randint(0, V, (N,), generator=g)
+    return ids, torch.randn(V, D, generator=g).to(wdt), torch.randn(N, D, generator=g).to(ydt)
+
+
+def half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def least(dtype):
+    # below its smallest normal number 2^-14 fp16 has steps of 2^-24: half of one is 2^-25
+    return 2.0 ** -25 if dtype == torch.float16 else 1e-37
+
+
+def check_lookup(y, ids, w, scale, ydt):
+    want = oracle.embedding(ids, w, scale)
+    assert y.dtype == ydt and y.shape == want.shape
+    got = y.detach().double().cpu()
+    # the product's rounding to fp32, then the one to the type
+    assert ((got - want).abs() <= (half(ydt) + 2.0 ** -23) * want.abs() + least(ydt)).all()
+
+
+def check_grad(dw, ids, dy, V, scale, padding_idx=None):
+    want, bound = oracle.embedding_grad(ids, dy, V, scale, padding_idx)
+    h = half(dw.dtype) if dw.dtype != torch.float32 else 0.0
+    err = (dw.detach().double().cpu() - want).abs()
+    assert (err <= bound * (1 + h) + h * want.abs() + least(dw.dtype)).all(), (err - bound).max()
+
+
+@pytest.mark.parametrize("wdt,ydt", [(a, b) for a in DTYPES for b in DTYPES])
+@pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 5, 64), (3, 5, 7), (64, 32, 515), (65, 3, 1000), (257, 100, 8),
+                                   (1000, 300, 24), (300, 17, 1160)])
+def test_lookup_and_gradient(N, V, D, wdt, ydt):
+    ids, w, dy = make(N, V, D, wdt, ydt)
+    scale = D ** 0.5
+    wg = w.cuda().requires_grad_(True)
+    y = embedding(ids.cuda(), wg, scale=scale, out_dtype=ydt)
+    check_lookup(y, ids, w, scale, ydt)
+    dw, = torch.autograd.grad(y, wg, dy.cuda())
+    assert dw.dtype == wdt
+    check_grad(dw, ids, dy, V, scale)
+
+
+@pytest.mark.parametrize("N,V,D", [(5000, 50, 40), (9000, 7000, 64), (20000, 1, 9), (20000, 3, 130),
+                                   (40000, 12000, 16), (70000, 500, 8), (140000, 3000, 8)])
+@pytest.mark.parametrize("padding_idx", [None, 0, -1])
+def test_gradient_of_many_tokens(N, V, D, padding_idx):
+    """Ids as a tokenizer gives them (the frequent ones very frequent), all one
+    id, more ids than one workgroup sorts."""
+    ids, w, dy = make(N, V, D, torch.float32, torch.bfloat16, zipf=True)
+    wg = w.cuda().requires_grad_(True)
+    y = embedding(ids.cuda(), wg, padding_idx=padding_idx, out_dtype=torch.bfloat16)
+    dw, = torch.autograd.grad(y, wg, dy.cuda())
+    check_grad(dw, ids, dy, V, 1.0, None if padding_idx is None else padding_idx % V)
+
+
+def test_large_vocabulary():
+    """More than 2^16 rows and ids whose low and high bits both matter."""
+    V = 70000
+    g = torch.Generator().manual_seed(4)
+    ids = torch.cat((torch.randint(0, V, (3000,), generator=g), torch.tensor([0, V - 1, 65535, 65536, 255, 256]),
+                     torch.arange(0, V, 257)))
+    ids = ids[torch.randperm(len(ids), generator=g)]
+    dy = torch.randn(len(ids), 8, generator=g)
+    wg = torch.randn(V, 8, generator=g).cuda().requires_grad_(True)
+    dw, = torch.autograd.grad(embedding(ids.cuda(), wg), wg, dy.cuda())
+    check_grad(dw, ids, dy, V, 1.0)
+
+
+def test_ids_of_any_shape_and_type():
+    ids, w, _ = make(24, 9, 16, torch.float32, torch.float32)
+    wg = w.cuda()
+    for t in (ids.reshape(2, 3, 4), ids.reshape(4, 6).t(), ids[::2], ids.reshape(2, 12)[:, ::3], ids[3], ids[:0],
+              ids.to(torch.int32).reshape(6, 4)):
+        y = embedding(t.cuda(), wg)
+        assert torch.equal(y.cpu(), w[t.long()])
+    base = torch.zeros(9, 33).cuda()
+    base[:, 1:17] = wg
+    assert torch.equal(embedding(ids.cuda(), base[:, 1:17]).cpu(), w[ids])       # rows not aligned
+    flat = torch.zeros(9 * 16 + 1).cuda()
+    flat[1:] = wg.reshape(-1)
+    off = flat[1:].view(9, 16).requires_grad_(True)                              # data not aligned
+    y = embedding(ids.cuda(), off)
+    assert torch.equal(y.cpu(), w[ids])
+    check_grad(torch.autograd.grad(y.sum(), off)[0], ids, torch.ones(24, 16), 9, 1.0)
+
+
+def test_gradient_with_strides_and_expanded():
+    ids, w, _ = make(30, 9, 16, torch.float32, torch.float32)
+    wg = w.cuda().requires_grad_(True)
+    dy = torch.randn(16, 30)
+    y = embedding(ids.cuda(), wg)
+    check_grad(torch.autograd.grad(y, wg, dy.cuda().t(), retain_graph=True)[0], ids, dy.t(), 9, 1.0)
+    one = torch.randn(30, 1)
+    check_grad(torch.autograd.grad(y, wg, one.cuda().expand(30, 16))[0], ids, one.expand(30, 16), 9, 1.0)
+
+
+def test_ids_outside_the_table():
+    """Rows of NaN, no gradient, and nothing read outside the table."""
+    ids = torch.tensor([0, -1, 5, 3, 1 << 40, -(1 << 40), 4])
+    w, dy = torch.randn(5, 12), torch.randn(7, 12)
+    wg = w.cuda().requires_grad_(True)
+    y = embedding(ids.cuda(), wg, scale=2.0)
+    ok = (ids >= 0) & (ids < 5)
+    assert torch.isnan(y[~ok.cuda()]).all() and torch.equal(y[ok.cuda()].cpu(), 2 * w[ids[ok]])
+    check_grad(torch.autograd.grad(y, wg, dy.cuda())[0], ids, dy, 5, 2.0)
+
+
+def test_nan_of_one_token_stays_in_its_row():
+    ids = torch.tensor([2, 3, 2, 1]).cuda()
+    dy = torch.ones(4, 8).cuda()
+    dy[1, 3] = float("nan")
+    dy[3, 2] = float("inf")
+    wg = torch.zeros(5, 8, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(embedding(ids, wg, padding_idx=0), wg, dy)
+    want = torch.zeros(5, 8)
+    want[2], want[3], want[1] = 2, 1, 1
+    want[3, 3], want[1, 2] = float("nan"), float("inf")
+    assert torch.allclose(dw.cpu(), want, rtol=0, atol=0, equal_nan=True)
+    # a NaN at the padding row's tokens reaches nothing
+    dw, = torch.autograd.grad(embedding(ids, wg, padding_idx=3), wg, dy)
+    assert not dw[3].any() and not torch.isnan(dw).any()
+
+
+def test_gradient_is_linear_and_differentiates_again():
+    """The gradient of the gradient is the lookup of the incoming table."""
+    ids, w, dy = make(40, 9, 16, torch.float32, torch.float32)
+    wg = w.cuda().requires_grad_(True)
+    v = dy.cuda().requires_grad_(True)
+    y = embedding(ids.cuda(), wg, scale=3.0, padding_idx=2)
+    dw, = torch.autograd.grad(y, wg, v, create_graph=True)
+    t = torch.randn(9, 16, device="cuda")
+    dv, = torch.autograd.grad(dw, v, t)
+    t2 = t.clone()
+    t2[2] = 0
+    assert torch.equal(dv, 3.0 * t2[ids.cuda()])
+
+
+def test_same_bits_every_run():
+    ids, w, dy = make(60000, 5000, 64, torch.float32, torch.bfloat16, zipf=True)
+    wg = w.cuda().requires_grad_(True)
+    got = [torch.autograd.grad(embedding(ids.cuda(), wg, out_dtype=torch.bfloat16), wg, dy.cuda())[0]
+           for _ in range(3)]
+    assert torch.equal(got[0], got[1]) and torch.equal(got[0], got[2])
+
+
+@pytest.mark.parametrize("N", [100, 20000])
+def test_captured_in_a_graph(N):
+    """Lookup and gradient captured, replayed on new ids with eager work between."""
+    ids, w, dy = make(N, 700, 64, torch.float32, torch.float32)
+    sid, sw, sdy = ids.cuda(), w.cuda(), dy.cuda()
+
+    def work():
+        wg = sw.detach().requires_grad_(True)
+        y = embedding(sid, wg, scale=2.0)
+        return y.detach(), torch.autograd.grad(y, wg, sdy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = work()
+    for i in range(4):
+        new = make(N, 700, 64, torch.float32, torch.float32, seed=i + 1, zipf=i % 2 == 0)
+        sid.copy_(new[0])
+        sdy.copy_(new[2])
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, work())), i
+        check_grad(out[1], new[0], new[2], 700, 2.0)
+
+
+@pytest.mark.parametrize("padding_idx", [None, 3])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_module_is_nn_embedding(padding_idx, dtype):
+    """The module's lookup has nn.Embedding's bits; hooks and state dicts are
+    nn.Embedding's; what it does not take goes to nn.Embedding."""
+    torch.manual_seed(0)
+    m = Embedding(50, 24, padding_idx=padding_idx).cuda().to(dtype)
+    ref = torch.nn.Embedding(50, 24, padding_idx=padding_idx).cuda().to(dtype)
+    ref.load_state_dict(m.state_dict())
+    ids = torch.randint(0, 50, (4, 30), device="cuda")
+    seen = []
+    m.register_forward_hook(lambda mod, a, out: seen.append(out))
+    y = m(ids)
+    assert seen and torch.equal(y, ref(ids))
+    dy = torch.randn(4, 30, 24).to(dtype)
+    y.backward(dy.cuda())
+    check_grad(m.weight.grad, ids.cpu(), dy, 50, 1.0, padding_idx)
+    with torch.no_grad():
+        assert torch.equal(torch.func.vmap(lambda i: torch.func.functional_call(m, dict(m.named_parameters()), i))(
+            ids), ref(ids))
+    s = Embedding(50, 24, sparse=True).cuda()
+    s(ids).sum().backward()
+    assert s.weight.grad.is_sparse
+    n = Embedding(50, 24, max_norm=1.0).cuda()
+    assert (n(ids).norm(dim=-1) <= 1.0 + 1e-5).all()
+
+
+def test_a_recurrent_language_model_step():
+    """The operators as a model uses them: tokens -> scaled embedding -> gated
+    recurrence -> tied-shape head and loss, packed documents; every gradient
+    against float64 autograd. fp32 throughout: the loss's products are the
+    library's, so the bar is 2e-4 of a gradient's largest value. Then the
+    same tokens one by one through the step."""
+    torch.manual_seed(1)
+    V, D, T = 96, 32, 150
+    cu = [0, 60, 60, 140]
+    p = {"emb": torch.randn(V, D) * 0.05, "px": torch.randn(3 * D, D) * D ** -0.5, "A_log": torch.zeros(4),
+         "dt_bias": torch.full((D,), -3.0), "head": torch.randn(V, D) * 0.1}
+    ids, labels = torch.randint(0, V, (1, T)), torch.randint(0, V, (T,))
+    labels[140:] = -100
+
+    def forward(q, own):
+        if own:
+            h = embedding(ids.cuda(), q["emb"], scale=D ** 0.5)
+        else:
+            h = q["emb"][ids] * D ** 0.5
+        x, f, wz = (h @ q["px"].t()).split(D, -1)
+        if own:
+            y, _ = gated_recurrence(x, f, wz, q["A_log"], q["dt_bias"], cu_seqlens=torch.tensor(cu, device="cuda"))
+            return fused_linear_cross_entropy(y[0], labels.cuda(), q["head"])
+        rate = q["A_log"].exp().repeat_interleave(D // 4)
+        g = -rate * F.softplus(f + q["dt_bias"])
+        u = (-(2 * g).expm1()).sqrt() * torch.sigmoid(wz) * x
+        ys, s = [], None
+        for t in range(T):
+            if t in cu:
+                s = torch.zeros(D, dtype=h.dtype)
+            s = g[0, t].exp() * s + u[0, t]
+            ys.append(s if t < cu[-1] else torch.zeros_like(s))
+        return F.cross_entropy(torch.stack(ys) @ q["head"].t(), labels, ignore_index=-100)
+
+    got = {n: t.cuda().requires_grad_(True) for n, t in p.items()}
+    ref = {n: t.double().requires_grad_(True) for n, t in p.items()}
+    la, lb = forward(got, True), forward(ref, False)
+    la.backward()
+    lb.backward()
+    assert abs(la.item() - lb.item()) < 1e-5 * abs(lb.item())
+    for n in p:
+        a, b = got[n].grad.double().cpu(), ref[n].grad
+        assert (a - b).abs().max() <= 2e-4 * b.abs().max(), n
+    with torch.no_grad():
+        h = embedding(ids.cuda(), got["emb"], scale=D ** 0.5)
+        x, f, wz = (h @ got["px"].t()).split(D, -1)
+        y, _ = gated_recurrence(x, f, wz, got["A_log"], got["dt_bias"])
+        s = torch.zeros(1, D, device="cuda")
+        for t in range(20):
+            ht = embedding(ids[:, t].cuda(), got["emb"], scale=D ** 0.5)
+            yt, _ = step_gated_recurrence(*(ht @ got["px"].t()).split(D, -1), got["A_log"], got["dt_bias"], s,
+                                          inplace=True)
+            # one fp32 product of 32 terms in another order each side, through 20 tokens
+            assert (yt - y[:, t]).abs().max() < 1e-4

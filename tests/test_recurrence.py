@@ -1,0 +1,170 @@
+"""The gated linear recurrence's oracle and the refusals of its entry points
+and of the embedding's, on the CPU."""
+
+import ctypes
+
+import pytest
+import torch
+
+import ngdn_recurrence_oracle as oracle
+from nested_recurrent_memory_amd import _lib, gated_recurrence, step_gated_recurrence
+from nested_recurrent_memory_amd.model_ops import Embedding, embedding
+
+
+def _inputs(B=2, T=5, D=4, H=2, dtype=torch.float64):
+    g = torch.Generator().manual_seed(B * 1000 + T * 10 + D)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    return dict(x=r(B, T, D).to(dtype), f=r(B, T, D).to(dtype), wz=r(B, T, D).to(dtype),
+                A_log=r(H).to(dtype), dt_bias=(r(D) - 2).to(dtype))
+
+
+def _loss(p, h0, cu, dy, dfinal):
+    o = oracle.recurrence(p["x"], p["f"], p["wz"], p["A_log"], p["dt_bias"], h0, cu)
+    return (o["y"][0] * dy).sum() + (o["final"][0] * dfinal).sum()
+
+
+@pytest.mark.parametrize("cu", [None, [0, 0, 3, 3, 4], [1, 2, 5]])
+def test_oracle_gradients_are_differences(cu):
+    """Central differences of the float64 forward: step 1e-5, whose own error
+    is of the order of 1e-10 of the third derivatives plus 1e-11 of rounding."""
+    p = _inputs(B=1 if cu else 2)
+    rows = len(cu) - 1 if cu else 2
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)  # noqa: E731
+    h0, dfinal, dy = r(rows, 4), r(rows, 4), r(*p["x"].shape)
+    o = oracle.recurrence(*(p[n] for n in ("x", "f", "wz", "A_log", "dt_bias")), h0, cu, dy, dfinal)
+    for name, t in [*p.items(), ("initial_state", h0)]:
+        want = o["d" + name][0]
+        for i in range(t.numel()):
+            flat, keep = t.view(-1), t.view(-1)[i].item()
+            flat[i] = keep + 1e-5
+            up = _loss(p, h0, cu, dy, dfinal)
+            flat[i] = keep - 1e-5
+            down = _loss(p, h0, cu, dy, dfinal)
+            flat[i] = keep
+            assert abs((up - down) / 2e-5 - want.view(-1)[i]) < 1e-6, (name, i)
+
+
+def test_shapes_and_types_are_refused():
+    p = _inputs(dtype=torch.float32)
+    args = [p[n] for n in ("x", "f", "wz", "A_log", "dt_bias")]
+
+    def bad(match, i=None, t=None, fn=gated_recurrence, **kw):
+        a = list(args)
+        if i is not None:
+            a[i] = t
+        with pytest.raises(ValueError, match=match):
+            fn(*a, **kw)
+
+    bad("x ", 0, p["x"][:, 0])
+    bad("x ", 1, p["f"][:, :3])
+    bad("x ", 2, p["wz"][..., :2])
+    bad("A_log", 3, torch.zeros(3))
+    bad("A_log", 3, torch.zeros(2, 2))
+    bad("dt_bias", 4, torch.zeros(5))
+    bad("f is", 1, p["f"].double())
+    bad("x is", 0, p["x"].long())
+    bad("initial_state", initial_state=torch.zeros(3, 4))
+    bad("cu_seqlens", cu_seqlens=torch.tensor([0, 5]))                     # B = 2
+    one = [p[n][:1] for n in ("x", "f", "wz")] + args[3:]
+    for cu in (torch.tensor([0.0, 5.0]), torch.tensor([[0, 5]]), torch.zeros(0, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            gated_recurrence(*one, cu_seqlens=cu)
+    with pytest.raises(ValueError, match="initial_state"):
+        gated_recurrence(*one, cu_seqlens=torch.tensor([0, 2, 5]), initial_state=torch.zeros(1, 4))
+    bad("no CPU path")
+    tok = [t[:, 0] for t in args[:3]] + args[3:]
+    with pytest.raises(ValueError, match="state"):
+        step_gated_recurrence(*tok, torch.zeros(2, 3))
+    with pytest.raises(ValueError, match="no CPU path"):
+        step_gated_recurrence(*tok, torch.zeros(2, 4))
+    with pytest.raises(ValueError, match="x "):
+        step_gated_recurrence(*args, torch.zeros(2, 4))
+
+
+def test_embedding_arguments_are_refused():
+    w, ids = torch.zeros(5, 4), torch.tensor([0, 1])
+    for bad in (dict(ids=ids.float()), dict(ids=ids.to(torch.int16)), dict(weight=w[0]),
+                dict(weight=w.double()), dict(weight=w.long()), dict(padding_idx=5),
+                dict(padding_idx=-6), dict(out_dtype=torch.float64), dict(weight=w[:0]),
+                dict(weight=w[:, :0])):
+        with pytest.raises(ValueError, match="embedding:"):
+            embedding(**{"ids": ids, "weight": w, **bad})
+    with pytest.raises(ValueError, match="no CPU path"):
+        embedding(ids, w)
+
+
+def test_embedding_module_off_the_gpu_is_torchs():
+    """The module in place of nn.Embedding keeps what nn.Embedding does off the
+    GPU, gradients included, and its state dict."""
+    m = Embedding(6, 3, padding_idx=2)
+    ref = torch.nn.Embedding(6, 3, padding_idx=2)
+    ref.load_state_dict(m.state_dict())
+    ids = torch.tensor([[0, 2, 5], [5, 1, 2]])
+    (m(ids) ** 2).sum().backward()
+    (ref(ids) ** 2).sum().backward()
+    assert torch.equal(m(ids), ref(ids)) and torch.equal(m.weight.grad, ref.weight.grad)
+
+
+FAKE = [ctypes.c_void_p(4096 * (i + 1)) for i in range(8)]
+
+
+def _args(**kw):
+    a = _lib.RecurrenceArgs()
+    a.B, a.T, a.D, a.H = 1, 16, 8, 2
+    for n in ("x", "f", "wz", "A_log", "dt_bias", "h0", "y", "final_state", "hs", "dy", "dx", "df", "dwz",
+              "dA_log", "ddt_bias", "ws"):
+        setattr(a, n, 4096)
+    for n, v in kw.items():
+        setattr(a, n, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(D=0), "D=0"), (dict(H=3), "multiple of H"), (dict(B=0), "B=0"), (dict(T=0), "T=0"),
+    (dict(x=None), "NULL"), (dict(hs=None), "NULL"), (dict(ws=None), "NULL"),
+    (dict(S=2), "packed"), (dict(cu=4096), "packed"), (dict(cu=4096, S=2, B=2), "packed"),
+    (dict(B=2, D=1 << 30, H=1), "exceeds"), (dict(cu=4096, S=1 << 30), "exceeds"),
+    (dict(B=1, T=1 << 30, D=1 << 20, H=1), "workgroups"),
+])
+def test_recurrence_entry_points_refuse_before_any_launch(kw, word):
+    so = _lib.lib()
+    a = _args(**kw)
+    for name in ("ngdn_recurrence_fwd", "ngdn_recurrence_bwd"):
+        assert getattr(so, name)(1, ctypes.byref(a), None) == 1
+        assert word.encode() in so.ngdn_last_error(), so.ngdn_last_error()
+    assert so.ngdn_recurrence_fwd(7, ctypes.byref(a), None) == 1
+    assert so.ngdn_recurrence_fwd(1, None, None) == 1 and b"NULL" in so.ngdn_last_error()
+
+
+def test_step_and_embedding_entry_points_refuse_before_any_launch():
+    so = _lib.lib()
+    a = _args(h0=None)
+    assert so.ngdn_recurrence_step(1, ctypes.byref(a), None) == 1 and b"NULL" in so.ngdn_last_error()
+    p = FAKE
+    for N, V, D, t in ((-1, 4, 4, 0), (4, 0, 4, 0), (4, 4, 0, 0), (4, 4, 4, 3), ((1 << 24) + 1, 4, 4, 0),
+                       (4, 1 << 24, 4, 0)):
+        assert so.ngdn_embedding_fwd(t, 0, N, V, D, 1.0, p[0], p[1], p[2], None) == 1
+        assert so.ngdn_embedding_bwd(t, 0, N, V, D, 1.0, -1, p[0], p[1], p[2], p[3], None) == 1
+    assert so.ngdn_embedding_fwd(0, 0, 4, 4, 4, 1.0, None, p[1], p[2], None) == 1
+    assert b"NULL" in so.ngdn_last_error()
+    assert so.ngdn_embedding_bwd(0, 0, 4, 4, 4, 1.0, -1, p[0], p[1], p[2], None, None) == 1
+
+
+def test_recurrence_struct_matches_header():
+    """The ctypes mirror of ngdn_recurrence_args has the header's fields, in
+    order and with the header's types."""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include",
+                             "ngdn.h")).read()
+    body = re.search(r"typedef struct ngdn_recurrence_args \{(.*?)\}", text, re.S).group(1)
+    fields = []
+    for decl in filter(None, (d.strip() for d in body.split(";"))):
+        ty, names = re.match(r"((?:const )?\w+)\s*(.*)", decl, re.S).groups()
+        for n in names.split(","):
+            n = n.strip()
+            fields.append((n.lstrip("* "), "ptr" if n.startswith("*") else ty))
+    ct = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "ptr": ctypes.c_void_p}
+    assert [(n, ct[t]) for n, t in fields] == list(_lib.RecurrenceArgs._fields_)
+    assert int(re.search(r"#define NGDN_REC_RUN (\d+)", text).group(1)) == _lib.REC_RUN
