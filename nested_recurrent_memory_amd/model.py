@@ -28,7 +28,8 @@ from transformers.modeling_utils import PreTrainedModel
 
 from .layer import NestedGDN2Attention
 from .layer_ops import FusedRMSNormGated, ShortConvolution
-from .model_ops import FusedLinearCrossEntropyLoss, GatedMLP, RMSNorm, add_rms_norm, rms_norm
+from .model_ops import (Embedding, FusedLinearCrossEntropyLoss, GatedMLP, RMSNorm, add_rms_norm,
+                        rms_norm)
 
 __all__ = ["NestedGDN2Config", "NestedGDN2Cache", "NestedGDN2Block", "NestedGDN2Model",
            "NestedGDN2ForCausalLM", "NestedGDN2PreTrainedModel"]
@@ -207,7 +208,7 @@ class NestedGDN2PreTrainedModel(PreTrainedModel):
 class NestedGDN2Model(NestedGDN2PreTrainedModel):
     def __init__(self, config):
         super().__init__(config)
-        self.embeddings = nn.Embedding(config.vocab_size, config.hidden_size)
+        self.embeddings = Embedding(config.vocab_size, config.hidden_size)
         self.layers = nn.ModuleList(NestedGDN2Block(config, i) for i in range(config.num_hidden_layers))
         self.norm = (RMSNorm if config.fuse_norm else nn.RMSNorm)(config.hidden_size,
                                                                   eps=config.norm_eps)
