@@ -1126,11 +1126,11 @@ int32_t rec_rows(const ngdn_recurrence_args* r, const char* what) {
                 r->S, r->B);
   if ((long long)r->S * r->D > (1LL << 31) - 1)
     return fail(NGDN_EINVAL, "%s: S*D = %lld exceeds 2^31 - 1", what, (long long)r->S * r->D);
-  // the largest grid: 256 work-items for 4 runs of 64 channels
-  const long long groups = (r->D + 63) / 64 * ((((long long)r->T + NGDN_REC_RUN - 1) / NGDN_REC_RUN + 3) / 4) * r->B;
-  if (groups > (1LL << 24) - 1)
-    return fail(NGDN_EINVAL, "%s: %lld workgroups exceed %lld (B*T*D is too large)", what, groups,
-                (1LL << 24) - 1);
+  // the backward's grid: 512 work-items for 64 tokens of 64 channels at least
+  const long long tiles = (r->D + 63LL) / 64 * ((r->T + 63LL) / 64) * r->B;
+  if (tiles > (1LL << 23) - 1)
+    return fail(NGDN_EINVAL, "%s: %lld workgroups exceed %lld (B*T*D is too large)", what, tiles,
+                (1LL << 23) - 1);
   return NGDN_OK;
 }
 

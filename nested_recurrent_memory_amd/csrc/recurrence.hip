@@ -9,8 +9,9 @@
 //   d dt_bias = sum df, d A_log = sum dg g.
 // Everything between loads and stores is fp32. The recurrence is linear, so a
 // run of tokens acts on the state before it as h -> A h + H with A = prod a;
-// runs of SEG tokens are reduced to (A, H), joined in order, and then formed
-// from the state that enters them.
+// runs are formed from zero in registers, joined in order, and completed from
+// the state that enters them.
+#include <algorithm>
 #include <initializer_list>
 
 #include "ngdn_kernels.h"
@@ -108,7 +109,7 @@ struct Run {
   unsigned start, end, used;
   int cur, last;
 };
-__device__ __forceinline__ Run run_of(const int* cu, int S, int t0, int n, int T) {
+__device__ Run run_of(const int* cu, int S, int t0, int n, int T) {
   Run r{0u, 0u, 0u, 0, 0};
   int lo = 0, hi = S + 1;                  // first boundary at or behind t0
   while (lo < hi) {
@@ -130,6 +131,14 @@ __device__ __forceinline__ Run run_of(const int* cu, int S, int t0, int n, int T
   r.last = s - 1;
   return r;
 }
+__device__ __forceinline__ int4 pack(const Run& r) {
+  return make_int4((int)(r.start | r.end << 16), (int)r.used, r.cur, r.last);
+}
+__device__ __forceinline__ Run unpack(const int4& v) {
+  const unsigned m = __builtin_amdgcn_readfirstlane(v.x);
+  return Run{m & 0xffffu, m >> 16, (unsigned)__builtin_amdgcn_readfirstlane(v.y),
+             __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w)};
+}
 // the sequence that token t starts: the last one with that boundary, from
 // sequence cur on
 __device__ __forceinline__ int seq_from(const int* cu, int S, int cur, int t) {
@@ -143,29 +152,6 @@ __device__ __forceinline__ int seq_before(const int* cu, int S, int cur, int t) 
   return cur < S ? cur : S - 1;
 }
 
-// One thread's VEC channels of one run.
-struct Place {
-  int b, seg, t0, n;
-  long long d;
-  bool live;
-};
-template <int VEC>
-__device__ __forceinline__ Place place(const RecArgs& a) {
-  const int nseg = (a.T + SEG - 1) / SEG, strips = (a.D + 64 * VEC - 1) / (64 * VEC);
-  const long long quads = (nseg + 3) / 4;
-  long long k = blockIdx.x;
-  Place p;
-  const int strip = (int)(k % strips);
-  k /= strips;
-  p.seg = (int)(k % quads) * 4 + wave_id();
-  p.b = (int)(k / quads);
-  p.t0 = p.seg * SEG;
-  p.n = a.T - p.t0 < SEG ? a.T - p.t0 : SEG;
-  p.d = (long long)strip * 64 * VEC + lane_id() * VEC;
-  p.live = p.seg < nseg && p.d < a.D;
-  return p;
-}
-
 template <int VEC>
 __device__ __forceinline__ void params(const RecArgs& a, long long d, float* bias2, float* nrate) {
   const int per = a.D / a.H;
@@ -176,263 +162,472 @@ __device__ __forceinline__ void params(const RecArgs& a, long long d, float* bia
   }
 }
 
+// ---------------------------------------------------------------- joining runs
+//
+// A workgroup has W waves, each a run of tokens of 64 VEC channels: a tile of
+// W runs. The state that enters a tile comes from the tiles before it (in the
+// backward: behind it) while those are still running, through device memory:
+// every tile publishes its (A, H) as soon as it has them; every GROUP-th also
+// the state behind it. A tile takes the state at its group's start and the
+// (A, H) of the tiles between, so the chain over a long row has a link every
+// GROUP tiles, and the order of the arithmetic does not depend on timing.
+// One 64-bit (32-bit) value is its own flag: all bits set before it is
+// published, which no published value has (a NaN of that pattern is changed).
+// Tiles are handed out by a counter, so all a tile waits for was started
+// before it and waits only for tiles before itself: every wait ends.
+// Against reducing, joining and applying in three launches: inputs are read
+// and their gates computed once instead of twice.
+
+constexpr int W = REC_WAVES;
+constexpr int GROUP = 2 * W;
+
+struct Sync {
+  unsigned* ticket;                 // NULL: one tile a row, nothing to join
+  unsigned long long* agg;          // [nchunk][nstrip][64 VEC] (A, H)
+  unsigned* base;                   // [nchunk / GROUP + 1][nstrip][64 VEC]
+  const int4* runs;                 // packed rows: every run's Run
+  int nchunk, nstrip, strips;       // nstrip = B strips
+};
+
+__device__ __forceinline__ unsigned bits(float x) { return __float_as_uint(x); }
+constexpr unsigned RESET = 0x80000000u;      // A = -0: nothing before passes (a >= +0 is never it)
+
+// (A2, H2) after (A1, H1); a reset keeps what is not finite before it out
+template <bool PACKED>
+__device__ __forceinline__ void join(float& A1, float& H1, float A2, float H2) {
+  if (PACKED && bits(A2) == RESET) {
+    A1 = A2;
+    H1 = H2;
+  } else {
+    H1 = fmaf(A2, H1, H2);
+    A1 = PACKED && bits(A1) == RESET ? A1 : A1 * A2;
+  }
+}
+template <bool PACKED>
+__device__ __forceinline__ float pass(float h, float A, float H) {
+  return PACKED && bits(A) == RESET ? H : fmaf(A, h, H);
+}
+
+__device__ __forceinline__ void publish(unsigned long long* p, float A, float H) {
+  const unsigned a = bits(A) == ~0u ? 0x7fc00000u : bits(A);
+  __hip_atomic_store(p, (unsigned long long)a << 32 | bits(H), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void publish(unsigned* p, float h) {
+  __hip_atomic_store(p, bits(h) == ~0u ? 0x7fc00000u : bits(h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename U>
+__device__ __forceinline__ U await(const U* p) {
+  U v;
+  while ((v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == (U)~(U)0)
+    __builtin_amdgcn_s_sleep(1);
+  return v;
+}
+
+template <int VEC>
+struct Joint {
+  float2 wave[W][64 * VEC];         // (A, H) of the tile's waves, in the order of the scan
+  float2 before[W][64 * VEC];       // of up to GROUP / W tiles before it each
+  float base[64 * VEC];
+};
+
+// From wave (A, H) to the state h entering the wave. step: the tile's place in
+// the scan's order (0 first), wv the wave's. first: the state entering tile 0.
+template <bool PACKED, int VEC>
+__device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int step, int strip, int wv,
+                                           const float* A, const float* H, const float* first, float* h) {
+  const int l = lane_id();
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) s.wave[wv][l * VEC + i] = make_float2(A[i], H[i]);
+  lds_barrier();
+  const int g0 = step / GROUP * GROUP, n = step - g0;      // tiles between the group's start and this one
+  const bool more = y.ticket != nullptr;
+  auto agg = [&](int k) { return y.agg + ((long long)k * y.nstrip + strip) * (64 * VEC) + l * VEC; };
+  auto base = [&](int k) { return y.base + ((long long)k * y.nstrip + strip) * (64 * VEC) + l * VEC; };
+  float tA[VEC], tH[VEC];                                   // the whole tile
+  if (more && wv == W - 1 && step + 1 < y.nchunk) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      tA[i] = 1.f;
+      tH[i] = 0.f;
+      for (int k = 0; k < W; ++k) {
+        const float2 v = s.wave[k][l * VEC + i];
+        join<PACKED>(tA[i], tH[i], v.x, v.y);
+      }
+      publish(agg(step) + i, tA[i], tH[i]);
+    }
+  }
+  if (more && step > 0) {
+    // wave wv: tiles g0 + 2 wv and + 1 of the n before; the last wave is never
+    // needed for them when n < GROUP - 1, and takes the state at g0 too
+    float bA[VEC], bH[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) { bA[i] = 1.f; bH[i] = 0.f; }
+    for (int k = wv * (GROUP / W); k < (wv + 1) * (GROUP / W) && k < n; ++k) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const unsigned long long v = await(agg(g0 + k) + i);
+        join<PACKED>(bA[i], bH[i], __uint_as_float((unsigned)(v >> 32)), __uint_as_float((unsigned)v));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s.before[wv][l * VEC + i] = make_float2(bA[i], bH[i]);
+    if (wv == W - 1) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        s.base[l * VEC + i] = g0 > 0 ? __uint_as_float(await(base(g0 / GROUP) + i)) : first[i];
+    }
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      h[i] = s.base[l * VEC + i];
+      for (int k = 0; k * (GROUP / W) < n; ++k) {
+        const float2 v = s.before[k][l * VEC + i];
+        h[i] = pass<PACKED>(h[i], v.x, v.y);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) h[i] = first[i];
+  }
+  if (more && wv == W - 1 && n == GROUP - 1 && step + 1 < y.nchunk) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) publish(base(g0 / GROUP + 1) + i, pass<PACKED>(h[i], tA[i], tH[i]));
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    for (int k = 0; k < wv; ++k) {
+      const float2 v = s.wave[k][l * VEC + i];
+      h[i] = pass<PACKED>(h[i], v.x, v.y);
+    }
+  }
+}
+
+__device__ __forceinline__ unsigned take(const Sync& y, unsigned* s_tile) {
+  if (!y.ticket) return blockIdx.x;
+  if (threadIdx.x == 0)
+    *s_tile = __hip_atomic_fetch_add(y.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(*s_tile);
+}
+
+// Before either pass: the flags' patterns, the counter, where the boundaries of
+// packed sequences fall in each run of `len` tokens, and sequences without
+// tokens (out = in or 0: their final state is their initial one, their initial
+// state's gradient the final one's).
+__global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long long n16, unsigned* ticket,
+                                                int4* runs, int len, const float* in, float* out) {
+  const long long i0 = (long long)blockIdx.x * 256 + threadIdx.x, step = (long long)gridDim.x * 256;
+  if (i0 == 0 && ticket) *ticket = 0;
+  for (long long i = i0; i < n16; i += step) fill[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
+  if (!a.cu) return;
+  const int nrun = (a.T + len - 1) / len;
+  for (long long i = i0; i < nrun; i += step) {
+    const int t0 = (int)i * len;
+    runs[i] = pack(run_of(a.cu, a.S, t0, a.T - t0 < len ? a.T - t0 : len, a.T));
+  }
+  if (!out) return;
+  for (long long c = i0; c < (long long)a.S * a.D; c += step) {
+    const long long s = c / a.D;
+    const int lo = a.cu[s] < a.T ? a.cu[s] : a.T, hi = a.cu[s + 1] < a.T ? a.cu[s + 1] : a.T;
+    if (lo >= hi) out[c] = in ? in[c] : 0.f;
+  }
+}
+
+template <typename E, int VEC>
+struct alignas(VEC * sizeof(E)) Raw { E v[VEC]; };
+
 }  // namespace
 
 // ---------------------------------------------------------------- forward
 
-// (A, H) of every run.
-template <typename E, int VEC>
-__global__ __launch_bounds__(256) void rec_reduce_fwd(RecArgs a) {
-  const Place p = place<VEC>(a);
-  if (!p.live) return;
-  float bias2[VEC], nrate[VEC], A[VEC], H[VEC];
-  params<VEC>(a, p.d, bias2, nrate);
-  Run r{0u, 0u, ~0u, 0, 0};
-  if (a.cu) r = run_of(a.cu, a.S, p.t0, p.n, a.T);
-  int cur = r.cur;
+// A wave has FSEG tokens of 64 VEC channels in registers: their gates, then
+// within the run h_t = H_t + P_t h_in from one pass, then y.
+template <typename E, int VEC, bool PACKED>
+__global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) {
+  constexpr int N = REC_FSEG;
+  __shared__ Joint<VEC> s_join;
+  __shared__ unsigned s_tile;
+  const unsigned tile = take(sy, &s_tile);
+  const int strip = tile % sy.nstrip, chunk = tile / sy.nstrip, wv = wave_id();
+  const int b = strip / sy.strips;
+  const long long d = (long long)(strip % sy.strips) * 64 * VEC + lane_id() * VEC;
+  const bool live = d < a.D;
+  const long long dl = live ? d : 0;                  // lanes behind D load channel 0, store nothing
+  const int t0 = (chunk * W + wv) * N, n = a.T - t0 < N ? a.T - t0 : N;     // n <= 0: no token
+  using R = Raw<E, VEC>;
+  const E* xp = static_cast<const E*>(a.x) + b * a.x_b + dl;
+  const E* fp = static_cast<const E*>(a.f) + b * a.f_b + dl;
+  const E* wp = static_cast<const E*>(a.wz) + b * a.w_b + dl;
+  R x[N], f[N], w[N];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) { A[i] = 1.f; H[i] = 0.f; }
-  for (int j = 0; j < p.n; ++j) {
-    const long long t = p.t0 + j;
-    float x[VEC], f[VEC], w[VEC];
-    loadv<E, VEC>(static_cast<const E*>(a.x) + p.b * a.x_b + t * a.x_t + p.d, x);
-    loadv<E, VEC>(static_cast<const E*>(a.f) + p.b * a.f_b + t * a.f_t + p.d, f);
-    loadv<E, VEC>(static_cast<const E*>(a.wz) + p.b * a.w_b + t * a.w_t + p.d, w);
-    const bool st = r.start >> j & 1, us = r.used >> j & 1;
-    if (st) cur = seq_from(a.cu, a.S, cur, (int)t);
+  for (int j = 0; j < N; ++j) {
+    const long long t = t0 + j < a.T ? t0 + j : a.T - 1;
+    x[j] = *reinterpret_cast<const R*>(xp + t * a.x_t);
+    f[j] = *reinterpret_cast<const R*>(fp + t * a.f_t);
+    w[j] = *reinterpret_cast<const R*>(wp + t * a.w_t);
+  }
+  float bias2[VEC], nrate[VEC], first[VEC];
+  params<VEC>(a, dl, bias2, nrate);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) first[i] = a.h0 && !PACKED ? a.h0[(long long)b * a.D + dl + i] : 0.f;
+  Run r{0u, 0u, 0u, 0, 0};
+  if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
+  float P[N][VEC], H[N][VEC];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const Decay k = decay(f[i], bias2[i], nrate[i]);
-      float beta, inv;
-      root(k.q, beta, inv);
-      float u = beta * sigmoid2(w[i]) * x[i], keep = k.a;
-      if (st) {
-        if (a.h0 && us) u += k.a * a.h0[(long long)cur * a.D + p.d + i];
-        keep = 0.f;
+      const Decay k = decay(to_f(f[j].v[i]), bias2[i], nrate[i]);
+      P[j][i] = k.a;
+      H[j][i] = __builtin_amdgcn_sqrtf(k.q) * sigmoid2(to_f(w[j].v[i])) * to_f(x[j].v[i]);
+    }
+  }
+  if (n < N) {                                        // behind the row: the state passes
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j >= n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) { P[j][i] = 1.f; H[j][i] = 0.f; }
+  }
+  // the first token that the state before the run does not reach
+  int cut = N;
+  if (PACKED) {
+    const unsigned stop = r.start | (~r.used & ((1u << N) - 1));
+    if (stop) cut = __builtin_ctz(stop);
+    int cur = r.cur;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const bool st = r.start >> j & 1, us = r.used >> j & 1;
+      if (st || !us) {
+        if (st) cur = seq_from(a.cu, a.S, cur, t0 + j);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float h = a.h0 && st && us ? a.h0[(long long)cur * a.D + dl + i] : 0.f;
+          H[j][i] = us ? fmaf(P[j][i], h, H[j][i]) : 0.f;
+          P[j][i] = 0.f;
+        }
+      } else if (j > 0) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          H[j][i] = fmaf(P[j][i], H[j - 1][i], H[j][i]);
+          P[j][i] *= P[j - 1][i];
+        }
       }
-      if (!us) { u = 0.f; keep = 0.f; H[i] = 0.f; }
-      H[i] = st ? u : keep * H[i] + u;
-      A[i] *= keep;
     }
-  }
-  const long long nseg = (a.T + SEG - 1) / SEG;
-  const long long o = ((long long)p.b * nseg + p.seg) * a.D + p.d;
+  } else {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    a.ws[o + i] = A[i];
-    a.hs[o + i] = H[i];
-  }
-}
-
-// The state entering every run (hs: H in, the state out), and for rows that
-// are not packed the final state.
-__global__ __launch_bounds__(64) void rec_carry_fwd(RecArgs a) {
-  const long long c = (long long)blockIdx.x * 64 + threadIdx.x;
-  if (c >= (long long)a.B * a.D) return;
-  const long long b = c / a.D, d = c % a.D, nseg = (a.T + SEG - 1) / SEG;
-  float h = (a.h0 && !a.cu) ? a.h0[c] : 0.f;
-  for (long long s = 0; s < nseg; ++s) {
-    const long long o = (b * nseg + s) * a.D + d;
-    const float H = a.hs[o];
-    a.hs[o] = h;
-    const float A = a.ws[o];
-    h = A == 0.f ? H : A * h + H;
-  }
-  if (a.final_state && !a.cu) a.final_state[c] = h;
-}
-
-// Every token from the state entering its run.
-template <typename E, int VEC>
-__global__ __launch_bounds__(256) void rec_apply_fwd(RecArgs a) {
-  const Place p = place<VEC>(a);
-  if (!p.live) return;
-  float bias2[VEC], nrate[VEC], h[VEC];
-  params<VEC>(a, p.d, bias2, nrate);
-  const long long nseg = (a.T + SEG - 1) / SEG;
+    for (int j = 1; j < N; ++j)
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) h[i] = a.hs[(p.b * nseg + p.seg) * a.D + p.d + i];
-  Run r{0u, 0u, ~0u, 0, 0};
-  if (a.cu) r = run_of(a.cu, a.S, p.t0, p.n, a.T);
-  int cur = r.cur;
-  for (int j = 0; j < p.n; ++j) {
-    const long long t = p.t0 + j;
-    float x[VEC], f[VEC], w[VEC], y[VEC];
-    loadv<E, VEC>(static_cast<const E*>(a.x) + p.b * a.x_b + t * a.x_t + p.d, x);
-    loadv<E, VEC>(static_cast<const E*>(a.f) + p.b * a.f_b + t * a.f_t + p.d, f);
-    loadv<E, VEC>(static_cast<const E*>(a.wz) + p.b * a.w_b + t * a.w_t + p.d, w);
-    const bool st = r.start >> j & 1, us = r.used >> j & 1, en = r.end >> j & 1;
-    if (st) cur = seq_from(a.cu, a.S, cur, (int)t);
+      for (int i = 0; i < VEC; ++i) {
+        H[j][i] = fmaf(P[j][i], H[j - 1][i], H[j][i]);
+        P[j][i] *= P[j - 1][i];
+      }
+  }
+  float h[VEC], A[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const Decay k = decay(f[i], bias2[i], nrate[i]);
-      float beta, inv;
-      root(k.q, beta, inv);
-      const float u = beta * sigmoid2(w[i]) * x[i];
-      if (st) h[i] = (a.h0 && us) ? a.h0[(long long)cur * a.D + p.d + i] : 0.f;
-      h[i] = us ? k.a * h[i] + u : 0.f;
-      if (en && a.final_state) a.final_state[(long long)cur * a.D + p.d + i] = h[i];
-      y[i] = h[i];
+  for (int i = 0; i < VEC; ++i) A[i] = PACKED && cut < N ? __uint_as_float(RESET) : P[N - 1][i];
+  join_tiles<PACKED, VEC>(s_join, sy, chunk, strip, wv, A, H[N - 1], first, h);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    if (!PACKED || j < cut)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) H[j][i] = fmaf(P[j][i], h[i], H[j][i]);
+  }
+  if (n <= 0 || !live) return;
+  if (a.hs) {                                         // the states entering runs of SEG tokens
+    const long long nrun = (a.T + SEG - 1) / SEG;
+#pragma unroll
+    for (int j = 0; j < N; j += SEG)
+      if (j < n) storev<float, VEC>(a.hs + (b * nrun + (t0 + j) / SEG) * a.D + d, j ? H[j ? j - 1 : 0] : h);
+  }
+  E* yp = static_cast<E*>(a.y) + ((long long)b * a.T + t0) * a.D + d;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < n) storev<E, VEC>(yp + (long long)j * a.D, H[j]);
+  if (!a.final_state) return;
+  if (PACKED) {
+    if (!r.end) return;
+    int cur = r.cur;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (r.start >> j & 1) cur = seq_from(a.cu, a.S, cur, t0 + j);
+      if (r.end >> j & 1) {
+        if (cur < 0) cur = 0;
+        storev<float, VEC>(a.final_state + (long long)cur * a.D + d, H[j]);
+      }
     }
-    storev<E, VEC>(static_cast<E*>(a.y) + ((long long)p.b * a.T + t) * a.D + p.d, y);
+  } else if (t0 + N >= a.T) {
+    // tokens behind the row pass the state on, so the last register has it
+    storev<float, VEC>(a.final_state + (long long)b * a.D + d, H[N - 1]);
   }
-}
-
-// Sequences without tokens: out = in (or 0). Their final state is their
-// initial one, their initial state's gradient the final one's.
-__global__ __launch_bounds__(256) void rec_empty(RecArgs a, const float* in, float* out) {
-  const long long c = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (c >= (long long)a.S * a.D) return;
-  const long long s = c / a.D;
-  const int lo = a.cu[s] < a.T ? a.cu[s] : a.T, hi = a.cu[s + 1] < a.T ? a.cu[s + 1] : a.T;
-  if (lo >= hi) out[c] = in ? in[c] : 0.f;
 }
 
 // ---------------------------------------------------------------- backward
 
-// (A, C) of every run in reverse: what flows to the token before it,
-// c = A c_in + C, c_t = a_t lam_t.
-template <typename E, int VEC>
-__global__ __launch_bounds__(256) void rec_reduce_bwd(RecArgs a) {
-  const Place p = place<VEC>(a);
-  if (!p.live) return;
-  float bias2[VEC], nrate[VEC], A[VEC], C[VEC];
-  params<VEC>(a, p.d, bias2, nrate);
-  Run r{0u, 0u, ~0u, 0, 0};
-  if (a.cu) r = run_of(a.cu, a.S, p.t0, p.n, a.T);
-  int cur = r.last;
+// A wave has SEG tokens. One pass over them in order forms the gates again, the
+// states from hs, what lam_t multiplies in each gradient, and (A, C) with
+// c = A c_in + C for what flows out of the run backwards (c_t = a_t lam_t).
+// The parameter gradients' sums over tokens, sum lam_t k_t, need no second
+// array: with G_t = a_t G_(t-1) + k_t they are sum dy_t G_t + c_in G_last.
+template <typename E, int VEC, bool PACKED>
+__global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, float* parts) {
+  constexpr int N = SEG;
+  __shared__ Joint<VEC> s_join;
+  __shared__ unsigned s_tile;
+  const unsigned tile = take(sy, &s_tile);
+  const int strip = tile % sy.nstrip, step = tile / sy.nstrip, wv = wave_id();
+  const int chunk = sy.nchunk - 1 - step, b = strip / sy.strips;
+  const long long d = (long long)(strip % sy.strips) * 64 * VEC + lane_id() * VEC;
+  const bool live = d < a.D;
+  const long long dl = live ? d : 0;
+  const int t0 = (chunk * W + wv) * N, n = a.T - t0 < N ? a.T - t0 : N;
+  using R = Raw<E, VEC>;
+  const E* xp = static_cast<const E*>(a.x) + b * a.x_b + dl;
+  const E* fp = static_cast<const E*>(a.f) + b * a.f_b + dl;
+  const E* wp = static_cast<const E*>(a.wz) + b * a.w_b + dl;
+  const E* gp = static_cast<const E*>(a.dy) + b * a.dy_b + dl;
+  R x[N], f[N], w[N], g[N];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) { A[i] = 1.f; C[i] = 0.f; }
-  for (int j = p.n - 1; j >= 0; --j) {
-    const long long t = p.t0 + j;
-    float f[VEC], g[VEC];
-    loadv<E, VEC>(static_cast<const E*>(a.f) + p.b * a.f_b + t * a.f_t + p.d, f);
-    loadv<E, VEC>(static_cast<const E*>(a.dy) + p.b * a.dy_b + t * a.dy_t + p.d, g);
-    const bool us = r.used >> j & 1, en = r.end >> j & 1;
-    if (en) cur = seq_before(a.cu, a.S, cur, (int)t);
+  for (int j = 0; j < N; ++j) {
+    const long long t = t0 + j < a.T ? t0 + j : a.T - 1;
+    f[j] = *reinterpret_cast<const R*>(fp + t * a.f_t);
+    w[j] = *reinterpret_cast<const R*>(wp + t * a.w_t);
+    x[j] = *reinterpret_cast<const R*>(xp + t * a.x_t);
+    g[j] = *reinterpret_cast<const R*>(gp + t * a.dy_t);
+  }
+  const long long nrun = (a.T + SEG - 1) / SEG;
+  float bias2[VEC], nrate[VEC], last[VEC], h[VEC];
+  params<VEC>(a, dl, bias2, nrate);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    last[i] = a.dfinal && !PACKED ? a.dfinal[(long long)b * a.D + dl + i] : 0.f;
+    h[i] = n > 0 ? a.hs[(b * nrun + t0 / SEG) * a.D + dl + i] : 0.f;
+  }
+  Run r{0u, 0u, 0u, 0, 0};
+  if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
+  float aa[N][VEC], bs[N][VEC], kw[N][VEC], kf[N][VEC], dy[N][VEC];
+  float A[VEC], C[VEC], Gb[VEC], Ga[VEC], sb[VEC], sa[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    A[i] = 1.f;
+    C[i] = Gb[i] = Ga[i] = sb[i] = sa[i] = 0.f;
+  }
+  int cur = r.cur;
+  bool open = true;                        // no sequence has ended in the run yet
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const bool st = PACKED && (r.start >> j & 1), us = PACKED ? (r.used >> j & 1) : j < n;
+    const bool en = PACKED && (r.end >> j & 1);
+    if (!us) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        aa[j][i] = PACKED ? 0.f : 1.f;     // behind the row the gradient passes
+        bs[j][i] = kw[j][i] = kf[j][i] = dy[j][i] = 0.f;
+        if (PACKED) Gb[i] = Ga[i] = 0.f;
+      }
+      continue;
+    }
+    if (PACKED && (st || en)) {
+      if (st) cur = seq_from(a.cu, a.S, cur, t0 + j);
+      if (cur < 0) cur = 0;
+    }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const Decay k = decay(f[i], bias2[i], nrate[i]);
-      if (en) {
-        A[i] = 0.f;
-        C[i] = a.dfinal ? a.dfinal[(long long)cur * a.D + p.d + i] : 0.f;
-      }
-      C[i] = us ? k.a * (g[i] + C[i]) : 0.f;
-      A[i] = us ? k.a * A[i] : 0.f;
-    }
-  }
-  const long long nseg = (a.T + SEG - 1) / SEG, n = (long long)a.B * nseg * a.D;
-  const long long o = ((long long)p.b * nseg + p.seg) * a.D + p.d;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    a.ws[o + i] = A[i];
-    a.ws[n + o + i] = C[i];
-  }
-}
-
-__global__ __launch_bounds__(64) void rec_carry_bwd(RecArgs a) {
-  const long long c = (long long)blockIdx.x * 64 + threadIdx.x;
-  if (c >= (long long)a.B * a.D) return;
-  const long long b = c / a.D, d = c % a.D, nseg = (a.T + SEG - 1) / SEG;
-  const long long n = (long long)a.B * nseg * a.D;
-  float h = (a.dfinal && !a.cu) ? a.dfinal[c] : 0.f;
-  for (long long s = nseg - 1; s >= 0; --s) {
-    const long long o = (b * nseg + s) * a.D + d;
-    const float C = a.ws[n + o], A = a.ws[o];
-    a.ws[n + o] = h;
-    h = A == 0.f ? C : A * h + C;
-  }
-  if (a.dh0 && !a.cu) a.dh0[c] = h;
-}
-
-// Every token's gradients from the state entering its run and the gradient
-// entering it from behind; the two sums over tokens a run at a time into ws
-// behind the carries.
-template <typename E, int VEC>
-__global__ __launch_bounds__(256) void rec_apply_bwd(RecArgs a) {
-  const Place p = place<VEC>(a);
-  if (!p.live) return;
-  float bias2[VEC], nrate[VEC], h[VEC], c[VEC], sb[VEC], sa[VEC];
-  params<VEC>(a, p.d, bias2, nrate);
-  const long long nseg = (a.T + SEG - 1) / SEG, n = (long long)a.B * nseg * a.D;
-  const long long o = ((long long)p.b * nseg + p.seg) * a.D + p.d;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    h[i] = a.hs[o + i];
-    c[i] = a.ws[n + o + i];
-    sb[i] = sa[i] = 0.f;
-  }
-  Run r{0u, 0u, ~0u, 0, 0};
-  if (a.cu) r = run_of(a.cu, a.S, p.t0, p.n, a.T);
-  float prev[SEG][VEC];
-  int cur = r.cur;
-#pragma unroll
-  for (int j = 0; j < SEG; ++j) {
-    if (j < p.n) {
-      const long long t = p.t0 + j;
-      float x[VEC], f[VEC], w[VEC];
-      loadv<E, VEC>(static_cast<const E*>(a.x) + p.b * a.x_b + t * a.x_t + p.d, x);
-      loadv<E, VEC>(static_cast<const E*>(a.f) + p.b * a.f_b + t * a.f_t + p.d, f);
-      loadv<E, VEC>(static_cast<const E*>(a.wz) + p.b * a.w_b + t * a.w_t + p.d, w);
-      const bool st = r.start >> j & 1, us = r.used >> j & 1;
-      if (st) cur = seq_from(a.cu, a.S, cur, (int)t);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const Decay k = decay(f[i], bias2[i], nrate[i]);
-        float beta, inv;
-        root(k.q, beta, inv);
-        if (st) h[i] = (a.h0 && us) ? a.h0[(long long)cur * a.D + p.d + i] : 0.f;
-        prev[j][i] = h[i];
-        h[i] = us ? k.a * h[i] + beta * sigmoid2(w[i]) * x[i] : 0.f;
+      const float xv = to_f(x[j].v[i]);
+      const Decay k = decay(to_f(f[j].v[i]), bias2[i], nrate[i]);
+      float beta, inv;
+      root(k.q, beta, inv);
+      const float s = sigmoid2(to_f(w[j].v[i]));
+      const float one = __builtin_amdgcn_rcpf(1.f + k.e), sz = k.up ? one : k.e * one;
+      if (st) h[i] = a.h0 ? a.h0[(long long)cur * a.D + dl + i] : 0.f;
+      const float u = beta * s * xv, ah = k.a * h[i];
+      const float ki = ah - k.a * k.a * inv * (s * xv);       // dg = lam ki
+      aa[j][i] = k.a;
+      bs[j][i] = beta * s;
+      kw[j][i] = u * (1.f - s);
+      kf[j][i] = nrate[i] * sz * ki;
+      dy[j][i] = to_f(g[j].v[i]);
+      if (en && a.dfinal) dy[j][i] += a.dfinal[(long long)cur * a.D + dl + i];
+      h[i] = ah + u;
+      Gb[i] = st ? kf[j][i] : fmaf(k.a, Gb[i], kf[j][i]);
+      Ga[i] = st ? ki * k.g2 : fmaf(k.a, Ga[i], ki * k.g2);
+      sb[i] = fmaf(dy[j][i], Gb[i], sb[i]);
+      sa[i] = fmaf(dy[j][i], Ga[i], sa[i]);
+      if (open) {
+        A[i] *= k.a;
+        C[i] = fmaf(A[i], dy[j][i], C[i]);
       }
     }
+    if (en) open = false;
   }
+  if (PACKED && (!open || r.used != (1u << N) - 1)) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) A[i] = __uint_as_float(RESET);
+  }
+  float c[VEC];
+  join_tiles<PACKED, VEC>(s_join, sy, step, strip, W - 1 - wv, A, C, last, c);
+  // what comes from behind a run whose last token is the last of its sequence
+  // (or in none) is not for it
+  if (PACKED && (n < N || (r.end >> (N - 1) & 1) || !(r.used >> (N - 1) & 1))) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c[i] = 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    sb[i] = fmaf(c[i], Gb[i], sb[i]);
+    sa[i] = fmaf(c[i], Ga[i], sa[i]);
+  }
+  const long long o = ((long long)b * a.T + t0) * a.D + d;
   cur = r.last;
 #pragma unroll
-  for (int j = SEG - 1; j >= 0; --j) {
-    if (j < p.n) {
-      const long long t = p.t0 + j;
-      float x[VEC], f[VEC], w[VEC], g[VEC], dx[VEC], df[VEC], dw[VEC];
-      loadv<E, VEC>(static_cast<const E*>(a.x) + p.b * a.x_b + t * a.x_t + p.d, x);
-      loadv<E, VEC>(static_cast<const E*>(a.f) + p.b * a.f_b + t * a.f_t + p.d, f);
-      loadv<E, VEC>(static_cast<const E*>(a.wz) + p.b * a.w_b + t * a.w_t + p.d, w);
-      loadv<E, VEC>(static_cast<const E*>(a.dy) + p.b * a.dy_b + t * a.dy_t + p.d, g);
-      const bool st = r.start >> j & 1, us = r.used >> j & 1, en = r.end >> j & 1;
-      if (en) cur = seq_before(a.cu, a.S, cur, (int)t);
+  for (int j = N - 1; j >= 0; --j) {
+    const bool st = PACKED && (r.start >> j & 1), us = !PACKED || (r.used >> j & 1);
+    if (PACKED && (!us || (r.end >> j & 1))) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        if (en) c[i] = a.dfinal ? a.dfinal[(long long)cur * a.D + p.d + i] : 0.f;
-        if (!us) {
-          dx[i] = df[i] = dw[i] = c[i] = 0.f;
-          continue;
-        }
-        const Decay k = decay(f[i], bias2[i], nrate[i]);
-        float beta, inv;
-        root(k.q, beta, inv);
-        const float s = sigmoid2(w[i]), lam = g[i] + c[i];
-        const float one = __builtin_amdgcn_rcpf(1.f + k.e), sz = k.up ? one : k.e * one;
-        const float dg = lam * (k.a * prev[j][i] - k.a * k.a * inv * s * x[i]);
-        dx[i] = lam * beta * s;
-        dw[i] = dx[i] * x[i] * (1.f - s);
-        df[i] = nrate[i] * sz * dg;
-        sb[i] += df[i];
-        sa[i] += dg * k.g2;
-        c[i] = k.a * lam;
-        if (st && a.dh0) a.dh0[(long long)cur * a.D + p.d + i] = c[i];
-      }
-      const long long q = ((long long)p.b * a.T + t) * a.D + p.d;
+      for (int i = 0; i < VEC; ++i) c[i] = 0.f;
+    }
+    float dx[VEC], df[VEC], dw[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float lam = dy[j][i] + c[i];
+      dx[i] = lam * bs[j][i];
+      dw[i] = lam * kw[j][i];
+      df[i] = lam * kf[j][i];
+      c[i] = aa[j][i] * lam;
+    }
+    if (live && j < n) {
+      const long long q = o + (long long)j * a.D;
       storev<E, VEC>(static_cast<E*>(a.dx) + q, dx);
       storev<E, VEC>(static_cast<E*>(a.df) + q, df);
       storev<E, VEC>(static_cast<E*>(a.dwz) + q, dw);
+      if (PACKED && st && us && a.dh0) {
+        cur = seq_before(a.cu, a.S, cur, t0 + j);
+        storev<float, VEC>(a.dh0 + (long long)cur * a.D + d, c);
+      }
     }
   }
+  if (!PACKED && t0 == 0 && a.dh0 && live) storev<float, VEC>(a.dh0 + (long long)b * a.D + d, c);
+  // the tile's sums, its waves' in order
+  lds_barrier();
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    a.ws[2 * n + o + i] = sb[i];
-    a.ws[3 * n + o + i] = sa[i];
+  for (int i = 0; i < VEC; ++i) s_join.wave[wv][lane_id() * VEC + i] = make_float2(sb[i], sa[i]);
+  lds_barrier();
+  if (wv == 0 && live) {
+    const long long rows = (long long)a.B * sy.nchunk, row = (long long)b * sy.nchunk + chunk;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      sb[i] = sa[i] = 0.f;
+      for (int k = 0; k < W; ++k) {
+        sb[i] += s_join.wave[k][lane_id() * VEC + i].x;
+        sa[i] += s_join.wave[k][lane_id() * VEC + i].y;
+      }
+    }
+    storev<float, VEC>(parts + row * a.D + d, sb);
+    storev<float, VEC>(parts + (rows + row) * a.D + d, sa);
   }
 }
 
-// Sums over runs, a slice of them a workgroup row: part[slice][2][D].
+// Sums over tiles, a slice of them a workgroup row: part[slice][2][D].
 __global__ __launch_bounds__(256) void rec_sum_runs(RecArgs a, const float* parts, long long rows,
                                                     float* out) {
   __shared__ float s[2][4][64];
@@ -504,87 +699,114 @@ __global__ __launch_bounds__(256) void rec_step_kernel(RecArgs a) {
 
 namespace {
 
-// channels a thread can take at once: every row of every tensor it reads or
-// writes starts on a multiple of that many elements
+// channels a thread can take at once: 4 bytes of the inputs' type, where every
+// row of every tensor starts on a multiple of that
 int vec_of(const RecArgs& a, size_t esz, std::initializer_list<const void*> ts,
            std::initializer_list<int64_t> strides) {
-  if (a.D % 2) return 1;
+  if (esz == 4 || a.D % 2) return 1;
   for (int64_t s : strides)
     if (s % 2) return 1;
   for (const void* t : ts)
-    if (reinterpret_cast<uintptr_t>(t) % (2 * esz)) return 1;
+    if (reinterpret_cast<uintptr_t>(t) % 4) return 1;
   return 2;
 }
 
+long long up(long long n, long long m) { return (n + m - 1) / m * m; }
+
+// The parts of ws (fp32 units): counter, (A, H) pairs, states at groups, runs of
+// packed rows, then the backward's sums over tokens a tile and over slices of them.
+struct Space {
+  long long agg, base, runs, parts, sums, all, nchunk;
+};
+Space space(long long B, long long T, long long D, bool backward) {
+  const long long len = backward ? SEG : REC_FSEG, wide = B * up(D, 128);
+  Space s;
+  s.nchunk = (T + W * len - 1) / (W * len);
+  s.agg = 16;
+  const bool many = s.nchunk > 1;
+  s.base = s.agg + (many ? 2 * s.nchunk * wide : 0);
+  s.runs = s.base + (many ? (s.nchunk / GROUP + 1) * wide : 0);
+  s.parts = s.runs + (B == 1 ? 4 * ((T + len - 1) / len) : 0);
+  s.sums = s.parts + (backward ? 2 * B * s.nchunk * D : 0);
+  s.all = s.sums + (backward ? 2 * REC_SLICES * D : 0);
+  return s;
+}
+
 template <int VEC>
-dim3 run_grid(const RecArgs& a) {
-  const long long nseg = (a.T + SEG - 1) / SEG;
-  return dim3((unsigned)((a.D + 64 * VEC - 1) / (64 * VEC) * ((nseg + 3) / 4) * a.B));
+Sync prepare(const RecArgs& a, const Space& s, int len, const float* in, float* out, hipStream_t st) {
+  Sync y{};
+  y.nchunk = (int)s.nchunk;
+  y.strips = (a.D + 64 * VEC - 1) / (64 * VEC);
+  y.nstrip = y.strips * a.B;
+  long long n16 = 0;
+  if (s.nchunk > 1) {
+    y.ticket = reinterpret_cast<unsigned*>(a.ws);
+    y.agg = reinterpret_cast<unsigned long long*>(a.ws + s.agg);
+    y.base = reinterpret_cast<unsigned*>(a.ws + s.base);
+    n16 = (s.runs - s.agg) / 4;
+  }
+  int4* runs = a.cu ? reinterpret_cast<int4*>(a.ws + s.runs) : nullptr;
+  y.runs = runs;
+  if (n16 || a.cu) {
+    long long n = n16;
+    if (a.cu) n = std::max(n, std::max((long long)(a.T + len - 1) / len, out ? (long long)a.S * a.D : 0));
+    const unsigned grid = (unsigned)std::min<long long>((n + 255) / 256, 1024);
+    hipLaunchKernelGGL(rec_init, dim3(grid), dim3(256), 0, st, a, reinterpret_cast<uint4*>(a.ws + s.agg),
+                       n16, y.ticket, runs, len, in, out);
+  }
+  return y;
 }
 
 template <typename E, int VEC>
 hipError_t fwd(const RecArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((rec_reduce_fwd<E, VEC>), run_grid<VEC>(a), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(rec_carry_fwd, dim3((unsigned)(((long long)a.B * a.D + 63) / 64)), dim3(64), 0, st, a);
-  hipLaunchKernelGGL((rec_apply_fwd<E, VEC>), run_grid<VEC>(a), dim3(256), 0, st, a);
-  if (a.cu && a.final_state && a.S > 0)
-    hipLaunchKernelGGL(rec_empty, dim3((unsigned)(((long long)a.S * a.D + 255) / 256)), dim3(256), 0,
-                       st, a, a.h0, a.final_state);
+  const Space s = space(a.B, a.T, a.D, false);
+  const Sync y = prepare<VEC>(a, s, REC_FSEG, a.h0, a.final_state, st);
+  const dim3 grid((unsigned)(s.nchunk * y.nstrip));
+  if (a.cu) hipLaunchKernelGGL((rec_fwd_kernel<E, VEC, true>), grid, dim3(64 * W), 0, st, a, y);
+  else hipLaunchKernelGGL((rec_fwd_kernel<E, VEC, false>), grid, dim3(64 * W), 0, st, a, y);
   return hipGetLastError();
 }
 
 template <typename E, int VEC>
 hipError_t bwd(const RecArgs& a, hipStream_t st) {
-  const long long nseg = (a.T + SEG - 1) / SEG, rows = a.B * nseg;
-  hipLaunchKernelGGL((rec_reduce_bwd<E, VEC>), run_grid<VEC>(a), dim3(256), 0, st, a);
-  hipLaunchKernelGGL(rec_carry_bwd, dim3((unsigned)(((long long)a.B * a.D + 63) / 64)), dim3(64), 0, st, a);
-  hipLaunchKernelGGL((rec_apply_bwd<E, VEC>), run_grid<VEC>(a), dim3(256), 0, st, a);
-  if (a.cu && a.dh0 && a.S > 0)
-    hipLaunchKernelGGL(rec_empty, dim3((unsigned)(((long long)a.S * a.D + 255) / 256)), dim3(256), 0,
-                       st, a, a.dfinal, a.dh0);
-  float* parts = a.ws + 2 * rows * a.D;
-  float* sums = a.ws + 4 * rows * a.D;
+  const Space s = space(a.B, a.T, a.D, true);
+  const Sync y = prepare<VEC>(a, s, SEG, a.dfinal, a.dh0, st);
+  const dim3 grid((unsigned)(s.nchunk * y.nstrip));
+  float* parts = a.ws + s.parts;
+  if (a.cu) hipLaunchKernelGGL((rec_bwd_kernel<E, VEC, true>), grid, dim3(64 * W), 0, st, a, y, parts);
+  else hipLaunchKernelGGL((rec_bwd_kernel<E, VEC, false>), grid, dim3(64 * W), 0, st, a, y, parts);
+  float* sums = a.ws + s.sums;
   hipLaunchKernelGGL(rec_sum_runs, dim3((a.D + 63) / 64, REC_SLICES), dim3(256), 0, st, a,
-                     (const float*)parts, rows, sums);
+                     (const float*)parts, s.nchunk * a.B, sums);
   hipLaunchKernelGGL(rec_sum_heads, dim3(a.H), dim3(64), 0, st, a, (const float*)sums);
   return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t rec_ws(int64_t B, int64_t T, int64_t D, bool backward) {
-  const int64_t nseg = (T + SEG - 1) / SEG;
-  if (!backward) return B * nseg * D;
-  return 4 * B * nseg * D + 2 * REC_SLICES * D;
-}
+int64_t rec_ws(int64_t B, int64_t T, int64_t D, bool backward) { return space(B, T, D, backward).all; }
 
 hipError_t rec_fwd(const RecArgs& a, int dtype, hipStream_t st) {
-  const size_t esz = dtype == NGDN_BF16 ? 2 : 4;
-  const int v = vec_of(a, esz, {a.x, a.f, a.wz, a.y}, {a.x_b, a.x_t, a.f_b, a.f_t, a.w_b, a.w_t});
-  if (dtype == NGDN_BF16) return v == 2 ? fwd<bf16, 2>(a, st) : fwd<bf16, 1>(a, st);
-  return v == 2 ? fwd<float, 2>(a, st) : fwd<float, 1>(a, st);
+  if (dtype == NGDN_F32) return fwd<float, 1>(a, st);
+  const int v = vec_of(a, 2, {a.x, a.f, a.wz, a.y}, {a.x_b, a.x_t, a.f_b, a.f_t, a.w_b, a.w_t});
+  return v == 2 ? fwd<bf16, 2>(a, st) : fwd<bf16, 1>(a, st);
 }
 
 hipError_t rec_bwd(const RecArgs& a, int dtype, hipStream_t st) {
-  const size_t esz = dtype == NGDN_BF16 ? 2 : 4;
-  const int v = vec_of(a, esz, {a.x, a.f, a.wz, a.dy, a.dx, a.df, a.dwz},
+  if (dtype == NGDN_F32) return bwd<float, 1>(a, st);
+  const int v = vec_of(a, 2, {a.x, a.f, a.wz, a.dy, a.dx, a.df, a.dwz},
                        {a.x_b, a.x_t, a.f_b, a.f_t, a.w_b, a.w_t, a.dy_b, a.dy_t});
-  if (dtype == NGDN_BF16) return v == 2 ? bwd<bf16, 2>(a, st) : bwd<bf16, 1>(a, st);
-  return v == 2 ? bwd<float, 2>(a, st) : bwd<float, 1>(a, st);
+  return v == 2 ? bwd<bf16, 2>(a, st) : bwd<bf16, 1>(a, st);
 }
 
 hipError_t rec_step(const RecArgs& a, int dtype, hipStream_t st) {
-  const size_t esz = dtype == NGDN_BF16 ? 2 : 4;
-  int v = vec_of(a, esz, {a.x, a.f, a.wz, a.y}, {a.x_b, a.f_b, a.w_b});
-  if (v == 2) v = vec_of(a, 4, {a.h0, a.final_state}, {});
+  int v = 1;
+  if (dtype == NGDN_BF16) v = vec_of(a, 2, {a.x, a.f, a.wz, a.y}, {a.x_b, a.f_b, a.w_b});
+  if ((reinterpret_cast<uintptr_t>(a.h0) | reinterpret_cast<uintptr_t>(a.final_state)) % 8) v = 1;
   const dim3 grid((unsigned)(((long long)a.B * (a.D / v) + 255) / 256));
-  if (dtype == NGDN_BF16) {
-    if (v == 2) hipLaunchKernelGGL((rec_step_kernel<bf16, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((rec_step_kernel<bf16, 1>), grid, dim3(256), 0, st, a);
-  } else {
-    if (v == 2) hipLaunchKernelGGL((rec_step_kernel<float, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((rec_step_kernel<float, 1>), grid, dim3(256), 0, st, a);
-  }
+  if (dtype == NGDN_F32) hipLaunchKernelGGL((rec_step_kernel<float, 1>), grid, dim3(256), 0, st, a);
+  else if (v == 2) hipLaunchKernelGGL((rec_step_kernel<bf16, 2>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((rec_step_kernel<bf16, 1>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
