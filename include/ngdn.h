@@ -596,8 +596,9 @@ int32_t ngdn_embedding_fwd(int32_t w_dtype, int32_t y_dtype, int64_t N, int64_t 
 /* Its gradient: dw[v,:] = scale sum of dy[n,:] over the n with ids[n] == v, in
  * fp32 and in an order that the ids alone fix, rounded once to w_dtype; every
  * row of dw [V,D] is written (zeros where no id points, and on row
- * padding_idx; negative: no such row). Ids outside [0, V) add nothing. ws:
- * ngdn_embedding_ws(N, V, D) int32, no initial contents. */
+ * padding_idx; negative: no such row). Ids outside [0, V) add nothing. dw
+ * 16-byte aligned; ws: ngdn_embedding_ws(N, V, D) int32, no initial contents.
+ * N <= 2^24, V < 2^24, N D <= 2^35. */
 int32_t ngdn_embedding_bwd(int32_t dy_dtype, int32_t w_dtype, int64_t N, int64_t V, int32_t D,
                            float scale, int64_t padding_idx, const int64_t* ids, const void* dy,
                            void* dw, int32_t* ws, void* stream);

@@ -1104,6 +1104,7 @@ int32_t embed_sizes(int32_t d0, int32_t d1, int64_t N, int64_t V, int32_t D, con
   if (N < 0 || V < 1 || D < 1 || N > (1LL << 24) || V > (1LL << 24) - 1 || D > (1 << 20))
     return fail(NGDN_EINVAL, "%s: N=%lld V=%lld D=%d (0 <= N <= 2^24, 1 <= V < 2^24, 1 <= D <= 2^20)",
                 what, (long long)N, (long long)V, D);
+  if (N * D > 1LL << 35) return fail(NGDN_EINVAL, "%s: N*D = %lld exceeds 2^35", what, (long long)N * D);
   return NGDN_OK;
 }
 
@@ -1154,7 +1155,8 @@ int32_t ngdn_embedding_bwd(int32_t dy_dtype, int32_t w_dtype, int64_t N, int64_t
                            void* dw, int32_t* ws, void* stream) {
   g_err[0] = 0;
   if (int32_t r = embed_sizes(dy_dtype, w_dtype, N, V, D, "ngdn_embedding_bwd")) return r;
-  if (!dw || (N > 0 && (!ids || !dy || !ws))) return fail(NGDN_EINVAL, "ngdn_embedding_bwd: NULL tensor");
+  if (!dw || !ws || (N > 0 && (!ids || !dy))) return fail(NGDN_EINVAL, "ngdn_embedding_bwd: NULL tensor");
+  if (reinterpret_cast<uintptr_t>(dw) & 15) return fail(NGDN_EINVAL, "ngdn_embedding_bwd: dw must be 16-byte aligned");
   ngdn::EmbedArgs a{};
   a.ids = reinterpret_cast<const long long*>(ids); a.dy = dy; a.dw = dw; a.ws = ws;
   a.N = N; a.V = V; a.D = D; a.scale = scale; a.padding_idx = padding_idx;
