@@ -623,7 +623,7 @@ int64_t ngdn_embedding_ws(int64_t N, int64_t V, int32_t D);
  * h0 and dfinal may be NULL (zeros), final_state and dh0 NULL (not written).
  * The forward with hs set ([B, ceil(T / NGDN_REC_RUN), D] fp32; the state
  * entering each run of NGDN_REC_RUN tokens) leaves there what the backward
- * reads; hs is required in both. The backward takes the forward's inputs, hs,
+ * reads (NULL: not written). The backward takes the forward's inputs, hs,
  * dy (strides dy_b, dy_t) and dfinal, and writes dx, df, dwz [B,T,D] in dtype
  * and, fp32, ddt_bias [D], dA_log [H] and dh0. ws: ngdn_recurrence_ws(...)
  * fp32, no initial contents. Sums over tokens are in a fixed order: the same

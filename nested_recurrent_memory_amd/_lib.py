@@ -164,7 +164,22 @@ def ptr(t):
 
 
 def stream_of(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # current_stream(device).cuda_stream without the Stream object (3 us less a call)
+    return _raw_stream(t.device.index)
+
+
+def on_device(t, name, *args):
+    """``call`` on t's device, whichever is current: a launch needs its stream's device."""
+    i = t.device.index
+    if i == _current_device():
+        call(name, *args, _raw_stream(i))
+    else:
+        with torch.cuda.device(i):
+            call(name, *args, _raw_stream(i))
+
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def ptr_of_stream(st):

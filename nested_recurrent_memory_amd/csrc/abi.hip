@@ -1171,7 +1171,7 @@ int32_t ngdn_recurrence_fwd(int32_t dtype, const ngdn_recurrence_args* r, void* 
   g_err[0] = 0;
   if (int32_t e = rec_check(dtype, r, "ngdn_recurrence_fwd")) return e;
   if (int32_t e = rec_rows(r, "ngdn_recurrence_fwd")) return e;
-  if (!r->y || !r->hs || !r->ws) return fail(NGDN_EINVAL, "ngdn_recurrence_fwd: NULL tensor");
+  if (!r->y || !r->ws) return fail(NGDN_EINVAL, "ngdn_recurrence_fwd: NULL tensor");
   return launched(ngdn::rec_fwd(*r, dtype, (hipStream_t)stream), "ngdn_recurrence_fwd");
 }
 

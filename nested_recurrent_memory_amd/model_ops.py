@@ -64,22 +64,32 @@ _TABLES = (torch.bfloat16, torch.float16, torch.float32)     # fp16 runs in fp32
 _EMBED_MOST = 1 << 24                                        # ids, and rows of the table
 
 
-def _embed_call(name, t, *args):
-    # on t's device, whichever is current: a launch needs its stream's device
-    if t.device.index == torch.cuda.current_device():
-        _lib.call(name, *args, _lib.stream_of(t))
-    else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, *args, _lib.stream_of(t))
+def _embed(t):
+    if t.dtype not in _EMBED:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _lookup(ids, weight, scale, ydt):
-    w = _work(weight).contiguous()
-    y = torch.empty(*ids.shape, w.shape[1], device=w.device, dtype=ydt if ydt in _EMBED else torch.float32)
-    if y.numel():
-        _embed_call("ngdn_embedding_fwd", w, _code(w), _code(y), ids.numel(), w.shape[0], w.shape[1],
-                    scale, _lib.ptr(ids), _lib.ptr(w), _lib.ptr(y))
-    return y.to(ydt)
+    w = _embed(weight)
+    V, D = w.shape
+    y = torch.empty((*ids.shape, D), device=w.device, dtype=ydt if ydt in _EMBED else torch.float32)
+    N = ids.numel()
+    if N:
+        _lib.on_device(w, "ngdn_embedding_fwd", _code(w), _code(y), N, V, D, scale, ids.data_ptr(),
+                       w.data_ptr(), y.data_ptr())
+    return y if y.dtype == ydt else y.to(ydt)
+
+
+def _lookup_grad(ids, dy, scale, padding_idx, V, wdt):
+    g = _embed(dy)
+    N, D = ids.numel(), dy.shape[-1]
+    dw = torch.empty((V, D), device=g.device, dtype=wdt if wdt in _EMBED else torch.float32)
+    ws = torch.empty(_lib.lib().ngdn_embedding_ws(N, V, D), device=g.device, dtype=torch.int32)
+    _lib.on_device(g, "ngdn_embedding_bwd", _code(g), _code(dw), N, V, D, scale,
+                   -1 if padding_idx is None else padding_idx, ids.data_ptr(), g.data_ptr(),
+                   dw.data_ptr(), ws.data_ptr())
+    return dw if dw.dtype == wdt else dw.to(wdt)
 
 
 class _EmbeddingFn(torch.autograd.Function):
@@ -94,7 +104,9 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
-        return None, _EmbeddingGradFn.apply(ids, dy, *ctx.cfg), None, None, None
+        # a graph is only wanted where the gradient is differentiated again
+        grad = _EmbeddingGradFn.apply if torch.is_grad_enabled() else _lookup_grad
+        return None, grad(ids, dy, *ctx.cfg), None, None, None
 
 
 class _EmbeddingGradFn(torch.autograd.Function):
@@ -102,14 +114,7 @@ class _EmbeddingGradFn(torch.autograd.Function):
     def forward(ctx, ids, dy, scale, padding_idx, V, wdt):
         ctx.save_for_backward(ids)
         ctx.cfg = (scale, padding_idx, dy.dtype)
-        g = _work(dy).contiguous()
-        N, D = ids.numel(), dy.shape[-1]
-        dw = torch.empty(V, D, device=g.device, dtype=wdt if wdt in _EMBED else torch.float32)
-        ws = torch.empty(_lib.lib().ngdn_embedding_ws(N, V, D), device=g.device, dtype=torch.int32)
-        _embed_call("ngdn_embedding_bwd", g, _code(g), _code(dw), N, V, D, scale,
-                    -1 if padding_idx is None else padding_idx, _lib.ptr(ids), _lib.ptr(g),
-                    _lib.ptr(dw), _lib.ptr(ws))
-        return dw.to(wdt)
+        return _lookup_grad(ids, dy, scale, padding_idx, V, wdt)
 
     @staticmethod
     def backward(ctx, ddw):
@@ -133,8 +138,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
                          "fp32, [V,D])")
     if ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"embedding: ids are {ids.dtype} (int32 or int64)")
-    V = weight.shape[0]
     if padding_idx is not None:
+        V = weight.shape[0]
         if not -V <= padding_idx < V:
             raise ValueError(f"embedding: padding_idx {padding_idx} outside the {V} rows of weight")
         padding_idx %= V
@@ -142,7 +147,13 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     if ydt not in _TABLES:
         raise ValueError(f"embedding: out_dtype {ydt} (bf16, fp16 or fp32)")
     _on_gpu("embedding", weight, ids)
-    return _EmbeddingFn.apply(ids.to(torch.int64).contiguous(), weight, float(scale), padding_idx, ydt)
+    if ids.dtype != torch.int64:
+        ids = ids.to(torch.int64)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    if not (weight.requires_grad and torch.is_grad_enabled()) and forward_ad._current_level < 0:
+        return _lookup(ids, weight.detach(), float(scale), ydt)
+    return _EmbeddingFn.apply(ids, weight, float(scale), padding_idx, ydt)
 
 
 class Embedding(nn.Embedding):

@@ -44,41 +44,42 @@ def _on_gpu(name, *ts):
                              "there is no CPU path")
 
 
-def _call(name, dtype, args, t):
-    # on t's device, whichever is current: a launch needs its stream's device
-    if t.device.index == torch.cuda.current_device():
-        _lib.call(name, _code(dtype), ctypes.byref(args), _lib.stream_of(t))
-    else:
-        with torch.cuda.device(t.device):
-            _lib.call(name, _code(dtype), ctypes.byref(args), _lib.stream_of(t))
-
-
 def _rows(t, dtype):
     """t in dtype with its last dimension consecutive: the kernels take any
     other strides."""
-    t = t.to(dtype)
+    if t.dtype != dtype:
+        t = t.to(dtype)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _f32(t):
-    return None if t is None else t.to(torch.float32).contiguous()
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        t = t.to(torch.float32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _fill(args, B, T, D, x, f, wz, A_log, dt_bias):
-    args.B, args.T, args.D, args.H = B, T, D, A_log.shape[0]
-    args.x, args.f, args.wz = x.data_ptr(), f.data_ptr(), wz.data_ptr()
-    args.A_log, args.dt_bias = A_log.data_ptr(), dt_bias.data_ptr()
-    args.x_b, args.f_b, args.w_b = x.stride(0), f.stride(0), wz.stride(0)
-    return args
+_WORK = (torch.bfloat16, torch.float32)                     # the kernels' types
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)     # fp16 runs in fp32
+
+
+def _token_args(B, T, D, x, f, wz, A_log, dt_bias):
+    a = _lib.RecurrenceArgs()
+    a.B, a.T, a.D, a.H = B, T, D, A_log.shape[0]
+    a.x, a.f, a.wz = x.data_ptr(), f.data_ptr(), wz.data_ptr()
+    a.A_log, a.dt_bias = A_log.data_ptr(), dt_bias.data_ptr()
+    a.x_b, a.f_b, a.w_b = x.stride(0), f.stride(0), wz.stride(0)
+    return a
 
 
 def _sequence_args(x, f, wz, A_log, dt_bias, h0, cu):
-    B, T, D = x.shape
-    a = _fill(_lib.RecurrenceArgs(), B, T, D, x, f, wz, A_log, dt_bias)
+    a = _token_args(*x.shape, x, f, wz, A_log, dt_bias)
     a.x_t, a.f_t, a.w_t = x.stride(1), f.stride(1), wz.stride(1)
     if cu is not None:
         a.S, a.cu = cu.shape[0] - 1, cu.data_ptr()
-    a.h0 = _lib.ptr(h0)
+    if h0 is not None:
+        a.h0 = h0.data_ptr()
     return a
 
 
@@ -86,13 +87,15 @@ class _RecurrenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, wz, A_log, dt_bias, h0, cu, want_final):
         B, T, D = x.shape
-        wd = x.dtype if x.dtype in (torch.bfloat16, torch.float32) else torch.float32
-        xw, fw, ww = (_rows(t, wd) for t in (x, f, wz))
+        wd = x.dtype if x.dtype in _WORK else torch.float32
+        xw, fw, ww = _rows(x, wd), _rows(f, wd), _rows(wz, wd)
         A, dt, h = _f32(A_log), _f32(dt_bias), _f32(h0)
-        cu = cu.to(torch.int32).contiguous() if cu is not None else None
+        if cu is not None:
+            cu = cu.to(torch.int32).contiguous()
         rows = B if cu is None else cu.shape[0] - 1
-        y = torch.empty(B, T, D, device=x.device, dtype=wd)
-        final = torch.empty(rows, D, device=x.device, dtype=torch.float32) if want_final else None
+        dev = x.device
+        y = torch.empty((B, T, D), device=dev, dtype=wd)
+        final = torch.empty((rows, D), device=dev, dtype=torch.float32) if want_final else None
         hs = None
         if y.numel() == 0 or rows == 0:       # no token: the states stay
             y.zero_()
@@ -100,16 +103,17 @@ class _RecurrenceFn(torch.autograd.Function):
                 final.copy_(h) if h is not None else final.zero_()
         else:
             a = _sequence_args(xw, fw, ww, A, dt, h, cu)
-            nseg = -(-T // _lib.REC_RUN)
-            hs = torch.empty(B, nseg, D, device=x.device, dtype=torch.float32)
-            ws = torch.empty(_lib.lib().ngdn_recurrence_ws(B, T, D, 0), device=x.device,
-                             dtype=torch.float32)
-            a.y, a.final_state, a.hs, a.ws = y.data_ptr(), _lib.ptr(final), hs.data_ptr(), ws.data_ptr()
-            _call("ngdn_recurrence_fwd", wd, a, x)
+            ws = torch.empty(_lib.lib().ngdn_recurrence_ws(B, T, D, 0), device=dev, dtype=torch.float32)
+            a.y, a.final_state, a.ws = y.data_ptr(), _lib.ptr(final), ws.data_ptr()
+            if any(ctx.needs_input_grad):
+                hs = torch.empty((B, -(-T // _lib.REC_RUN), D), device=dev, dtype=torch.float32)
+                a.hs = hs.data_ptr()
+            _lib.on_device(y, "ngdn_recurrence_fwd", _code(wd), ctypes.byref(a))
         ctx.save_for_backward(xw, fw, ww, A, dt, h, cu, hs)
-        ctx.dtypes = tuple(t.dtype if t is not None else None for t in (x, f, wz, A_log, dt_bias, h0))
+        ctx.dtypes = (x.dtype, f.dtype, wz.dtype, A_log.dtype, dt_bias.dtype,
+                      h0.dtype if h0 is not None else None)
         ctx.set_materialize_grads(False)
-        return y.to(x.dtype), final
+        return y if y.dtype == x.dtype else y.to(x.dtype), final
 
     @staticmethod
     @once_differentiable
@@ -118,8 +122,9 @@ class _RecurrenceFn(torch.autograd.Function):
         B, T, D = xw.shape
         wd, dev = xw.dtype, xw.device
         rows = B if cu is None else cu.shape[0] - 1
-        dh0 = torch.empty(rows, D, device=dev, dtype=torch.float32) if ctx.needs_input_grad[5] else None
-        dx, df, dw = (torch.empty(B, T, D, device=dev, dtype=wd) for _ in range(3))
+        dh0 = torch.empty((rows, D), device=dev, dtype=torch.float32) if ctx.needs_input_grad[5] else None
+        dx = torch.empty((B, T, D), device=dev, dtype=wd)
+        df, dw = torch.empty_like(dx), torch.empty_like(dx)
         dA, ddt = torch.empty_like(A), torch.empty_like(dt)
         dfinal = _f32(dfinal)
         if hs is None:
@@ -128,16 +133,16 @@ class _RecurrenceFn(torch.autograd.Function):
             if dh0 is not None:
                 dh0.copy_(dfinal) if dfinal is not None else dh0.zero_()
         else:
-            dyw = _rows(dy, wd) if dy is not None else torch.zeros(B, T, D, device=dev, dtype=wd)
+            dyw = _rows(dy, wd) if dy is not None else torch.zeros_like(dx)
             a = _sequence_args(xw, fw, ww, A, dt, h, cu)
             ws = torch.empty(_lib.lib().ngdn_recurrence_ws(B, T, D, 1), device=dev, dtype=torch.float32)
             a.hs, a.ws, a.dy, a.dfinal = hs.data_ptr(), ws.data_ptr(), dyw.data_ptr(), _lib.ptr(dfinal)
             a.dy_b, a.dy_t = dyw.stride(0), dyw.stride(1)
             a.dx, a.df, a.dwz = dx.data_ptr(), df.data_ptr(), dw.data_ptr()
             a.dA_log, a.ddt_bias, a.dh0 = dA.data_ptr(), ddt.data_ptr(), _lib.ptr(dh0)
-            _call("ngdn_recurrence_bwd", wd, a, xw)
-        return tuple(g.to(d) if g is not None else None
-                     for g, d in zip((dx, df, dw, dA, ddt, dh0), ctx.dtypes)) + (None, None)
+            _lib.on_device(dx, "ngdn_recurrence_bwd", _code(wd), ctypes.byref(a))
+        return (*(g if g is None or g.dtype == d else g.to(d)
+                  for g, d in zip((dx, df, dw, dA, ddt, dh0), ctx.dtypes)), None, None)
 
 
 def _check(name, x, f, wz, A_log, dt_bias, dims):
@@ -150,7 +155,7 @@ def _check(name, x, f, wz, A_log, dt_bias, dims):
         raise ValueError(f"{name}: dt_bias {tuple(dt_bias.shape)}, A_log {tuple(A_log.shape)} for "
                          f"D={D} (dt_bias [D], A_log [H] with D a multiple of H)")
     for n, t in (("x", x), ("f", f), ("wz", wz), ("A_log", A_log), ("dt_bias", dt_bias)):
-        if t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        if t.dtype not in _TYPES:
             raise ValueError(f"{name}: {n} is {t.dtype} (bf16, fp16 or fp32)")
 
 
@@ -202,8 +207,8 @@ def step_gated_recurrence(x, f, wz, A_log, dt_bias, state, *, inplace=False):
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, f, wz, A_log, dt_bias, state)):
         raise RuntimeError(f"{name} is forward-only (decoding); call it under torch.no_grad() or on "
                            "tensors that do not require grad")
-    wd = x.dtype if x.dtype in (torch.bfloat16, torch.float32) else torch.float32
-    xw, fw, ww = (_rows(t, wd) for t in (x, f, wz))
+    wd = x.dtype if x.dtype in _WORK else torch.float32
+    xw, fw, ww = _rows(x, wd), _rows(f, wd), _rows(wz, wd)
     A, dt = _f32(A_log), _f32(dt_bias)
     if inplace:
         if state.dtype != torch.float32 or not state.is_contiguous():
@@ -212,9 +217,9 @@ def step_gated_recurrence(x, f, wz, A_log, dt_bias, state, *, inplace=False):
     else:
         s_in = _f32(state)
         s_out = torch.empty_like(s_in)
-    y = torch.empty(B, D, device=x.device, dtype=wd)
+    y = torch.empty((B, D), device=x.device, dtype=wd)
     if B:
-        a = _fill(_lib.RecurrenceArgs(), B, 1, D, xw, fw, ww, A, dt)
+        a = _token_args(B, 1, D, xw, fw, ww, A, dt)
         a.h0, a.final_state, a.y = s_in.data_ptr(), s_out.data_ptr(), y.data_ptr()
-        _call("ngdn_recurrence_step", wd, a, x)
-    return y.to(x.dtype), s_out
+        _lib.on_device(y, "ngdn_recurrence_step", _code(wd), ctypes.byref(a))
+    return y if y.dtype == x.dtype else y.to(x.dtype), s_out
