@@ -167,26 +167,29 @@ __device__ __forceinline__ void params(const RecArgs& a, long long d, float* bia
 // A workgroup has W waves, each a run of tokens of 64 VEC channels: a tile of
 // W runs. The state that enters a tile comes from the tiles before it (in the
 // backward: behind it) while those are still running, through device memory:
-// every tile publishes its (A, H) as soon as it has them; every GROUP-th also
-// the state behind it. A tile takes the state at its group's start and the
-// (A, H) of the tiles between, so the chain over a long row has a link every
-// GROUP tiles, and the order of the arithmetic does not depend on timing.
+// every tile publishes its (A, H) as soon as it has them; the last of a group of
+// W or 2 W also the state behind it. A tile takes the state at its group's start
+// and the (A, H) of the tiles between, so the chain over a long row has a link a
+// group, and the order of the arithmetic does not depend on timing.
 // One 64-bit (32-bit) value is its own flag: all bits set before it is
 // published, which no published value has (a NaN of that pattern is changed).
-// Tiles are handed out by a counter, so all a tile waits for was started
-// before it and waits only for tiles before itself: every wait ends.
+// A strip's tiles are handed out by a counter, so all a tile waits for was
+// started before it and waits only for tiles before itself: every wait ends.
+// A counter for each strip: 512 workgroups that start together on one counter
+// take 6 us to get their numbers.
 // Against reducing, joining and applying in three launches: inputs are read
 // and their gates computed once instead of twice.
 
 constexpr int W = REC_WAVES;
-constexpr int GROUP = 2 * W;
+constexpr int LINE = 32;            // ints in a cache line
 
 struct Sync {
-  unsigned* ticket;                 // NULL: one tile a row, nothing to join
+  int* ticket;                      // [nstrip] counters, LINE apart (NULL: one tile a row, nothing to join)
   unsigned long long* agg;          // [nchunk][nstrip][64 VEC] (A, H)
-  unsigned* base;                   // [nchunk / GROUP + 1][nstrip][64 VEC]
+  unsigned* base;                   // [groups][nstrip][64 VEC]
   const int4* runs;                 // packed rows: every run's Run
   int nchunk, nstrip, strips;       // nstrip = B strips
+  int each;                         // tiles of a group for each wave to look at, 1 or 2
 };
 
 __device__ __forceinline__ unsigned bits(float x) { return __float_as_uint(x); }
@@ -226,7 +229,7 @@ __device__ __forceinline__ U await(const U* p) {
 template <int VEC>
 struct Joint {
   float2 wave[W][64 * VEC];         // (A, H) of the tile's waves, in the order of the scan
-  float2 before[W][64 * VEC];       // of up to GROUP / W tiles before it each
+  float2 before[W][64 * VEC];       // of up to two tiles before it each
   float base[64 * VEC];
 };
 
@@ -239,7 +242,7 @@ __device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int ste
 #pragma unroll
   for (int i = 0; i < VEC; ++i) s.wave[wv][l * VEC + i] = make_float2(A[i], H[i]);
   lds_barrier();
-  const int g0 = step / GROUP * GROUP, n = step - g0;      // tiles between the group's start and this one
+  const int group = y.each * W, g0 = step / group * group, n = step - g0;   // n tiles from the group's start
   const bool more = y.ticket != nullptr;
   auto agg = [&](int k) { return y.agg + ((long long)k * y.nstrip + strip) * (64 * VEC) + l * VEC; };
   auto base = [&](int k) { return y.base + ((long long)k * y.nstrip + strip) * (64 * VEC) + l * VEC; };
@@ -257,12 +260,12 @@ __device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int ste
     }
   }
   if (more && step > 0) {
-    // wave wv: tiles g0 + 2 wv and + 1 of the n before; the last wave is never
-    // needed for them when n < GROUP - 1, and takes the state at g0 too
+    // wave wv: `each` of the n tiles; the last wave, which has one less, also the
+    // state at g0
     float bA[VEC], bH[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { bA[i] = 1.f; bH[i] = 0.f; }
-    for (int k = wv * (GROUP / W); k < (wv + 1) * (GROUP / W) && k < n; ++k) {
+    for (int k = wv * y.each; k < (wv + 1) * y.each && k < n; ++k) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const unsigned long long v = await(agg(g0 + k) + i);
@@ -274,13 +277,13 @@ __device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int ste
     if (wv == W - 1) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        s.base[l * VEC + i] = g0 > 0 ? __uint_as_float(await(base(g0 / GROUP) + i)) : first[i];
+        s.base[l * VEC + i] = g0 > 0 ? __uint_as_float(await(base(g0 / group) + i)) : first[i];
     }
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       h[i] = s.base[l * VEC + i];
-      for (int k = 0; k * (GROUP / W) < n; ++k) {
+      for (int k = 0; k * y.each < n; ++k) {
         const float2 v = s.before[k][l * VEC + i];
         h[i] = pass<PACKED>(h[i], v.x, v.y);
       }
@@ -289,9 +292,9 @@ __device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int ste
 #pragma unroll
     for (int i = 0; i < VEC; ++i) h[i] = first[i];
   }
-  if (more && wv == W - 1 && n == GROUP - 1 && step + 1 < y.nchunk) {
+  if (more && wv == W - 1 && n == group - 1 && step + 1 < y.nchunk) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) publish(base(g0 / GROUP + 1) + i, pass<PACKED>(h[i], tA[i], tH[i]));
+    for (int i = 0; i < VEC; ++i) publish(base(g0 / group + 1) + i, pass<PACKED>(h[i], tA[i], tH[i]));
   }
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
@@ -302,33 +305,51 @@ __device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int ste
   }
 }
 
-__device__ __forceinline__ unsigned take(const Sync& y, unsigned* s_tile) {
-  if (!y.ticket) return blockIdx.x;
+// A workgroup's strip: every nstrip workgroups one of each, turned on by one
+// each time, so that the workgroups of one XCD (every 8th) go over all strips. A
+// strip's rows lie a whole row apart and fall on few of the XCD's L2 channels:
+// with a strip always on the same XCD, 65536 x 2048 took 278 us, turned 243.
+__device__ __forceinline__ int strip_of(const Sync& y) {
+  const unsigned q = blockIdx.x / y.nstrip, r = blockIdx.x - q * y.nstrip;
+  return (r + q) % y.nstrip;
+}
+// The tile's place in its strip's scan.
+__device__ __forceinline__ int take(const Sync& y, int strip, int* s_step) {
+  if (!y.ticket) return 0;
   if (threadIdx.x == 0)
-    *s_tile = __hip_atomic_fetch_add(y.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *s_step = __hip_atomic_fetch_add(y.ticket + strip * LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(*s_tile);
+  return __builtin_amdgcn_readfirstlane(*s_step);
 }
 
 // Before either pass: the flags' patterns, the counter, where the boundaries of
 // packed sequences fall in each run of `len` tokens, and sequences without
 // tokens (out = in or 0: their final state is their initial one, their initial
 // state's gradient the final one's).
-__global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long long n16, unsigned* ticket,
+__global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long long n16, int* ticket, int tickets,
                                                 int4* runs, int len, const float* in, float* out) {
   const long long i0 = (long long)blockIdx.x * 256 + threadIdx.x, step = (long long)gridDim.x * 256;
-  if (i0 == 0 && ticket) *ticket = 0;
+  for (long long i = i0; i < tickets; i += step) ticket[i * LINE] = 0;
   for (long long i = i0; i < n16; i += step) fill[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
   if (!a.cu) return;
+  // the search and the walk are chains of reads: from LDS where the boundaries fit
+  constexpr int FIT = 4096;
+  __shared__ int s_cu[FIT];
+  const int* cu = a.cu;
+  if (a.S < FIT) {
+    for (int i = threadIdx.x; i <= a.S; i += 256) s_cu[i] = a.cu[i];
+    __syncthreads();
+    cu = s_cu;
+  }
   const int nrun = (a.T + len - 1) / len;
   for (long long i = i0; i < nrun; i += step) {
     const int t0 = (int)i * len;
-    runs[i] = pack(run_of(a.cu, a.S, t0, a.T - t0 < len ? a.T - t0 : len, a.T));
+    runs[i] = pack(run_of(cu, a.S, t0, a.T - t0 < len ? a.T - t0 : len, a.T));
   }
   if (!out) return;
   for (long long c = i0; c < (long long)a.S * a.D; c += step) {
     const long long s = c / a.D;
-    const int lo = a.cu[s] < a.T ? a.cu[s] : a.T, hi = a.cu[s + 1] < a.T ? a.cu[s + 1] : a.T;
+    const int lo = cu[s] < a.T ? cu[s] : a.T, hi = cu[s + 1] < a.T ? cu[s + 1] : a.T;
     if (lo >= hi) out[c] = in ? in[c] : 0.f;
   }
 }
@@ -346,9 +367,8 @@ template <typename E, int VEC, bool PACKED>
 __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) {
   constexpr int N = REC_FSEG;
   __shared__ Joint<VEC> s_join;
-  __shared__ unsigned s_tile;
-  const unsigned tile = take(sy, &s_tile);
-  const int strip = tile % sy.nstrip, chunk = tile / sy.nstrip, wv = wave_id();
+  __shared__ int s_step;
+  const int strip = strip_of(sy), chunk = take(sy, strip, &s_step), wv = wave_id();
   const int b = strip / sy.strips;
   const long long d = (long long)(strip % sy.strips) * 64 * VEC + lane_id() * VEC;
   const bool live = d < a.D;
@@ -473,9 +493,8 @@ template <typename E, int VEC, bool PACKED>
 __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, float* parts) {
   constexpr int N = SEG;
   __shared__ Joint<VEC> s_join;
-  __shared__ unsigned s_tile;
-  const unsigned tile = take(sy, &s_tile);
-  const int strip = tile % sy.nstrip, step = tile / sy.nstrip, wv = wave_id();
+  __shared__ int s_step;
+  const int strip = strip_of(sy), step = take(sy, strip, &s_step), wv = wave_id();
   const int chunk = sy.nchunk - 1 - step, b = strip / sy.strips;
   const long long d = (long long)(strip % sy.strips) * 64 * VEC + lane_id() * VEC;
   const bool live = d < a.D;
@@ -627,46 +646,56 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
   }
 }
 
-// Sums over tiles, a slice of them a workgroup row: part[slice][2][D].
-__global__ __launch_bounds__(256) void rec_sum_runs(RecArgs a, const float* parts, long long rows,
-                                                    float* out) {
+// Sums over tiles ([2][rows][D]), a slice of them a workgroup row: [2][slices][D].
+__global__ __launch_bounds__(256) void rec_sum_runs(const float* parts, long long rows, int D, int slices, float* out) {
   __shared__ float s[2][4][64];
   const int d = blockIdx.x * 64 + lane_id(), w = wave_id();
-  const long long per = (rows + REC_SLICES - 1) / REC_SLICES, r0 = blockIdx.y * per;
+  const long long per = (rows + slices - 1) / slices, r0 = blockIdx.y * per;
   const long long r1 = r0 + per < rows ? r0 + per : rows;
   float b = 0.f, g = 0.f;
-  if (d < a.D) {
+  if (d < D) {
+#pragma unroll 8
     for (long long r = r0 + w; r < r1; r += 4) {
-      b += parts[r * a.D + d];
-      g += parts[(rows + r) * a.D + d];
+      b += parts[r * D + d];
+      g += parts[(rows + r) * D + d];
     }
   }
   s[0][w][lane_id()] = b;
   s[1][w][lane_id()] = g;
   __syncthreads();
-  if (w < 2 && d < a.D) {
+  if (w < 2 && d < D) {
     const int l = lane_id();
-    out[((long long)blockIdx.y * 2 + w) * a.D + d] = s[w][0][l] + s[w][1][l] + s[w][2][l] + s[w][3][l];
+    out[((long long)w * slices + blockIdx.y) * D + d] = s[w][0][l] + s[w][1][l] + s[w][2][l] + s[w][3][l];
   }
 }
 
-// The last sum, a wave a head: dt_bias' gradient a channel, A_log's a head.
-__global__ __launch_bounds__(64) void rec_sum_heads(RecArgs a, const float* part) {
-  const int h = blockIdx.x, per = a.D / a.H;
-  float s = 0.f;
-  for (int i = threadIdx.x; i < per; i += 64) {
-    const int d = h * per + i;
+// The last sum over n rows ([2][n][D]), a workgroup a head: dt_bias' gradient a
+// channel, A_log's the sum over the head's.
+__global__ __launch_bounds__(256) void rec_sum_heads(RecArgs a, const float* part, int n) {
+  __shared__ float s[2][4][64];
+  const int h = blockIdx.x, per = a.D / a.H, l = lane_id(), w = wave_id();
+  float sum = 0.f;
+  for (int i0 = 0; i0 < per; i0 += 64) {
+    const bool live = i0 + l < per;
+    const int d = h * per + (live ? i0 + l : 0);
     float b = 0.f, g = 0.f;
-    for (int k = 0; k < REC_SLICES; ++k) {
-      b += part[(k * 2LL) * a.D + d];
-      g += part[(k * 2LL + 1) * a.D + d];
+#pragma unroll 8
+    for (int k = w; k < n; k += 4) {
+      b += part[(long long)k * a.D + d];
+      g += part[(long long)(n + k) * a.D + d];
     }
-    a.ddt_bias[d] = b;
-    s += g;
+    __syncthreads();
+    s[0][w][l] = b;
+    s[1][w][l] = g;
+    __syncthreads();
+    if (w == 0 && live) {
+      a.ddt_bias[d] = s[0][0][l] + s[0][1][l] + s[0][2][l] + s[0][3][l];
+      sum += s[1][0][l] + s[1][1][l] + s[1][2][l] + s[1][3][l];
+    }
   }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, WAVE);
-  if (threadIdx.x == 0) a.dA_log[h] = s * 0.69314718055994531f;     // g2 -> g
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
+  if (threadIdx.x == 0) a.dA_log[h] = sum * 0.69314718055994531f;     // g2 -> g
 }
 
 // ---------------------------------------------------------------- one token
@@ -713,7 +742,7 @@ int vec_of(const RecArgs& a, size_t esz, std::initializer_list<const void*> ts,
 
 long long up(long long n, long long m) { return (n + m - 1) / m * m; }
 
-// The parts of ws (fp32 units): counter, (A, H) pairs, states at groups, runs of
+// The parts of ws (fp32 units): counters, (A, H) pairs, states at groups, runs of
 // packed rows, then the backward's sums over tokens a tile and over slices of them.
 struct Space {
   long long agg, base, runs, parts, sums, all, nchunk;
@@ -722,10 +751,10 @@ Space space(long long B, long long T, long long D, bool backward) {
   const long long len = backward ? SEG : REC_FSEG, wide = B * up(D, 128);
   Space s;
   s.nchunk = (T + W * len - 1) / (W * len);
-  s.agg = 16;
   const bool many = s.nchunk > 1;
+  s.agg = many ? B * ((D + 63) / 64) * LINE : 16;
   s.base = s.agg + (many ? 2 * s.nchunk * wide : 0);
-  s.runs = s.base + (many ? (s.nchunk / GROUP + 1) * wide : 0);
+  s.runs = s.base + (many ? (s.nchunk / W + 1) * wide : 0);
   s.parts = s.runs + (B == 1 ? 4 * ((T + len - 1) / len) : 0);
   s.sums = s.parts + (backward ? 2 * B * s.nchunk * D : 0);
   s.all = s.sums + (backward ? 2 * REC_SLICES * D : 0);
@@ -738,9 +767,14 @@ Sync prepare(const RecArgs& a, const Space& s, int len, const float* in, float* 
   y.nchunk = (int)s.nchunk;
   y.strips = (a.D + 64 * VEC - 1) / (64 * VEC);
   y.nstrip = y.strips * a.B;
+  // The larger group's fewer links pay where few strips go on at once and the
+  // chain sets the time, its looking at more tiles costs where it does not:
+  // 8 strips (16384 x 1024 packed, forward and backward) 149 us against 154,
+  // 64 strips (4 x 8192 x 2048) 383 against 371, 16 (65536 x 2048) 244 against 237
+  y.each = y.nstrip <= 8 ? 2 : 1;
   long long n16 = 0;
   if (s.nchunk > 1) {
-    y.ticket = reinterpret_cast<unsigned*>(a.ws);
+    y.ticket = reinterpret_cast<int*>(a.ws);
     y.agg = reinterpret_cast<unsigned long long*>(a.ws + s.agg);
     y.base = reinterpret_cast<unsigned*>(a.ws + s.base);
     n16 = (s.runs - s.agg) / 4;
@@ -748,11 +782,11 @@ Sync prepare(const RecArgs& a, const Space& s, int len, const float* in, float* 
   int4* runs = a.cu ? reinterpret_cast<int4*>(a.ws + s.runs) : nullptr;
   y.runs = runs;
   if (n16 || a.cu) {
-    long long n = n16;
+    long long n = std::max<long long>(n16, y.nstrip);
     if (a.cu) n = std::max(n, std::max((long long)(a.T + len - 1) / len, out ? (long long)a.S * a.D : 0));
     const unsigned grid = (unsigned)std::min<long long>((n + 255) / 256, 1024);
     hipLaunchKernelGGL(rec_init, dim3(grid), dim3(256), 0, st, a, reinterpret_cast<uint4*>(a.ws + s.agg),
-                       n16, y.ticket, runs, len, in, out);
+                       n16, y.ticket, y.ticket ? y.nstrip : 0, runs, len, in, out);
   }
   return y;
 }
@@ -775,10 +809,16 @@ hipError_t bwd(const RecArgs& a, hipStream_t st) {
   float* parts = a.ws + s.parts;
   if (a.cu) hipLaunchKernelGGL((rec_bwd_kernel<E, VEC, true>), grid, dim3(64 * W), 0, st, a, y, parts);
   else hipLaunchKernelGGL((rec_bwd_kernel<E, VEC, false>), grid, dim3(64 * W), 0, st, a, y, parts);
-  float* sums = a.ws + s.sums;
-  hipLaunchKernelGGL(rec_sum_runs, dim3((a.D + 63) / 64, REC_SLICES), dim3(256), 0, st, a,
-                     (const float*)parts, s.nchunk * a.B, sums);
-  hipLaunchKernelGGL(rec_sum_heads, dim3(a.H), dim3(64), 0, st, a, (const float*)sums);
+  // many tiles: first slices of them, over the whole card
+  const long long rows = s.nchunk * a.B;
+  if (rows > REC_SLICES) {
+    float* sums = a.ws + s.sums;
+    hipLaunchKernelGGL(rec_sum_runs, dim3((a.D + 63) / 64, REC_SLICES), dim3(256), 0, st, (const float*)parts,
+                       rows, a.D, REC_SLICES, sums);
+    hipLaunchKernelGGL(rec_sum_heads, dim3(a.H), dim3(256), 0, st, a, (const float*)sums, REC_SLICES);
+  } else {
+    hipLaunchKernelGGL(rec_sum_heads, dim3(a.H), dim3(256), 0, st, a, (const float*)parts, (int)rows);
+  }
   return hipGetLastError();
 }
 
