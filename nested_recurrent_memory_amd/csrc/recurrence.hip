@@ -219,11 +219,22 @@ __device__ __forceinline__ void publish(unsigned* p, float h) {
   __hip_atomic_store(p, bits(h) == ~0u ? 0x7fc00000u : bits(h), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 template <typename U>
-__device__ __forceinline__ U await(const U* p) {
-  U v;
-  while ((v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) == (U)~(U)0)
+__device__ __forceinline__ U peek(const U* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// v[i] (of a peek) until all are there; a look takes a microsecond, so all VEC
+// at once
+template <int VEC, typename U>
+__device__ __forceinline__ void await(const U* p, U* v) {
+  while (true) {
+    bool there = true;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) there = there && v[i] != (U)~(U)0;
+    if (there) return;
     __builtin_amdgcn_s_sleep(1);
-  return v;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = peek(p + i);
+  }
 }
 
 template <int VEC>
@@ -265,19 +276,51 @@ __device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int ste
     float bA[VEC], bH[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) { bA[i] = 1.f; bH[i] = 0.f; }
-    for (int k = wv * y.each; k < (wv + 1) * y.each && k < n; ++k) {
+    const int k0 = wv * y.each, k1 = k0 + 1;
+    const bool one = k0 < n, two = y.each > 1 && k1 < n, far = wv == W - 1 && g0 > 0;
+    unsigned long long v0[VEC], v1[VEC];
+    unsigned hb[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const unsigned long long v = await(agg(g0 + k) + i);
-        join<PACKED>(bA[i], bH[i], __uint_as_float((unsigned)(v >> 32)), __uint_as_float((unsigned)v));
-      }
+    for (int i = 0; i < VEC; ++i) {
+      v0[i] = one ? peek(agg(g0 + k0) + i) : 0;
+      v1[i] = two ? peek(agg(g0 + k1) + i) : 0;
+      hb[i] = far ? peek(base(g0 / group) + i) : bits(first[i]);
     }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s.before[wv][l * VEC + i] = make_float2(bA[i], bH[i]);
-    if (wv == W - 1) {
+    auto add = [&](int k, unsigned long long* v) {
+      await<VEC>(agg(g0 + k), v);
 #pragma unroll
       for (int i = 0; i < VEC; ++i)
-        s.base[l * VEC + i] = g0 > 0 ? __uint_as_float(await(base(g0 / group) + i)) : first[i];
+        join<PACKED>(bA[i], bH[i], __uint_as_float((unsigned)(v[i] >> 32)), __uint_as_float((unsigned)v[i]));
+    };
+    if (one) add(k0, v0);
+    if (two) add(k1, v1);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s.before[wv][l * VEC + i] = make_float2(bA[i], bH[i]);
+    // the group's last tile is a link of the chain: everything up to its own end is
+    // joined before the state at g0 is there, which then goes on in one operation
+    const bool link = n == group - 1 && step + 1 < y.nchunk;
+    if (link) lds_barrier();
+    if (wv == W - 1) {
+      float gA[VEC], gH[VEC];
+      if (link) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          gA[i] = 1.f;
+          gH[i] = 0.f;
+          for (int k = 0; k * y.each < n; ++k) {
+            const float2 v = s.before[k][l * VEC + i];
+            join<PACKED>(gA[i], gH[i], v.x, v.y);
+          }
+          join<PACKED>(gA[i], gH[i], tA[i], tH[i]);
+        }
+      }
+      if (far) await<VEC>(base(g0 / group), hb);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float h0 = __uint_as_float(hb[i]);
+        if (link) publish(base(g0 / group + 1) + i, pass<PACKED>(h0, gA[i], gH[i]));
+        s.base[l * VEC + i] = h0;
+      }
     }
     lds_barrier();
 #pragma unroll
@@ -291,10 +334,6 @@ __device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int ste
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) h[i] = first[i];
-  }
-  if (more && wv == W - 1 && n == group - 1 && step + 1 < y.nchunk) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) publish(base(g0 / group + 1) + i, pass<PACKED>(h[i], tA[i], tH[i]));
   }
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
