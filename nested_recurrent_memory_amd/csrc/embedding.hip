@@ -50,9 +50,10 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a, int lg) {
 // stable radix sort of (id, position), from the low digit up. Ids that get no
 // gradient sort behind the others, as V. Up to ONE ids one workgroup sorts in
 // LDS; above, every pass is a count and a scatter over blocks of BLOCK ids.
-// Every launch of the sort also clears a share of dw with workgroups of its
-// own: the sort waits on latency, the clearing on HBM, and the rows with a sum
-// are written after both.
+// Every launch of the sort also clears a share of dw's last rows with workgroups
+// of its own: the sort waits on latency, the clearing on HBM, and the rows with a
+// sum are written after both. What does not fit beside the sort is cleared beside
+// the sums, there only the rows without one (embed_sum).
 
 namespace {
 
@@ -238,10 +239,17 @@ __global__ __launch_bounds__(ST) void embed_scatter(SortArgs s) {
   }
   int all = 0, before = 0;
   if (threadIdx.x < BUCKETS) {
-    for (int b = 0; b < s.nblock; ++b) {
-      const int c = s.table[b * BUCKETS + threadIdx.x];
-      all += c;
-      before += b < (int)blockIdx.x ? c : 0;
+    // 16 loads ahead of their additions: one at a time, beside the clearing, a
+    // table of 32 blocks took 50 us to add
+    for (int b = 0; b < s.nblock; b += 16) {
+      int c[16];
+#pragma unroll
+      for (int u = 0; u < 16; ++u) c[u] = b + u < s.nblock ? s.table[(b + u) * BUCKETS + threadIdx.x] : 0;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) {
+        all += c[u];
+        before += b + u < (int)blockIdx.x ? c[u] : 0;
+      }
     }
   }
   rank_keys<ROUNDS>(key, rank, s.shift, s.bits, s_count, s_total);
@@ -274,12 +282,43 @@ struct EmbedSum {
   float* parts;
   int* owners;
   int N, V, D, seg, nseg, tiles;
+  int sums;               // workgroups that sum; those behind clear rows [0, rows) that no id has
+  int rows;
   float scale;
 };
+
+// Rows of dw that no sorted key is: a wave looks for ROWS of them at once.
+constexpr int ROWS = 16;
+template <typename T, int VEC>
+__device__ __forceinline__ void clear_rows(const EmbedSum& a, int wave) {
+  const int l = lane_id(), v0 = wave * ROWS;
+  bool gone = false;
+  if (l < ROWS && v0 + l < a.rows) {
+    int lo = 0, hi = a.N;
+    while (lo < hi) {
+      const int m = (lo + hi) / 2;
+      if (a.key[m] < v0 + l) lo = m + 1; else hi = m;
+    }
+    gone = lo == a.N || a.key[lo] != v0 + l;
+  }
+  unsigned long long m = __ballot(gone);
+  float zero[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) zero[e] = 0.f;
+  while (m) {
+    T* row = static_cast<T*>(a.dw) + (long long)(v0 + __builtin_ctzll(m)) * a.D;
+    m &= m - 1;
+    for (int c = l * VEC; c < a.D; c += WAVE * VEC) put<T, VEC>(row + c, zero);
+  }
+}
 
 template <typename G, typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_sum(EmbedSum a) {
   constexpr int AHEAD = 8;                    // rows loaded before the first is added
+  if ((int)blockIdx.x >= a.sums) {
+    clear_rows<T, VEC>(a, (blockIdx.x - a.sums) * 4 + wave_id());
+    return;
+  }
   const long long item = (long long)blockIdx.x * 4 + wave_id();
   const int k = (int)(item / a.tiles), l = lane_id();
   if (k >= a.nseg) return;
@@ -390,7 +429,11 @@ struct Space {
 Space space(long long N, long long V, long long D) {
   Space s;
   s.nblock = (int)((N + BLOCK - 1) / BLOCK);
+  // Long segments leave fewer parts, short ones more waves: the longest that gives
+  // 16 waves a CU at 512 columns a wave. 131072 x 2048: sums and joining 226 us with
+  // segments of 64, 247 with 32, 272 with 16
   s.seg = 16;
+  while (s.seg < WAVE && (N / (2 * s.seg)) * ((D + 511) / 512) >= 4096) s.seg *= 2;
   s.nseg = (int)((N + s.seg - 1) / s.seg);
   s.pos0 = up4(N);
   s.key1 = s.pos0 + up4(N);
@@ -416,7 +459,7 @@ hipError_t fwd(const EmbedArgs& a, hipStream_t st) {
 }
 
 template <typename G, typename W, int VEC>
-hipError_t sum(const EmbedArgs& a, const Space& s, const int* key, const int* pos, hipStream_t st) {
+hipError_t sum(const EmbedArgs& a, const Space& s, const int* key, const int* pos, int rows, hipStream_t st) {
   EmbedSum m{};
   m.key = key;
   m.pos = pos;
@@ -425,8 +468,9 @@ hipError_t sum(const EmbedArgs& a, const Space& s, const int* key, const int* po
   m.owners = a.ws + s.owners;
   m.N = (int)a.N; m.V = (int)a.V; m.D = a.D; m.seg = s.seg; m.nseg = s.nseg; m.scale = a.scale;
   m.tiles = (a.D + WAVE * VEC - 1) / (WAVE * VEC);
-  const long long items = (long long)m.nseg * m.tiles;
-  hipLaunchKernelGGL((embed_sum<G, W, VEC>), dim3((unsigned)((items + 3) / 4)), dim3(256), 0, st, m);
+  m.sums = (int)(((long long)m.nseg * m.tiles + 3) / 4);
+  m.rows = rows;
+  hipLaunchKernelGGL((embed_sum<G, W, VEC>), dim3(m.sums + (rows + 4 * ROWS - 1) / (4 * ROWS)), dim3(256), 0, st, m);
   if (m.nseg > 1) {
     const unsigned rows = (unsigned)std::min(m.nseg - 1, std::max(1, 1024 / m.tiles));
     hipLaunchKernelGGL((embed_join<W, VEC>), dim3(m.tiles, rows), dim3(256), 0, st, m);
@@ -437,7 +481,11 @@ hipError_t sum(const EmbedArgs& a, const Space& s, const int* key, const int* po
 template <typename G, typename W>
 hipError_t bwd(const EmbedArgs& a, hipStream_t st) {
   const Space s = space(a.N, a.V, a.D);
-  const long long bytes = a.V * a.D * (long long)sizeof(W), words = bytes / 16;
+  // what is cleared beside the sort: 128 MiB take about as long as it does
+  constexpr long long BESIDE = 128LL << 20;
+  const long long row = a.D * (long long)sizeof(W), bytes = a.V * row, all = bytes / 16;
+  const int rows = a.N == 0 || bytes <= BESIDE ? 0 : (int)(a.V - BESIDE / row);
+  const long long from = rows * row / 16, words = all - from;
   int bits = 1;
   while ((1LL << bits) <= a.V) ++bits;               // ids 0..V
   SortArgs r{};
@@ -447,23 +495,24 @@ hipError_t bwd(const EmbedArgs& a, hipStream_t st) {
   r.table = a.ws + s.table;
   r.owners = a.ws + s.owners;
   r.dw = static_cast<uint4*>(a.dw);
-  r.tail = reinterpret_cast<unsigned short*>(static_cast<char*>(a.dw) + words * 16);
+  r.tail = reinterpret_cast<unsigned short*>(static_cast<char*>(a.dw) + all * 16);
   r.N = (int)a.N; r.V = (int)a.V;
   r.pad = a.padding_idx >= 0 && a.padding_idx < a.V ? (int)a.padding_idx : -1;
   r.passes = (bits + DIGIT - 1) / DIGIT;
   r.bits = (bits + r.passes - 1) / r.passes;
   const int clears = (int)std::min<long long>(512, (words + ST - 1) / ST + 1);
   const int *key = r.key[0], *pos = r.pos[0];
-  r.w1 = words;
-  r.tails = (int)(bytes - words * 16) / 2;
+  r.w0 = from;
+  r.w1 = all;
+  r.tails = (int)(bytes - all * 16) / 2;
   if (a.N <= ONE) {
     hipLaunchKernelGGL(embed_sort_one, dim3(1 + clears), dim3(ST), 0, st, r);
   } else {
     r.nblock = s.nblock;
     const int launches = 2 * r.passes;
     for (int p = 0; p < launches; ++p) {
-      r.w0 = words * p / launches;
-      r.w1 = words * (p + 1) / launches;
+      r.w0 = from + words * p / launches;
+      r.w1 = from + words * (p + 1) / launches;
       r.shift = p / 2 * r.bits;
       if (p % 2 == 0) {
         hipLaunchKernelGGL(embed_count, dim3(s.nblock + clears), dim3(ST), 0, st, r);
@@ -479,8 +528,8 @@ hipError_t bwd(const EmbedArgs& a, hipStream_t st) {
   if (a.N == 0) return hipGetLastError();
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dw) |
                        reinterpret_cast<uintptr_t>(a.ws);
-  if (a.D % 8 == 0 && at % 16 == 0) return sum<G, W, 8>(a, s, key, pos, st);
-  return sum<G, W, 1>(a, s, key, pos, st);
+  if (a.D % 8 == 0 && at % 16 == 0) return sum<G, W, 8>(a, s, key, pos, rows, st);
+  return sum<G, W, 1>(a, s, key, pos, rows, st);
 }
 
 }  // namespace

@@ -89,6 +89,28 @@ def test_large_vocabulary():
     check_grad(dw, ids, dy, V, 1.0)
 
 
+@pytest.mark.parametrize("N", [1, 3000, 20000])
+@pytest.mark.parametrize("V,D,dtype", [(70001, 515, torch.float32), (70001, 520, torch.float32),
+                                       (66001, 1031, torch.bfloat16)])
+def test_large_gradient_is_written_whole(N, V, D, dtype):
+    """A table of more than 128 MiB, part of it cleared beside the sums: every row,
+    ids at both ends, between and together, and rows of any alignment."""
+    g = torch.Generator().manual_seed(N + D)
+    ids = torch.randint(0, V, (N,), generator=g)
+    for i, v in enumerate((0, V - 1, 1, 15, 16, 17, V // 2, 3, 3)):
+        if i < N:
+            ids[i] = v
+    ids, dy = ids.cuda(), torch.randint(-8, 9, (N, D), generator=g).to(dtype).cuda()
+    w = torch.zeros(V, D, dtype=dtype, device="cuda", requires_grad=True)
+    junk = torch.full((V, D), 7.0, dtype=dtype, device="cuda")      # freed: what dw is made of
+    y = embedding(ids, w)
+    del junk
+    dw, = torch.autograd.grad(y, w, dy)
+    # whole numbers below 2^8 rows each: every sum is exact in fp32 and rounded once
+    want = torch.zeros(V, D, dtype=torch.float32, device="cuda").index_add_(0, ids, dy.float())
+    assert torch.equal(dw, want.to(dtype))
+
+
 def test_ids_of_any_shape_and_type():
     ids, w, _ = make(24, 9, 16, torch.float32, torch.float32)
     wg = w.cuda()
