@@ -417,6 +417,70 @@ __global__ __launch_bounds__(256) void embed_join(EmbedSum a) {
   }
 }
 
+// The whole gradient of at most FEW ids in one launch: a workgroup has HAND rows
+// of dw, looks all ids over for them, and its waves take the rows' tiles of 64
+// VEC columns in turn, to clear them or to add what points at them.
+constexpr int FEW = 256, HAND = 16;
+template <typename G, typename T, int VEC>
+__global__ __launch_bounds__(FEW) void embed_few(EmbedArgs a) {
+  constexpr int AHEAD = 8;
+  __shared__ int s_row[FEW], s_at[FEW], s_pos[FEW], s_count[FEW / WAVE], s_first[HAND + 1];
+  const int l = lane_id(), w = wave_id(), n = threadIdx.x;
+  const long long v0 = (long long)blockIdx.x * HAND;
+  const long long id = n < a.N ? a.ids[n] : -1;
+  const bool mine = id >= v0 && id < v0 + HAND && id < a.V && id != a.padding_idx;
+  const unsigned long long m = __ballot(mine);
+  if (l == 0) s_count[w] = __popcll(m);
+  __syncthreads();
+  int at = __popcll(m & ((1ull << l) - 1)), count = 0;
+#pragma unroll
+  for (int k = 0; k < FEW / WAVE; ++k) {
+    at += k < w ? s_count[k] : 0;
+    count += s_count[k];
+  }
+  if (mine) {
+    s_row[at] = (int)(id - v0);
+    s_at[at] = n;
+  }
+  __syncthreads();
+  // by row, in the order of their positions within one
+  if (n < count) {
+    int rank = 0;
+    for (int k = 0; k < count; ++k) rank += s_row[k] < s_row[n] || (s_row[k] == s_row[n] && k < n);
+    s_pos[rank] = s_at[n];
+  }
+  if (n <= HAND) {
+    int first = 0;
+    for (int k = 0; k < count; ++k) first += s_row[k] < n;
+    s_first[n] = first;
+  }
+  __syncthreads();
+  const int tiles = (a.D + WAVE * VEC - 1) / (WAVE * VEC);
+  const int rows = a.V - v0 < HAND ? (int)(a.V - v0) : HAND;
+  for (int item = w; item < rows * tiles; item += FEW / WAVE) {
+    const int r = item / tiles, c = (item % tiles * WAVE + l) * VEC;
+    if (c >= a.D) continue;
+    const G* dy = static_cast<const G*>(a.dy) + c;
+    const int k1 = s_first[r + 1];
+    float acc[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    for (int k = s_first[r]; k < k1; k += AHEAD) {
+      float v[AHEAD][VEC];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) get<G, VEC>(dy + (long long)s_pos[k + u < k1 ? k + u : k1 - 1] * a.D, v[u]);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (k + u < k1)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] += v[u][e];
+    }
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] *= a.scale;
+    put<T, VEC>(static_cast<T*>(a.dw) + (v0 + r) * a.D + c, acc);
+  }
+}
+
 namespace {
 
 long long up4(long long n) { return (n + 3) / 4 * 4; }
@@ -480,11 +544,20 @@ hipError_t sum(const EmbedArgs& a, const Space& s, const int* key, const int* po
 
 template <typename G, typename W>
 hipError_t bwd(const EmbedArgs& a, hipStream_t st) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dw) |
+                       reinterpret_cast<uintptr_t>(a.ws);
+  const bool vec = a.D % 8 == 0 && at % 16 == 0;
+  if (a.N <= FEW) {
+    const dim3 grid((unsigned)((a.V + HAND - 1) / HAND));
+    if (vec) hipLaunchKernelGGL((embed_few<G, W, 8>), grid, dim3(FEW), 0, st, a);
+    else hipLaunchKernelGGL((embed_few<G, W, 1>), grid, dim3(FEW), 0, st, a);
+    return hipGetLastError();
+  }
   const Space s = space(a.N, a.V, a.D);
   // what is cleared beside the sort: 128 MiB take about as long as it does
   constexpr long long BESIDE = 128LL << 20;
   const long long row = a.D * (long long)sizeof(W), bytes = a.V * row, all = bytes / 16;
-  const int rows = a.N == 0 || bytes <= BESIDE ? 0 : (int)(a.V - BESIDE / row);
+  const int rows = bytes <= BESIDE ? 0 : (int)(a.V - BESIDE / row);
   const long long from = rows * row / 16, words = all - from;
   int bits = 1;
   while ((1LL << bits) <= a.V) ++bits;               // ids 0..V
@@ -525,10 +598,7 @@ hipError_t bwd(const EmbedArgs& a, hipStream_t st) {
     key = r.key[0];
     pos = r.pos[0];
   }
-  if (a.N == 0) return hipGetLastError();
-  const uintptr_t at = reinterpret_cast<uintptr_t>(a.dy) | reinterpret_cast<uintptr_t>(a.dw) |
-                       reinterpret_cast<uintptr_t>(a.ws);
-  if (a.D % 8 == 0 && at % 16 == 0) return sum<G, W, 8>(a, s, key, pos, rows, st);
+  if (vec) return sum<G, W, 8>(a, s, key, pos, rows, st);
   return sum<G, W, 1>(a, s, key, pos, rows, st);
 }
 

@@ -73,7 +73,7 @@ def _embed(t):
 def _lookup(ids, weight, scale, ydt):
     w = _embed(weight)
     V, D = w.shape
-    y = torch.empty((*ids.shape, D), device=w.device, dtype=ydt if ydt in _EMBED else torch.float32)
+    y = w.new_empty((*ids.shape, D), dtype=ydt if ydt in _EMBED else torch.float32)
     N = ids.numel()
     if N:
         _lib.on_device(w, "ngdn_embedding_fwd", _code(w), _code(y), N, V, D, scale, ids.data_ptr(),
@@ -84,8 +84,8 @@ def _lookup(ids, weight, scale, ydt):
 def _lookup_grad(ids, dy, scale, padding_idx, V, wdt):
     g = _embed(dy)
     N, D = ids.numel(), dy.shape[-1]
-    dw = torch.empty((V, D), device=g.device, dtype=wdt if wdt in _EMBED else torch.float32)
-    ws = torch.empty(_lib.lib().ngdn_embedding_ws(N, V, D), device=g.device, dtype=torch.int32)
+    dw = g.new_empty((V, D), dtype=wdt if wdt in _EMBED else torch.float32)
+    ws = ids.new_empty((_lib.lib().ngdn_embedding_ws(N, V, D) + 1) // 2)
     _lib.on_device(g, "ngdn_embedding_bwd", _code(g), _code(dw), N, V, D, scale,
                    -1 if padding_idx is None else padding_idx, ids.data_ptr(), g.data_ptr(),
                    dw.data_ptr(), ws.data_ptr())
