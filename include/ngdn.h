@@ -628,7 +628,7 @@ int64_t ngdn_embedding_ws(int64_t N, int64_t V, int32_t D);
  * and, fp32, ddt_bias [D], dA_log [H] and dh0. ws: ngdn_recurrence_ws(...)
  * fp32, no initial contents. Sums over tokens are in a fixed order: the same
  * inputs give the same bits. */
-#define NGDN_REC_RUN 8
+#define NGDN_REC_RUN 16
 typedef struct ngdn_recurrence_args {
   int32_t B, T, D, H, S;
   int64_t x_b, x_t, f_b, f_t, w_b, w_t, dy_b, dy_t;

@@ -34,7 +34,7 @@ P = ctypes.c_void_p
 I32 = ctypes.c_int32
 I64 = ctypes.c_int64
 WPARTS = 1024         # NGDN_WPARTS: rows of partial weight-gradient sums in the ws arguments
-REC_RUN = 8           # NGDN_REC_RUN: tokens a run of the gated recurrence's saved states
+REC_RUN = 16          # NGDN_REC_RUN: tokens a run of the gated recurrence's saved states
 PARAM_SPLIT = 16      # NGDN_PARAM_SPLIT: slices of firings per head in ngdn_param_grads
 PD = ctypes.POINTER(Dims)
 

@@ -492,12 +492,11 @@ hipError_t l0_bwd_intra(const L0BwdIntraArgs& a, int dtype, int K, int V, hipStr
 hipError_t l0_bwd_fused(const L0BwdIntraArgs& a, int dtype, int K, int V, hipStream_t st);
 
 // The gated linear recurrence (recurrence.hip); what each field holds is at
-// ngdn_recurrence_args in ngdn.h. A wave has REC_FSEG tokens in the forward,
-// REC_SEG in the backward (the tokens between the states it reads), a
+// ngdn_recurrence_args in ngdn.h. A wave has a run of REC_RUN tokens, a
 // workgroup REC_WAVES waves; the parameter gradients' sums over tokens are cut
 // into REC_SLICES.
 using RecArgs = ngdn_recurrence_args;
-constexpr int REC_SEG = NGDN_REC_RUN, REC_FSEG = 16, REC_WAVES = 8;
+constexpr int REC_RUN = NGDN_REC_RUN, REC_WAVES = 8;
 constexpr int REC_SLICES = 32;
 int64_t rec_ws(int64_t B, int64_t T, int64_t D, bool backward);
 hipError_t rec_fwd(const RecArgs& a, int dtype, hipStream_t st);

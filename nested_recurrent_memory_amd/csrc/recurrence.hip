@@ -12,7 +12,6 @@
 // runs are formed from zero in registers, joined in order, and completed from
 // the state that enters them.
 #include <algorithm>
-#include <initializer_list>
 
 #include "ngdn_kernels.h"
 
@@ -20,7 +19,7 @@ namespace ngdn {
 
 namespace {
 
-constexpr int SEG = REC_SEG;
+constexpr int N = REC_RUN;          // tokens a run, which a wave has in registers
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -76,30 +75,6 @@ __device__ __forceinline__ void root(float q, float& beta, float& inv) {
   beta = q * inv;
 }
 
-template <typename E, int VEC>
-__device__ __forceinline__ void loadv(const E* p, float* o) {
-  if constexpr (VEC == 1) {
-    o[0] = to_f(*p);
-  } else {
-    struct alignas(VEC * sizeof(E)) Pack { E v[VEC]; };
-    const Pack k = *reinterpret_cast<const Pack*>(p);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = to_f(k.v[i]);
-  }
-}
-template <typename E, int VEC>
-__device__ __forceinline__ void storev(E* p, const float* x) {
-  if constexpr (VEC == 1) {
-    *p = from_f<E>(x[0]);
-  } else {
-    struct alignas(VEC * sizeof(E)) Pack { E v[VEC]; };
-    Pack k;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) k.v[i] = from_f<E>(x[i]);
-    *reinterpret_cast<Pack*>(p) = k;
-  }
-}
-
 // Where the tokens [t0, t0 + n) of a packed row stand: bit j of start / end /
 // used says whether token t0 + j is the first / the last of its sequence / in
 // one at all; cur is the sequence of token t0 (or the one before it), last that
@@ -152,25 +127,23 @@ __device__ __forceinline__ int seq_before(const int* cu, int S, int cur, int t) 
   return cur < S ? cur : S - 1;
 }
 
-template <int VEC>
-__device__ __forceinline__ void params(const RecArgs& a, long long d, float* bias2, float* nrate) {
-  const int per = a.D / a.H;
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    bias2[i] = a.dt_bias[d + i] * LOG2E;
-    nrate[i] = -__builtin_amdgcn_exp2f(a.A_log[(d + i) / per] * LOG2E);
-  }
+// bias2 and nrate of a channel
+__device__ __forceinline__ void params(const RecArgs& a, unsigned d, float& bias2, float& nrate) {
+  bias2 = a.dt_bias[d] * LOG2E;
+  nrate = -__builtin_amdgcn_exp2f(a.A_log[d / (unsigned)(a.D / a.H)] * LOG2E);
 }
 
 // ---------------------------------------------------------------- joining runs
 //
-// A workgroup has W waves, each a run of tokens of 64 VEC channels: a tile of
-// W runs. The state that enters a tile comes from the tiles before it (in the
-// backward: behind it) while those are still running, through device memory:
-// every tile publishes its (A, H) as soon as it has them; the last of a group of
-// W or 2 W also the state behind it. A tile takes the state at its group's start
-// and the (A, H) of the tiles between, so the chain over a long row has a link a
-// group, and the order of the arithmetic does not depend on timing.
+// A workgroup has W waves, each a run of N tokens of 64 channels (a strip): a
+// tile of W runs. The state that enters a tile comes from the tiles before it (in
+// the backward: behind it) while those are still running, through device memory:
+// every tile publishes its (A, H) as soon as it has them; the last of a group of W
+// also the state behind it. A tile takes the state at its group's start and the
+// (A, H) of the tiles between, a wave each, so the chain over a long row has a
+// link a group, and the order of the arithmetic does not depend on timing. Groups
+// of 2 W: 16384 x 512 forward 25.0 us against 26.2, 4 x 6000 x 2048 98.3 against
+// 97.4, within noise elsewhere.
 // One 64-bit (32-bit) value is its own flag: all bits set before it is
 // published, which no published value has (a NaN of that pattern is changed).
 // A strip's tiles are handed out by a counter, so all a tile waits for was
@@ -178,18 +151,22 @@ __device__ __forceinline__ void params(const RecArgs& a, long long d, float* bia
 // A counter for each strip: 512 workgroups that start together on one counter
 // take 6 us to get their numbers.
 // Against reducing, joining and applying in three launches: inputs are read
-// and their gates computed once instead of twice.
+// and their gates computed once instead of twice (65536 x 2048 bf16 forward
+// 1900 us, then 250).
+// One channel a lane leaves room for four workgroups a CU, whose loading,
+// computing and waiting overlap; with two channels (4-byte loads of bf16) two
+// fit: 16384 x 1024 packed, both passes, 146 us against 135, 333 x 1024 forward
+// 13.7 against 11.1, only the longest forward gains (65536 x 2048 234 against 243).
 
 constexpr int W = REC_WAVES;
 constexpr int LINE = 32;            // ints in a cache line
 
 struct Sync {
   int* ticket;                      // [nstrip] counters, LINE apart (NULL: one tile a row, nothing to join)
-  unsigned long long* agg;          // [nchunk][nstrip][64 VEC] (A, H)
-  unsigned* base;                   // [groups][nstrip][64 VEC]
+  unsigned long long* agg;          // [nchunk][nstrip][64] (A, H)
+  unsigned* base;                   // [groups][nstrip][64]
   const int4* runs;                 // packed rows: every run's Run
   int nchunk, nstrip, strips;       // nstrip = B strips
-  int each;                         // tiles of a group for each wave to look at, 1 or 2
 };
 
 __device__ __forceinline__ unsigned bits(float x) { return __float_as_uint(x); }
@@ -197,18 +174,18 @@ constexpr unsigned RESET = 0x80000000u;      // A = -0: nothing before passes (a
 
 // (A2, H2) after (A1, H1); a reset keeps what is not finite before it out
 template <bool PACKED>
-__device__ __forceinline__ void join(float& A1, float& H1, float A2, float H2) {
-  if (PACKED && bits(A2) == RESET) {
-    A1 = A2;
-    H1 = H2;
+__device__ __forceinline__ void join(float& A1, float& H1, float2 v) {
+  if (PACKED && bits(v.x) == RESET) {
+    A1 = v.x;
+    H1 = v.y;
   } else {
-    H1 = fmaf(A2, H1, H2);
-    A1 = PACKED && bits(A1) == RESET ? A1 : A1 * A2;
+    H1 = fmaf(v.x, H1, v.y);
+    A1 = PACKED && bits(A1) == RESET ? A1 : A1 * v.x;
   }
 }
 template <bool PACKED>
-__device__ __forceinline__ float pass(float h, float A, float H) {
-  return PACKED && bits(A) == RESET ? H : fmaf(A, h, H);
+__device__ __forceinline__ float pass(float h, float2 v) {
+  return PACKED && bits(v.x) == RESET ? v.y : fmaf(v.x, h, v.y);
 }
 
 __device__ __forceinline__ void publish(unsigned long long* p, float A, float H) {
@@ -222,126 +199,74 @@ template <typename U>
 __device__ __forceinline__ U peek(const U* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// v[i] (of a peek) until all are there; a look takes a microsecond, so all VEC
-// at once
-template <int VEC, typename U>
-__device__ __forceinline__ void await(const U* p, U* v) {
-  while (true) {
-    bool there = true;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) there = there && v[i] != (U)~(U)0;
-    if (there) return;
+template <typename U>
+__device__ __forceinline__ U await(const U* p, U v) {
+  while (v == (U)~(U)0) {
     __builtin_amdgcn_s_sleep(1);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = peek(p + i);
+    v = peek(p);
   }
+  return v;
+}
+__device__ __forceinline__ float2 pair(unsigned long long v) {
+  return make_float2(__uint_as_float((unsigned)(v >> 32)), __uint_as_float((unsigned)v));
 }
 
-template <int VEC>
 struct Joint {
-  float2 wave[W][64 * VEC];         // (A, H) of the tile's waves, in the order of the scan
-  float2 before[W][64 * VEC];       // of up to two tiles before it each
-  float base[64 * VEC];
+  float2 wave[W][64];               // (A, H) of the tile's waves, in the order of the scan
+  float2 before[W][64];             // of the group's tiles before it
+  float base[64];
+  int step;
 };
 
-// From wave (A, H) to the state h entering the wave. step: the tile's place in
-// the scan's order (0 first), wv the wave's. first: the state entering tile 0.
-template <bool PACKED, int VEC>
-__device__ __forceinline__ void join_tiles(Joint<VEC>& s, const Sync& y, int step, int strip, int wv,
-                                           const float* A, const float* H, const float* first, float* h) {
+// From wave (A, H) to the state entering the wave. step: the tile's place in the
+// scan's order (0 first), wv the wave's. first: the state entering tile 0.
+template <bool PACKED>
+__device__ __forceinline__ float join_tiles(Joint& s, const Sync& y, int step, int strip, int wv, float A, float H,
+                                            float first) {
   const int l = lane_id();
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) s.wave[wv][l * VEC + i] = make_float2(A[i], H[i]);
+  s.wave[wv][l] = make_float2(A, H);
   lds_barrier();
-  const int group = y.each * W, g0 = step / group * group, n = step - g0;   // n tiles from the group's start
-  const bool more = y.ticket != nullptr;
-  auto agg = [&](int k) { return y.agg + ((long long)k * y.nstrip + strip) * (64 * VEC) + l * VEC; };
-  auto base = [&](int k) { return y.base + ((long long)k * y.nstrip + strip) * (64 * VEC) + l * VEC; };
-  float tA[VEC], tH[VEC];                                   // the whole tile
-  if (more && wv == W - 1 && step + 1 < y.nchunk) {
+  float h = first;
+  if (y.ticket) {
+    const int group = step / W, n = step - group * W;         // n tiles from the group's start
+    const bool go = step + 1 < y.nchunk, link = n == W - 1 && go;
+    auto agg = [&](int k) { return y.agg + ((long long)k * y.nstrip + strip) * 64 + l; };
+    auto base = [&](int k) { return y.base + ((long long)k * y.nstrip + strip) * 64 + l; };
+    float tA = 1.f, tH = 0.f;                                 // the whole tile
+    if (wv == W - 1 && go) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      tA[i] = 1.f;
-      tH[i] = 0.f;
-      for (int k = 0; k < W; ++k) {
-        const float2 v = s.wave[k][l * VEC + i];
-        join<PACKED>(tA[i], tH[i], v.x, v.y);
+      for (int k = 0; k < W; ++k) join<PACKED>(tA, tH, s.wave[k][l]);
+      publish(agg(step), tA, tH);
+    }
+    if (step > 0) {
+      // each wave one of the n tiles, the last, which has none, the state at the
+      // group's start, which it looks at before it waits for the tiles
+      const bool one = wv < n, far = wv == W - 1 && group > 0;
+      const unsigned hb = far ? peek(base(group)) : bits(first);
+      if (one) {
+        const unsigned long long* p = agg(group * W + wv);
+        s.before[wv][l] = pair(await(p, peek(p)));
       }
-      publish(agg(step) + i, tA[i], tH[i]);
-    }
-  }
-  if (more && step > 0) {
-    // wave wv: `each` of the n tiles; the last wave, which has one less, also the
-    // state at g0
-    float bA[VEC], bH[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) { bA[i] = 1.f; bH[i] = 0.f; }
-    const int k0 = wv * y.each, k1 = k0 + 1;
-    const bool one = k0 < n, two = y.each > 1 && k1 < n, far = wv == W - 1 && g0 > 0;
-    unsigned long long v0[VEC], v1[VEC];
-    unsigned hb[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      v0[i] = one ? peek(agg(g0 + k0) + i) : 0;
-      v1[i] = two ? peek(agg(g0 + k1) + i) : 0;
-      hb[i] = far ? peek(base(g0 / group) + i) : bits(first[i]);
-    }
-    auto add = [&](int k, unsigned long long* v) {
-      await<VEC>(agg(g0 + k), v);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        join<PACKED>(bA[i], bH[i], __uint_as_float((unsigned)(v[i] >> 32)), __uint_as_float((unsigned)v[i]));
-    };
-    if (one) add(k0, v0);
-    if (two) add(k1, v1);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s.before[wv][l * VEC + i] = make_float2(bA[i], bH[i]);
-    // the group's last tile is a link of the chain: everything up to its own end is
-    // joined before the state at g0 is there, which then goes on in one operation
-    const bool link = n == group - 1 && step + 1 < y.nchunk;
-    if (link) lds_barrier();
-    if (wv == W - 1) {
-      float gA[VEC], gH[VEC];
-      if (link) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          gA[i] = 1.f;
-          gH[i] = 0.f;
-          for (int k = 0; k * y.each < n; ++k) {
-            const float2 v = s.before[k][l * VEC + i];
-            join<PACKED>(gA[i], gH[i], v.x, v.y);
-          }
-          join<PACKED>(gA[i], gH[i], tA[i], tH[i]);
+      // the group's last tile is a link of the chain: everything up to its own end is
+      // joined before the state at its start is there, which then goes on in one operation
+      if (link) lds_barrier();
+      if (wv == W - 1) {
+        float gA = 1.f, gH = 0.f;
+        if (link) {
+          for (int k = 0; k < n; ++k) join<PACKED>(gA, gH, s.before[k][l]);
+          join<PACKED>(gA, gH, make_float2(tA, tH));
         }
+        h = __uint_as_float(far ? await(base(group), hb) : hb);
+        if (link) publish(base(group + 1), pass<PACKED>(h, make_float2(gA, gH)));
+        s.base[l] = h;
       }
-      if (far) await<VEC>(base(g0 / group), hb);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float h0 = __uint_as_float(hb[i]);
-        if (link) publish(base(g0 / group + 1) + i, pass<PACKED>(h0, gA[i], gH[i]));
-        s.base[l * VEC + i] = h0;
-      }
-    }
-    lds_barrier();
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      h[i] = s.base[l * VEC + i];
-      for (int k = 0; k * y.each < n; ++k) {
-        const float2 v = s.before[k][l * VEC + i];
-        h[i] = pass<PACKED>(h[i], v.x, v.y);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) h[i] = first[i];
-  }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    for (int k = 0; k < wv; ++k) {
-      const float2 v = s.wave[k][l * VEC + i];
-      h[i] = pass<PACKED>(h[i], v.x, v.y);
+      lds_barrier();
+      h = s.base[l];
+      for (int k = 0; k < n; ++k) h = pass<PACKED>(h, s.before[k][l]);
     }
   }
+  for (int k = 0; k < wv; ++k) h = pass<PACKED>(h, s.wave[k][l]);
+  return h;
 }
 
 // A workgroup's strip: every nstrip workgroups one of each, turned on by one
@@ -353,20 +278,20 @@ __device__ __forceinline__ int strip_of(const Sync& y) {
   return (r + q) % y.nstrip;
 }
 // The tile's place in its strip's scan.
-__device__ __forceinline__ int take(const Sync& y, int strip, int* s_step) {
+__device__ __forceinline__ int take(const Sync& y, int strip, Joint& s) {
   if (!y.ticket) return 0;
   if (threadIdx.x == 0)
-    *s_step = __hip_atomic_fetch_add(y.ticket + strip * LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s.step = __hip_atomic_fetch_add(y.ticket + strip * LINE, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(*s_step);
+  return __builtin_amdgcn_readfirstlane(s.step);
 }
 
-// Before either pass: the flags' patterns, the counter, where the boundaries of
-// packed sequences fall in each run of `len` tokens, and sequences without
-// tokens (out = in or 0: their final state is their initial one, their initial
-// state's gradient the final one's).
+// Before either pass: the flags' patterns, the counters, where the boundaries of
+// packed sequences fall in each run, and sequences without tokens (out = in or
+// 0: their final state is their initial one, their initial state's gradient the
+// final one's).
 __global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long long n16, int* ticket, int tickets,
-                                                int4* runs, int len, const float* in, float* out) {
+                                                int4* runs, const float* in, float* out) {
   const long long i0 = (long long)blockIdx.x * 256 + threadIdx.x, step = (long long)gridDim.x * 256;
   for (long long i = i0; i < tickets; i += step) ticket[i * LINE] = 0;
   for (long long i = i0; i < n16; i += step) fill[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
@@ -380,10 +305,10 @@ __global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long lon
     __syncthreads();
     cu = s_cu;
   }
-  const int nrun = (a.T + len - 1) / len;
+  const int nrun = (a.T + N - 1) / N;
   for (long long i = i0; i < nrun; i += step) {
-    const int t0 = (int)i * len;
-    runs[i] = pack(run_of(cu, a.S, t0, a.T - t0 < len ? a.T - t0 : len, a.T));
+    const int t0 = (int)i * N;
+    runs[i] = pack(run_of(cu, a.S, t0, a.T - t0 < N ? a.T - t0 : N, a.T));
   }
   if (!out) return;
   for (long long c = i0; c < (long long)a.S * a.D; c += step) {
@@ -393,60 +318,50 @@ __global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long lon
   }
 }
 
-template <typename E, int VEC>
-struct alignas(VEC * sizeof(E)) Raw { E v[VEC]; };
-
 }  // namespace
 
 // ---------------------------------------------------------------- forward
 
-// A wave has FSEG tokens of 64 VEC channels in registers: their gates, then
-// within the run h_t = H_t + P_t h_in from one pass, then y.
-template <typename E, int VEC, bool PACKED>
+// A wave has the gates of its run in registers, then within the run
+// h_t = H_t + P_t h_in from one pass, then y.
+template <typename E, bool PACKED>
 __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) {
-  constexpr int N = REC_FSEG;
-  __shared__ Joint<VEC> s_join;
-  __shared__ int s_step;
-  const int strip = strip_of(sy), chunk = take(sy, strip, &s_step), wv = wave_id();
-  const int b = strip / sy.strips;
-  const long long d = (long long)(strip % sy.strips) * 64 * VEC + lane_id() * VEC;
+  __shared__ Joint s_join;
+  const int strip = strip_of(sy), chunk = take(sy, strip, s_join), wv = wave_id(), b = strip / sy.strips;
+  const int d = strip % sy.strips * 64 + lane_id();
   const bool live = d < a.D;
-  const long long dl = live ? d : 0;                  // lanes behind D load channel 0, store nothing
+  const int dl = live ? d : 0;                        // lanes behind D work on channel 0 and store nothing
   const int t0 = (chunk * W + wv) * N, n = a.T - t0 < N ? a.T - t0 : N;     // n <= 0: no token
-  using R = Raw<E, VEC>;
   const E* xp = static_cast<const E*>(a.x) + b * a.x_b + dl;
   const E* fp = static_cast<const E*>(a.f) + b * a.f_b + dl;
   const E* wp = static_cast<const E*>(a.wz) + b * a.w_b + dl;
-  R x[N], f[N], w[N];
+  E x[N], f[N], w[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const long long t = t0 + j < a.T ? t0 + j : a.T - 1;
-    x[j] = *reinterpret_cast<const R*>(xp + t * a.x_t);
-    f[j] = *reinterpret_cast<const R*>(fp + t * a.f_t);
-    w[j] = *reinterpret_cast<const R*>(wp + t * a.w_t);
+    x[j] = xp[t * a.x_t];
+    f[j] = fp[t * a.f_t];
+    w[j] = wp[t * a.w_t];
   }
-  float bias2[VEC], nrate[VEC], first[VEC];
-  params<VEC>(a, dl, bias2, nrate);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) first[i] = a.h0 && !PACKED ? a.h0[(long long)b * a.D + dl + i] : 0.f;
+  float bias2, nrate;
+  params(a, dl, bias2, nrate);
+  const float first = a.h0 && !PACKED ? a.h0[(long long)b * a.D + dl] : 0.f;
   Run r{0u, 0u, 0u, 0, 0};
   if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
-  float P[N][VEC], H[N][VEC];
+  float P[N], H[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const Decay k = decay(to_f(f[j].v[i]), bias2[i], nrate[i]);
-      P[j][i] = k.a;
-      H[j][i] = __builtin_amdgcn_sqrtf(k.q) * sigmoid2(to_f(w[j].v[i])) * to_f(x[j].v[i]);
-    }
+    const Decay k = decay(to_f(f[j]), bias2, nrate);
+    P[j] = k.a;
+    H[j] = __builtin_amdgcn_sqrtf(k.q) * sigmoid2(to_f(w[j])) * to_f(x[j]);
   }
   if (n < N) {                                        // behind the row: the state passes
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (j >= n)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) { P[j][i] = 1.f; H[j][i] = 0.f; }
+      if (j >= n) {
+        P[j] = 1.f;
+        H[j] = 0.f;
+      }
   }
   // the first token that the state before the run does not reach
   int cut = N;
@@ -459,50 +374,32 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
       const bool st = r.start >> j & 1, us = r.used >> j & 1;
       if (st || !us) {
         if (st) cur = seq_from(a.cu, a.S, cur, t0 + j);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float h = a.h0 && st && us ? a.h0[(long long)cur * a.D + dl + i] : 0.f;
-          H[j][i] = us ? fmaf(P[j][i], h, H[j][i]) : 0.f;
-          P[j][i] = 0.f;
-        }
+        const float h = a.h0 && st && us ? a.h0[(long long)cur * a.D + dl] : 0.f;
+        H[j] = us ? fmaf(P[j], h, H[j]) : 0.f;
+        P[j] = 0.f;
       } else if (j > 0) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          H[j][i] = fmaf(P[j][i], H[j - 1][i], H[j][i]);
-          P[j][i] *= P[j - 1][i];
-        }
+        H[j] = fmaf(P[j], H[j - 1], H[j]);
+        P[j] *= P[j - 1];
       }
     }
   } else {
 #pragma unroll
-    for (int j = 1; j < N; ++j)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        H[j][i] = fmaf(P[j][i], H[j - 1][i], H[j][i]);
-        P[j][i] *= P[j - 1][i];
-      }
+    for (int j = 1; j < N; ++j) {
+      H[j] = fmaf(P[j], H[j - 1], H[j]);
+      P[j] *= P[j - 1];
+    }
   }
-  float h[VEC], A[VEC];
+  const float A = PACKED && cut < N ? __uint_as_float(RESET) : P[N - 1];
+  const float h = join_tiles<PACKED>(s_join, sy, chunk, strip, wv, A, H[N - 1], first);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) A[i] = PACKED && cut < N ? __uint_as_float(RESET) : P[N - 1][i];
-  join_tiles<PACKED, VEC>(s_join, sy, chunk, strip, wv, A, H[N - 1], first, h);
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (!PACKED || j < cut)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) H[j][i] = fmaf(P[j][i], h[i], H[j][i]);
-  }
+  for (int j = 0; j < N; ++j)
+    if (!PACKED || j < cut) H[j] = fmaf(P[j], h, H[j]);
   if (n <= 0 || !live) return;
-  if (a.hs) {                                         // the states entering runs of SEG tokens
-    const long long nrun = (a.T + SEG - 1) / SEG;
-#pragma unroll
-    for (int j = 0; j < N; j += SEG)
-      if (j < n) storev<float, VEC>(a.hs + (b * nrun + (t0 + j) / SEG) * a.D + d, j ? H[j ? j - 1 : 0] : h);
-  }
+  if (a.hs) a.hs[(b * ((a.T + N - 1LL) / N) + t0 / N) * a.D + d] = h;
   E* yp = static_cast<E*>(a.y) + ((long long)b * a.T + t0) * a.D + d;
 #pragma unroll
   for (int j = 0; j < N; ++j)
-    if (j < n) storev<E, VEC>(yp + (long long)j * a.D, H[j]);
+    if (j < n) yp[(long long)j * a.D] = from_f<E>(H[j]);
   if (!a.final_state) return;
   if (PACKED) {
     if (!r.end) return;
@@ -512,64 +409,51 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
       if (r.start >> j & 1) cur = seq_from(a.cu, a.S, cur, t0 + j);
       if (r.end >> j & 1) {
         if (cur < 0) cur = 0;
-        storev<float, VEC>(a.final_state + (long long)cur * a.D + d, H[j]);
+        a.final_state[(long long)cur * a.D + d] = H[j];
       }
     }
   } else if (t0 + N >= a.T) {
     // tokens behind the row pass the state on, so the last register has it
-    storev<float, VEC>(a.final_state + (long long)b * a.D + d, H[N - 1]);
+    a.final_state[(long long)b * a.D + d] = H[N - 1];
   }
 }
 
 // ---------------------------------------------------------------- backward
 
-// A wave has SEG tokens. One pass over them in order forms the gates again, the
-// states from hs, what lam_t multiplies in each gradient, and (A, C) with
-// c = A c_in + C for what flows out of the run backwards (c_t = a_t lam_t).
-// The parameter gradients' sums over tokens, sum lam_t k_t, need no second
-// array: with G_t = a_t G_(t-1) + k_t they are sum dy_t G_t + c_in G_last.
-template <typename E, int VEC, bool PACKED>
+// One pass over the run's tokens in order forms the gates again, the states from
+// hs, what lam_t multiplies in each gradient, and (A, C) with c = A c_in + C for
+// what flows out of the run backwards (c_t = a_t lam_t). The parameter gradients'
+// sums over tokens, sum lam_t k_t, need no second array: with
+// G_t = a_t G_(t-1) + k_t they are sum dy_t G_t + c_in G_last.
+template <typename E, bool PACKED>
 __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, float* parts) {
-  constexpr int N = SEG;
-  __shared__ Joint<VEC> s_join;
-  __shared__ int s_step;
-  const int strip = strip_of(sy), step = take(sy, strip, &s_step), wv = wave_id();
-  const int chunk = sy.nchunk - 1 - step, b = strip / sy.strips;
-  const long long d = (long long)(strip % sy.strips) * 64 * VEC + lane_id() * VEC;
+  __shared__ Joint s_join;
+  const int strip = strip_of(sy), step = take(sy, strip, s_join), wv = wave_id();
+  const int chunk = sy.nchunk - 1 - step, b = strip / sy.strips, d = strip % sy.strips * 64 + lane_id();
   const bool live = d < a.D;
-  const long long dl = live ? d : 0;
+  const int dl = live ? d : 0;
   const int t0 = (chunk * W + wv) * N, n = a.T - t0 < N ? a.T - t0 : N;
-  using R = Raw<E, VEC>;
   const E* xp = static_cast<const E*>(a.x) + b * a.x_b + dl;
   const E* fp = static_cast<const E*>(a.f) + b * a.f_b + dl;
   const E* wp = static_cast<const E*>(a.wz) + b * a.w_b + dl;
   const E* gp = static_cast<const E*>(a.dy) + b * a.dy_b + dl;
-  R x[N], f[N], w[N], g[N];
+  E x[N], f[N], w[N], g[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const long long t = t0 + j < a.T ? t0 + j : a.T - 1;
-    f[j] = *reinterpret_cast<const R*>(fp + t * a.f_t);
-    w[j] = *reinterpret_cast<const R*>(wp + t * a.w_t);
-    x[j] = *reinterpret_cast<const R*>(xp + t * a.x_t);
-    g[j] = *reinterpret_cast<const R*>(gp + t * a.dy_t);
+    f[j] = fp[t * a.f_t];
+    w[j] = wp[t * a.w_t];
+    x[j] = xp[t * a.x_t];
+    g[j] = gp[t * a.dy_t];
   }
-  const long long nrun = (a.T + SEG - 1) / SEG;
-  float bias2[VEC], nrate[VEC], last[VEC], h[VEC];
-  params<VEC>(a, dl, bias2, nrate);
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    last[i] = a.dfinal && !PACKED ? a.dfinal[(long long)b * a.D + dl + i] : 0.f;
-    h[i] = n > 0 ? a.hs[(b * nrun + t0 / SEG) * a.D + dl + i] : 0.f;
-  }
+  float bias2, nrate;
+  params(a, dl, bias2, nrate);
+  const float last = a.dfinal && !PACKED ? a.dfinal[(long long)b * a.D + dl] : 0.f;
+  float h = n > 0 ? a.hs[(b * ((a.T + N - 1LL) / N) + t0 / N) * a.D + dl] : 0.f;
   Run r{0u, 0u, 0u, 0, 0};
   if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
-  float aa[N][VEC], bs[N][VEC], kw[N][VEC], kf[N][VEC], dy[N][VEC];
-  float A[VEC], C[VEC], Gb[VEC], Ga[VEC], sb[VEC], sa[VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    A[i] = 1.f;
-    C[i] = Gb[i] = Ga[i] = sb[i] = sa[i] = 0.f;
-  }
+  float aa[N], bs[N], kw[N], kf[N], dy[N];
+  float A = 1.f, C = 0.f, Gb = 0.f, Ga = 0.f, sb = 0.f, sa = 0.f;
   int cur = r.cur;
   bool open = true;                        // no sequence has ended in the run yet
 #pragma unroll
@@ -577,111 +461,81 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
     const bool st = PACKED && (r.start >> j & 1), us = PACKED ? (r.used >> j & 1) : j < n;
     const bool en = PACKED && (r.end >> j & 1);
     if (!us) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        aa[j][i] = PACKED ? 0.f : 1.f;     // behind the row the gradient passes
-        bs[j][i] = kw[j][i] = kf[j][i] = dy[j][i] = 0.f;
-        if (PACKED) Gb[i] = Ga[i] = 0.f;
-      }
+      aa[j] = PACKED ? 0.f : 1.f;          // behind the row the gradient passes
+      bs[j] = kw[j] = kf[j] = dy[j] = 0.f;
+      if (PACKED) Gb = Ga = 0.f;
       continue;
     }
     if (PACKED && (st || en)) {
       if (st) cur = seq_from(a.cu, a.S, cur, t0 + j);
       if (cur < 0) cur = 0;
     }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float xv = to_f(x[j].v[i]);
-      const Decay k = decay(to_f(f[j].v[i]), bias2[i], nrate[i]);
-      float beta, inv;
-      root(k.q, beta, inv);
-      const float s = sigmoid2(to_f(w[j].v[i]));
-      const float one = __builtin_amdgcn_rcpf(1.f + k.e), sz = k.up ? one : k.e * one;
-      if (st) h[i] = a.h0 ? a.h0[(long long)cur * a.D + dl + i] : 0.f;
-      const float u = beta * s * xv, ah = k.a * h[i];
-      const float ki = ah - k.a * k.a * inv * (s * xv);       // dg = lam ki
-      aa[j][i] = k.a;
-      bs[j][i] = beta * s;
-      kw[j][i] = u * (1.f - s);
-      kf[j][i] = nrate[i] * sz * ki;
-      dy[j][i] = to_f(g[j].v[i]);
-      if (en && a.dfinal) dy[j][i] += a.dfinal[(long long)cur * a.D + dl + i];
-      h[i] = ah + u;
-      Gb[i] = st ? kf[j][i] : fmaf(k.a, Gb[i], kf[j][i]);
-      Ga[i] = st ? ki * k.g2 : fmaf(k.a, Ga[i], ki * k.g2);
-      sb[i] = fmaf(dy[j][i], Gb[i], sb[i]);
-      sa[i] = fmaf(dy[j][i], Ga[i], sa[i]);
-      if (open) {
-        A[i] *= k.a;
-        C[i] = fmaf(A[i], dy[j][i], C[i]);
-      }
+    const float xv = to_f(x[j]);
+    const Decay k = decay(to_f(f[j]), bias2, nrate);
+    float beta, inv;
+    root(k.q, beta, inv);
+    const float s = sigmoid2(to_f(w[j]));
+    const float one = __builtin_amdgcn_rcpf(1.f + k.e), sz = k.up ? one : k.e * one;
+    if (st) h = a.h0 ? a.h0[(long long)cur * a.D + dl] : 0.f;
+    const float u = beta * s * xv, ah = k.a * h;
+    const float ki = ah - k.a * k.a * inv * (s * xv);       // dg = lam ki
+    aa[j] = k.a;
+    bs[j] = beta * s;
+    kw[j] = u * (1.f - s);
+    kf[j] = nrate * sz * ki;
+    dy[j] = to_f(g[j]);
+    if (en && a.dfinal) dy[j] += a.dfinal[(long long)cur * a.D + dl];
+    h = ah + u;
+    Gb = st ? kf[j] : fmaf(k.a, Gb, kf[j]);
+    Ga = st ? ki * k.g2 : fmaf(k.a, Ga, ki * k.g2);
+    sb = fmaf(dy[j], Gb, sb);
+    sa = fmaf(dy[j], Ga, sa);
+    if (open) {
+      A *= k.a;
+      C = fmaf(A, dy[j], C);
     }
     if (en) open = false;
   }
-  if (PACKED && (!open || r.used != (1u << N) - 1)) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) A[i] = __uint_as_float(RESET);
-  }
-  float c[VEC];
-  join_tiles<PACKED, VEC>(s_join, sy, step, strip, W - 1 - wv, A, C, last, c);
+  if (PACKED && (!open || r.used != (1u << N) - 1)) A = __uint_as_float(RESET);
+  float c = join_tiles<PACKED>(s_join, sy, step, strip, W - 1 - wv, A, C, last);
   // what comes from behind a run whose last token is the last of its sequence
   // (or in none) is not for it
-  if (PACKED && (n < N || (r.end >> (N - 1) & 1) || !(r.used >> (N - 1) & 1))) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) c[i] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    sb[i] = fmaf(c[i], Gb[i], sb[i]);
-    sa[i] = fmaf(c[i], Ga[i], sa[i]);
-  }
+  if (PACKED && (n < N || (r.end >> (N - 1) & 1) || !(r.used >> (N - 1) & 1))) c = 0.f;
+  sb = fmaf(c, Gb, sb);
+  sa = fmaf(c, Ga, sa);
   const long long o = ((long long)b * a.T + t0) * a.D + d;
   cur = r.last;
 #pragma unroll
   for (int j = N - 1; j >= 0; --j) {
     const bool st = PACKED && (r.start >> j & 1), us = !PACKED || (r.used >> j & 1);
-    if (PACKED && (!us || (r.end >> j & 1))) {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) c[i] = 0.f;
-    }
-    float dx[VEC], df[VEC], dw[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const float lam = dy[j][i] + c[i];
-      dx[i] = lam * bs[j][i];
-      dw[i] = lam * kw[j][i];
-      df[i] = lam * kf[j][i];
-      c[i] = aa[j][i] * lam;
-    }
+    if (PACKED && (!us || (r.end >> j & 1))) c = 0.f;
+    const float lam = dy[j] + c;
+    c = aa[j] * lam;
     if (live && j < n) {
       const long long q = o + (long long)j * a.D;
-      storev<E, VEC>(static_cast<E*>(a.dx) + q, dx);
-      storev<E, VEC>(static_cast<E*>(a.df) + q, df);
-      storev<E, VEC>(static_cast<E*>(a.dwz) + q, dw);
+      static_cast<E*>(a.dx)[q] = from_f<E>(lam * bs[j]);
+      static_cast<E*>(a.df)[q] = from_f<E>(lam * kf[j]);
+      static_cast<E*>(a.dwz)[q] = from_f<E>(lam * kw[j]);
       if (PACKED && st && us && a.dh0) {
         cur = seq_before(a.cu, a.S, cur, t0 + j);
-        storev<float, VEC>(a.dh0 + (long long)cur * a.D + d, c);
+        a.dh0[(long long)cur * a.D + d] = c;
       }
     }
   }
-  if (!PACKED && t0 == 0 && a.dh0 && live) storev<float, VEC>(a.dh0 + (long long)b * a.D + d, c);
+  if (!PACKED && t0 == 0 && a.dh0 && live) a.dh0[(long long)b * a.D + d] = c;
   // the tile's sums, its waves' in order
   lds_barrier();
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) s_join.wave[wv][lane_id() * VEC + i] = make_float2(sb[i], sa[i]);
+  s_join.wave[wv][lane_id()] = make_float2(sb, sa);
   lds_barrier();
   if (wv == 0 && live) {
     const long long rows = (long long)a.B * sy.nchunk, row = (long long)b * sy.nchunk + chunk;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      sb[i] = sa[i] = 0.f;
-      for (int k = 0; k < W; ++k) {
-        sb[i] += s_join.wave[k][lane_id() * VEC + i].x;
-        sa[i] += s_join.wave[k][lane_id() * VEC + i].y;
-      }
+    sb = sa = 0.f;
+    for (int k = 0; k < W; ++k) {
+      sb += s_join.wave[k][lane_id()].x;
+      sa += s_join.wave[k][lane_id()].y;
     }
-    storev<float, VEC>(parts + row * a.D + d, sb);
-    storev<float, VEC>(parts + (rows + row) * a.D + d, sa);
+    parts[row * a.D + d] = sb;
+    parts[(rows + row) * a.D + d] = sa;
   }
 }
 
@@ -739,45 +593,25 @@ __global__ __launch_bounds__(256) void rec_sum_heads(RecArgs a, const float* par
 
 // ---------------------------------------------------------------- one token
 
-// y = h' = a h + beta s x for B rows of D channels, VEC channels a thread.
-template <typename E, int VEC>
+// y = h' = a h + beta s x for B rows of D channels, a channel a thread.
+template <typename E>
 __global__ __launch_bounds__(256) void rec_step_kernel(RecArgs a) {
-  const int per = a.D / VEC;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (long long)a.B * per) return;
-  const long long b = i / per, d = (i - b * per) * VEC;
-  float x[VEC], f[VEC], w[VEC], h[VEC], bias2[VEC], nrate[VEC];
-  loadv<E, VEC>(static_cast<const E*>(a.x) + b * a.x_b + d, x);
-  loadv<E, VEC>(static_cast<const E*>(a.f) + b * a.f_b + d, f);
-  loadv<E, VEC>(static_cast<const E*>(a.wz) + b * a.w_b + d, w);
-  loadv<float, VEC>(a.h0 + b * a.D + d, h);
-  params<VEC>(a, d, bias2, nrate);
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    const Decay k = decay(f[v], bias2[v], nrate[v]);
-    float beta, inv;
-    root(k.q, beta, inv);
-    h[v] = k.a * h[v] + beta * sigmoid2(w[v]) * x[v];
-  }
-  storev<float, VEC>(a.final_state + b * a.D + d, h);
-  storev<E, VEC>(static_cast<E*>(a.y) + b * a.D + d, h);
+  if (i >= (long long)a.B * a.D) return;
+  const unsigned b = (unsigned)i / (unsigned)a.D, d = (unsigned)i - b * a.D;      // B D < 2^31
+  const float x = to_f(static_cast<const E*>(a.x)[b * a.x_b + d]), f = to_f(static_cast<const E*>(a.f)[b * a.f_b + d]);
+  const float w = to_f(static_cast<const E*>(a.wz)[b * a.w_b + d]);
+  float bias2, nrate;
+  params(a, d, bias2, nrate);
+  const Decay k = decay(f, bias2, nrate);
+  const float h = fmaf(k.a, a.h0[i], __builtin_amdgcn_sqrtf(k.q) * sigmoid2(w) * x);
+  a.final_state[i] = h;
+  static_cast<E*>(a.y)[i] = from_f<E>(h);
 }
 
 // ---------------------------------------------------------------- launches
 
 namespace {
-
-// channels a thread can take at once: 4 bytes of the inputs' type, where every
-// row of every tensor starts on a multiple of that
-int vec_of(const RecArgs& a, size_t esz, std::initializer_list<const void*> ts,
-           std::initializer_list<int64_t> strides) {
-  if (esz == 4 || a.D % 2) return 1;
-  for (int64_t s : strides)
-    if (s % 2) return 1;
-  for (const void* t : ts)
-    if (reinterpret_cast<uintptr_t>(t) % 4) return 1;
-  return 2;
-}
 
 long long up(long long n, long long m) { return (n + m - 1) / m * m; }
 
@@ -787,30 +621,24 @@ struct Space {
   long long agg, base, runs, parts, sums, all, nchunk;
 };
 Space space(long long B, long long T, long long D, bool backward) {
-  const long long len = backward ? SEG : REC_FSEG, wide = B * up(D, 128);
+  const long long wide = B * up(D, 64);
   Space s;
-  s.nchunk = (T + W * len - 1) / (W * len);
+  s.nchunk = (T + W * N - 1) / (W * N);
   const bool many = s.nchunk > 1;
-  s.agg = many ? B * ((D + 63) / 64) * LINE : 16;
+  s.agg = many ? wide / 64 * LINE : 16;
   s.base = s.agg + (many ? 2 * s.nchunk * wide : 0);
   s.runs = s.base + (many ? (s.nchunk / W + 1) * wide : 0);
-  s.parts = s.runs + (B == 1 ? 4 * ((T + len - 1) / len) : 0);
+  s.parts = s.runs + (B == 1 ? 4 * ((T + N - 1) / N) : 0);
   s.sums = s.parts + (backward ? 2 * B * s.nchunk * D : 0);
   s.all = s.sums + (backward ? 2 * REC_SLICES * D : 0);
   return s;
 }
 
-template <int VEC>
-Sync prepare(const RecArgs& a, const Space& s, int len, const float* in, float* out, hipStream_t st) {
+Sync prepare(const RecArgs& a, const Space& s, const float* in, float* out, hipStream_t st) {
   Sync y{};
   y.nchunk = (int)s.nchunk;
-  y.strips = (a.D + 64 * VEC - 1) / (64 * VEC);
+  y.strips = (a.D + 63) / 64;
   y.nstrip = y.strips * a.B;
-  // The larger group's fewer links pay where few strips go on at once and the
-  // chain sets the time, its looking at more tiles costs where it does not:
-  // 8 strips (16384 x 1024 packed, forward and backward) 149 us against 154,
-  // 64 strips (4 x 8192 x 2048) 383 against 371, 16 (65536 x 2048) 244 against 237
-  y.each = y.nstrip <= 8 ? 2 : 1;
   long long n16 = 0;
   if (s.nchunk > 1) {
     y.ticket = reinterpret_cast<int*>(a.ws);
@@ -822,32 +650,32 @@ Sync prepare(const RecArgs& a, const Space& s, int len, const float* in, float* 
   y.runs = runs;
   if (n16 || a.cu) {
     long long n = std::max<long long>(n16, y.nstrip);
-    if (a.cu) n = std::max(n, std::max((long long)(a.T + len - 1) / len, out ? (long long)a.S * a.D : 0));
+    if (a.cu) n = std::max(n, std::max((long long)(a.T + N - 1) / N, out ? (long long)a.S * a.D : 0));
     const unsigned grid = (unsigned)std::min<long long>((n + 255) / 256, 1024);
     hipLaunchKernelGGL(rec_init, dim3(grid), dim3(256), 0, st, a, reinterpret_cast<uint4*>(a.ws + s.agg),
-                       n16, y.ticket, y.ticket ? y.nstrip : 0, runs, len, in, out);
+                       n16, y.ticket, y.ticket ? y.nstrip : 0, runs, in, out);
   }
   return y;
 }
 
-template <typename E, int VEC>
+template <typename E>
 hipError_t fwd(const RecArgs& a, hipStream_t st) {
   const Space s = space(a.B, a.T, a.D, false);
-  const Sync y = prepare<VEC>(a, s, REC_FSEG, a.h0, a.final_state, st);
+  const Sync y = prepare(a, s, a.h0, a.final_state, st);
   const dim3 grid((unsigned)(s.nchunk * y.nstrip));
-  if (a.cu) hipLaunchKernelGGL((rec_fwd_kernel<E, VEC, true>), grid, dim3(64 * W), 0, st, a, y);
-  else hipLaunchKernelGGL((rec_fwd_kernel<E, VEC, false>), grid, dim3(64 * W), 0, st, a, y);
+  if (a.cu) hipLaunchKernelGGL((rec_fwd_kernel<E, true>), grid, dim3(64 * W), 0, st, a, y);
+  else hipLaunchKernelGGL((rec_fwd_kernel<E, false>), grid, dim3(64 * W), 0, st, a, y);
   return hipGetLastError();
 }
 
-template <typename E, int VEC>
+template <typename E>
 hipError_t bwd(const RecArgs& a, hipStream_t st) {
   const Space s = space(a.B, a.T, a.D, true);
-  const Sync y = prepare<VEC>(a, s, SEG, a.dfinal, a.dh0, st);
+  const Sync y = prepare(a, s, a.dfinal, a.dh0, st);
   const dim3 grid((unsigned)(s.nchunk * y.nstrip));
   float* parts = a.ws + s.parts;
-  if (a.cu) hipLaunchKernelGGL((rec_bwd_kernel<E, VEC, true>), grid, dim3(64 * W), 0, st, a, y, parts);
-  else hipLaunchKernelGGL((rec_bwd_kernel<E, VEC, false>), grid, dim3(64 * W), 0, st, a, y, parts);
+  if (a.cu) hipLaunchKernelGGL((rec_bwd_kernel<E, true>), grid, dim3(64 * W), 0, st, a, y, parts);
+  else hipLaunchKernelGGL((rec_bwd_kernel<E, false>), grid, dim3(64 * W), 0, st, a, y, parts);
   // many tiles: first slices of them, over the whole card
   const long long rows = s.nchunk * a.B;
   if (rows > REC_SLICES) {
@@ -866,26 +694,17 @@ hipError_t bwd(const RecArgs& a, hipStream_t st) {
 int64_t rec_ws(int64_t B, int64_t T, int64_t D, bool backward) { return space(B, T, D, backward).all; }
 
 hipError_t rec_fwd(const RecArgs& a, int dtype, hipStream_t st) {
-  if (dtype == NGDN_F32) return fwd<float, 1>(a, st);
-  const int v = vec_of(a, 2, {a.x, a.f, a.wz, a.y}, {a.x_b, a.x_t, a.f_b, a.f_t, a.w_b, a.w_t});
-  return v == 2 ? fwd<bf16, 2>(a, st) : fwd<bf16, 1>(a, st);
+  return dtype == NGDN_F32 ? fwd<float>(a, st) : fwd<bf16>(a, st);
 }
 
 hipError_t rec_bwd(const RecArgs& a, int dtype, hipStream_t st) {
-  if (dtype == NGDN_F32) return bwd<float, 1>(a, st);
-  const int v = vec_of(a, 2, {a.x, a.f, a.wz, a.dy, a.dx, a.df, a.dwz},
-                       {a.x_b, a.x_t, a.f_b, a.f_t, a.w_b, a.w_t, a.dy_b, a.dy_t});
-  return v == 2 ? bwd<bf16, 2>(a, st) : bwd<bf16, 1>(a, st);
+  return dtype == NGDN_F32 ? bwd<float>(a, st) : bwd<bf16>(a, st);
 }
 
 hipError_t rec_step(const RecArgs& a, int dtype, hipStream_t st) {
-  int v = 1;
-  if (dtype == NGDN_BF16) v = vec_of(a, 2, {a.x, a.f, a.wz, a.y}, {a.x_b, a.f_b, a.w_b});
-  if ((reinterpret_cast<uintptr_t>(a.h0) | reinterpret_cast<uintptr_t>(a.final_state)) % 8) v = 1;
-  const dim3 grid((unsigned)(((long long)a.B * (a.D / v) + 255) / 256));
-  if (dtype == NGDN_F32) hipLaunchKernelGGL((rec_step_kernel<float, 1>), grid, dim3(256), 0, st, a);
-  else if (v == 2) hipLaunchKernelGGL((rec_step_kernel<bf16, 2>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((rec_step_kernel<bf16, 1>), grid, dim3(256), 0, st, a);
+  const dim3 grid((unsigned)(((long long)a.B * a.D + 255) / 256));
+  if (dtype == NGDN_F32) hipLaunchKernelGGL((rec_step_kernel<float>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((rec_step_kernel<bf16>), grid, dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
