@@ -218,6 +218,43 @@ struct Joint {
   int step;
 };
 
+// A lane's element of a row: the row's address is the wave's and the lane's part
+// 32 bits, so that the next token costs scalar additions and no vector instruction
+// (a vector 64-bit address for each load: 4 x 8192 x 2048, both passes, 358 us
+// against 330, 65536 x 2048 forward 243 against 228).
+template <typename E>
+using Device = __attribute__((address_space(1))) E;
+template <typename E>
+__device__ __forceinline__ E load_at(const E* row, unsigned bytes) {
+  return *(const Device<E>*)((const Device<char>*)row + bytes);
+}
+template <typename E>
+__device__ __forceinline__ void store_at(E* row, unsigned bytes, float x) {
+  *(Device<E>*)((Device<char>*)row + bytes) = from_f<E>(x);
+}
+// The compiler takes that form only where it sees the 32 bits widened in the same block.
+__device__ __forceinline__ unsigned here(unsigned bytes) {
+  asm volatile("" : "+v"(bytes));
+  return bytes;
+}
+// The run's n tokens of K tensors, token by token; p: their first tokens' rows, row:
+// elements from one to the next. Behind the n the last again. (The barrier keeps
+// the sum in scalar registers, where it would be rearranged into vector ones.)
+template <int K, typename E>
+__device__ __forceinline__ void load_run(E (&v)[K][N], const E* (&p)[K], const long long (&row)[K], int n,
+                                         unsigned bytes) {
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k][j] = load_at(p[k], bytes);
+      if (j + 1 < N) {
+        p[k] += j + 1 < n ? row[k] : 0;
+        asm volatile("" : "+s"(p[k]));
+      }
+    }
+}
+
 // From wave (A, H) to the state entering the wave. step: the tile's place in the
 // scan's order (0 first), wv the wave's. first: the state entering tile 0.
 template <bool PACKED>
@@ -330,19 +367,15 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
   const int strip = strip_of(sy), chunk = take(sy, strip, s_join), wv = wave_id(), b = strip / sy.strips;
   const int d = strip % sy.strips * 64 + lane_id();
   const bool live = d < a.D;
-  const int dl = live ? d : 0;                        // lanes behind D work on channel 0 and store nothing
+  const unsigned dl = live ? d : 0, lane = dl * (unsigned)sizeof(E);                        // lanes behind D work on channel 0 and store nothing
   const int t0 = (chunk * W + wv) * N, n = a.T - t0 < N ? a.T - t0 : N;     // n <= 0: no token
-  const E* xp = static_cast<const E*>(a.x) + b * a.x_b + dl;
-  const E* fp = static_cast<const E*>(a.f) + b * a.f_b + dl;
-  const E* wp = static_cast<const E*>(a.wz) + b * a.w_b + dl;
-  E x[N], f[N], w[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const long long t = t0 + j < a.T ? t0 + j : a.T - 1;
-    x[j] = xp[t * a.x_t];
-    f[j] = fp[t * a.f_t];
-    w[j] = wp[t * a.w_t];
-  }
+  const long long ts = n > 0 ? t0 : a.T - 1;
+  E v[3][N];                                          // f, wz, x
+  const long long row[3] = {a.f_t, a.w_t, a.x_t};
+  const E* p[3] = {static_cast<const E*>(a.f) + b * a.f_b + ts * a.f_t,
+                   static_cast<const E*>(a.wz) + b * a.w_b + ts * a.w_t,
+                   static_cast<const E*>(a.x) + b * a.x_b + ts * a.x_t};
+  load_run(v, p, row, n, lane);
   float bias2, nrate;
   params(a, dl, bias2, nrate);
   const float first = a.h0 && !PACKED ? a.h0[(long long)b * a.D + dl] : 0.f;
@@ -351,9 +384,9 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
   float P[N], H[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const Decay k = decay(to_f(f[j]), bias2, nrate);
+    const Decay k = decay(to_f(v[0][j]), bias2, nrate);
     P[j] = k.a;
-    H[j] = __builtin_amdgcn_sqrtf(k.q) * sigmoid2(to_f(w[j])) * to_f(x[j]);
+    H[j] = __builtin_amdgcn_sqrtf(k.q) * sigmoid2(to_f(v[1][j])) * to_f(v[2][j]);
   }
   if (n < N) {                                        // behind the row: the state passes
 #pragma unroll
@@ -396,10 +429,16 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
     if (!PACKED || j < cut) H[j] = fmaf(P[j], h, H[j]);
   if (n <= 0 || !live) return;
   if (a.hs) a.hs[(b * ((a.T + N - 1LL) / N) + t0 / N) * a.D + d] = h;
-  E* yp = static_cast<E*>(a.y) + ((long long)b * a.T + t0) * a.D + d;
+  E* yp = static_cast<E*>(a.y) + ((long long)b * a.T + t0) * a.D;
+  if (n >= N) {
+    const unsigned o = here(lane);
 #pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (j < n) yp[(long long)j * a.D] = from_f<E>(H[j]);
+    for (int j = 0; j < N; ++j, yp += a.D) store_at(yp, o, H[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j, yp += a.D)
+      if (j < n) store_at(yp, lane, H[j]);
+  }
   if (!a.final_state) return;
   if (PACKED) {
     if (!r.end) return;
@@ -431,21 +470,16 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
   const int strip = strip_of(sy), step = take(sy, strip, s_join), wv = wave_id();
   const int chunk = sy.nchunk - 1 - step, b = strip / sy.strips, d = strip % sy.strips * 64 + lane_id();
   const bool live = d < a.D;
-  const int dl = live ? d : 0;
+  const unsigned dl = live ? d : 0, lane = dl * (unsigned)sizeof(E);
   const int t0 = (chunk * W + wv) * N, n = a.T - t0 < N ? a.T - t0 : N;
-  const E* xp = static_cast<const E*>(a.x) + b * a.x_b + dl;
-  const E* fp = static_cast<const E*>(a.f) + b * a.f_b + dl;
-  const E* wp = static_cast<const E*>(a.wz) + b * a.w_b + dl;
-  const E* gp = static_cast<const E*>(a.dy) + b * a.dy_b + dl;
-  E x[N], f[N], w[N], g[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const long long t = t0 + j < a.T ? t0 + j : a.T - 1;
-    f[j] = fp[t * a.f_t];
-    w[j] = wp[t * a.w_t];
-    x[j] = xp[t * a.x_t];
-    g[j] = gp[t * a.dy_t];
-  }
+  const long long ts = n > 0 ? t0 : a.T - 1;
+  E v[4][N];                                          // f, wz, x, dy
+  const long long row[4] = {a.f_t, a.w_t, a.x_t, a.dy_t};
+  const E* p[4] = {static_cast<const E*>(a.f) + b * a.f_b + ts * a.f_t,
+                   static_cast<const E*>(a.wz) + b * a.w_b + ts * a.w_t,
+                   static_cast<const E*>(a.x) + b * a.x_b + ts * a.x_t,
+                   static_cast<const E*>(a.dy) + b * a.dy_b + ts * a.dy_t};
+  load_run(v, p, row, n, lane);
   float bias2, nrate;
   params(a, dl, bias2, nrate);
   const float last = a.dfinal && !PACKED ? a.dfinal[(long long)b * a.D + dl] : 0.f;
@@ -470,11 +504,11 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
       if (st) cur = seq_from(a.cu, a.S, cur, t0 + j);
       if (cur < 0) cur = 0;
     }
-    const float xv = to_f(x[j]);
-    const Decay k = decay(to_f(f[j]), bias2, nrate);
+    const float xv = to_f(v[2][j]);
+    const Decay k = decay(to_f(v[0][j]), bias2, nrate);
     float beta, inv;
     root(k.q, beta, inv);
-    const float s = sigmoid2(to_f(w[j]));
+    const float s = sigmoid2(to_f(v[1][j]));
     const float one = __builtin_amdgcn_rcpf(1.f + k.e), sz = k.up ? one : k.e * one;
     if (st) h = a.h0 ? a.h0[(long long)cur * a.D + dl] : 0.f;
     const float u = beta * s * xv, ah = k.a * h;
@@ -483,7 +517,7 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
     bs[j] = beta * s;
     kw[j] = u * (1.f - s);
     kf[j] = nrate * sz * ki;
-    dy[j] = to_f(g[j]);
+    dy[j] = to_f(v[3][j]);
     if (en && a.dfinal) dy[j] += a.dfinal[(long long)cur * a.D + dl];
     h = ah + u;
     Gb = st ? kf[j] : fmaf(k.a, Gb, kf[j]);
@@ -496,33 +530,50 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
     }
     if (en) open = false;
   }
-  if (PACKED && (!open || r.used != (1u << N) - 1)) A = __uint_as_float(RESET);
+  constexpr unsigned ALL = (1u << N) - 1;
+  if (PACKED && (!open || r.used != ALL)) A = __uint_as_float(RESET);
   float c = join_tiles<PACKED>(s_join, sy, step, strip, W - 1 - wv, A, C, last);
   // what comes from behind a run whose last token is the last of its sequence
   // (or in none) is not for it
   if (PACKED && (n < N || (r.end >> (N - 1) & 1) || !(r.used >> (N - 1) & 1))) c = 0.f;
   sb = fmaf(c, Gb, sb);
   sa = fmaf(c, Ga, sa);
-  const long long o = ((long long)b * a.T + t0) * a.D + d;
-  cur = r.last;
+  if (live) {
+    const long long o = ((long long)b * a.T + t0) * a.D;
+    if (PACKED ? !(r.start | r.end) && r.used == ALL : n >= N) {
+      E *dx = static_cast<E*>(a.dx) + o + (N - 1LL) * a.D, *df = static_cast<E*>(a.df) + o + (N - 1LL) * a.D;
+      E* dw = static_cast<E*>(a.dwz) + o + (N - 1LL) * a.D;
+      const unsigned l = here(lane);
 #pragma unroll
-  for (int j = N - 1; j >= 0; --j) {
-    const bool st = PACKED && (r.start >> j & 1), us = !PACKED || (r.used >> j & 1);
-    if (PACKED && (!us || (r.end >> j & 1))) c = 0.f;
-    const float lam = dy[j] + c;
-    c = aa[j] * lam;
-    if (live && j < n) {
-      const long long q = o + (long long)j * a.D;
-      static_cast<E*>(a.dx)[q] = from_f<E>(lam * bs[j]);
-      static_cast<E*>(a.df)[q] = from_f<E>(lam * kf[j]);
-      static_cast<E*>(a.dwz)[q] = from_f<E>(lam * kw[j]);
-      if (PACKED && st && us && a.dh0) {
-        cur = seq_before(a.cu, a.S, cur, t0 + j);
-        a.dh0[(long long)cur * a.D + d] = c;
+      for (int j = N - 1; j >= 0; --j, dx -= a.D, df -= a.D, dw -= a.D) {
+        const float lam = dy[j] + c;
+        c = aa[j] * lam;
+        store_at(dx, l, lam * bs[j]);
+        store_at(df, l, lam * kf[j]);
+        store_at(dw, l, lam * kw[j]);
+      }
+    } else {
+      cur = r.last;
+#pragma unroll
+      for (int j = N - 1; j >= 0; --j) {
+        const bool st = PACKED && (r.start >> j & 1), us = !PACKED || (r.used >> j & 1);
+        if (PACKED && (!us || (r.end >> j & 1))) c = 0.f;
+        const float lam = dy[j] + c;
+        c = aa[j] * lam;
+        if (j < n) {
+          const long long q = o + (long long)j * a.D + d;
+          static_cast<E*>(a.dx)[q] = from_f<E>(lam * bs[j]);
+          static_cast<E*>(a.df)[q] = from_f<E>(lam * kf[j]);
+          static_cast<E*>(a.dwz)[q] = from_f<E>(lam * kw[j]);
+          if (PACKED && st && us && a.dh0) {
+            cur = seq_before(a.cu, a.S, cur, t0 + j);
+            a.dh0[(long long)cur * a.D + d] = c;
+          }
+        }
       }
     }
+    if (!PACKED && t0 == 0 && a.dh0) a.dh0[(long long)b * a.D + d] = c;
   }
-  if (!PACKED && t0 == 0 && a.dh0 && live) a.dh0[(long long)b * a.D + d] = c;
   // the tile's sums, its waves' in order
   lds_barrier();
   s_join.wave[wv][lane_id()] = make_float2(sb, sa);
