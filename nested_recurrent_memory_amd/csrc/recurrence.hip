@@ -93,15 +93,18 @@ __device__ Run run_of(const int* cu, int S, int t0, int n, int T) {
   }
   int s = lo;
   r.cur = s - 1;
-  for (int j = 0; j < n; ++j) {
-    while (s <= S && cu[s] <= t0 + j) {
-      if (cu[s] == t0 + j) r.start |= 1u << j;
-      ++s;
+  // from boundary to boundary (a boundary that lies lower than one before it counts
+  // as there)
+  for (int at = t0;;) {
+    const int next = s <= S ? (cu[s] > at ? cu[s] : at) : 0x7fffffff, to = next < t0 + n ? next : t0 + n;
+    if (s >= 1 && s <= S && to > at) {
+      r.used |= (1u << (to - t0)) - (1u << (at - t0));
+      if (next == to || to == T) r.end |= 1u << (to - 1 - t0);
     }
-    if (s >= 1 && s <= S) {
-      r.used |= 1u << j;
-      if (cu[s] == t0 + j + 1 || t0 + j + 1 == T) r.end |= 1u << j;
-    }
+    if (next >= t0 + n) break;
+    r.start |= 1u << (next - t0);
+    at = next;
+    ++s;
   }
   r.last = s - 1;
   return r;
@@ -329,30 +332,30 @@ __device__ __forceinline__ int take(const Sync& y, int strip, Joint& s) {
 // final one's).
 __global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long long n16, int* ticket, int tickets,
                                                 int4* runs, const float* in, float* out) {
-  const long long i0 = (long long)blockIdx.x * 256 + threadIdx.x, step = (long long)gridDim.x * 256;
-  for (long long i = i0; i < tickets; i += step) ticket[i * LINE] = 0;
+  const unsigned i0 = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
+  if (a.cu) {
+    // the search and the walk are chains of reads: from LDS where the boundaries fit
+    constexpr int FIT = 4096;
+    __shared__ int s_cu[FIT];
+    const int* cu = a.cu;
+    if (a.S < FIT) {
+      for (int i = threadIdx.x; i <= a.S; i += 256) s_cu[i] = a.cu[i];
+      __syncthreads();
+      cu = s_cu;
+    }
+    const unsigned nrun = (a.T + N - 1u) / N, n = out ? (unsigned)a.S * a.D : 0u;     // S D < 2^31
+    for (unsigned i = i0; i < nrun; i += step) {
+      const int t0 = (int)i * N;
+      runs[i] = pack(run_of(cu, a.S, t0, a.T - t0 < N ? a.T - t0 : N, a.T));
+    }
+    for (unsigned c = i0; c < n; c += step) {
+      const unsigned s = c / (unsigned)a.D;
+      const int lo = cu[s] < a.T ? cu[s] : a.T, hi = cu[s + 1] < a.T ? cu[s + 1] : a.T;
+      if (lo >= hi) out[c] = in ? in[c] : 0.f;
+    }
+  }
+  for (unsigned i = i0; i < (unsigned)tickets; i += step) ticket[(long long)i * LINE] = 0;
   for (long long i = i0; i < n16; i += step) fill[i] = make_uint4(~0u, ~0u, ~0u, ~0u);
-  if (!a.cu) return;
-  // the search and the walk are chains of reads: from LDS where the boundaries fit
-  constexpr int FIT = 4096;
-  __shared__ int s_cu[FIT];
-  const int* cu = a.cu;
-  if (a.S < FIT) {
-    for (int i = threadIdx.x; i <= a.S; i += 256) s_cu[i] = a.cu[i];
-    __syncthreads();
-    cu = s_cu;
-  }
-  const int nrun = (a.T + N - 1) / N;
-  for (long long i = i0; i < nrun; i += step) {
-    const int t0 = (int)i * N;
-    runs[i] = pack(run_of(cu, a.S, t0, a.T - t0 < N ? a.T - t0 : N, a.T));
-  }
-  if (!out) return;
-  for (long long c = i0; c < (long long)a.S * a.D; c += step) {
-    const long long s = c / a.D;
-    const int lo = cu[s] < a.T ? cu[s] : a.T, hi = cu[s + 1] < a.T ? cu[s + 1] : a.T;
-    if (lo >= hi) out[c] = in ? in[c] : 0.f;
-  }
 }
 
 }  // namespace
