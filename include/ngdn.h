@@ -626,7 +626,7 @@ int64_t ngdn_embedding_ws(int64_t N, int64_t V, int32_t D);
  * reads (NULL: not written). The backward takes the forward's inputs, hs,
  * dy (strides dy_b, dy_t) and dfinal, and writes dx, df, dwz [B,T,D] in dtype
  * and, fp32, ddt_bias [D], dA_log [H] and dh0. ws: ngdn_recurrence_ws(...)
- * fp32, no initial contents. Sums over tokens are in a fixed order: the same
+ * fp32, 16-byte aligned, no initial contents. Sums over tokens are in a fixed order: the same
  * inputs give the same bits. */
 #define NGDN_REC_RUN 16
 typedef struct ngdn_recurrence_args {

@@ -1100,7 +1100,8 @@ namespace {
 int32_t embed_sizes(int32_t d0, int32_t d1, int64_t N, int64_t V, int32_t D, const char* what) {
   for (int32_t d : {d0, d1})
     if (d != NGDN_F32 && d != NGDN_BF16) return fail(NGDN_EINVAL, "%s: dtype %d", what, d);
-  // positions and ids are kept in 32 bits; grids have a workgroup for at most 4 rows
+  // positions and ids are kept in 32 bits; the largest grid, a wave for 16 rows of
+  // 64 columns, has under 2^32 work-items
   if (N < 0 || V < 1 || D < 1 || N > (1LL << 24) || V > (1LL << 24) - 1 || D > (1 << 20))
     return fail(NGDN_EINVAL, "%s: N=%lld V=%lld D=%d (0 <= N <= 2^24, 1 <= V < 2^24, 1 <= D <= 2^20)",
                 what, (long long)N, (long long)V, D);
@@ -1127,6 +1128,7 @@ int32_t rec_rows(const ngdn_recurrence_args* r, const char* what) {
                 r->S, r->B);
   if ((long long)r->S * r->D > (1LL << 31) - 1)
     return fail(NGDN_EINVAL, "%s: S*D = %lld exceeds 2^31 - 1", what, (long long)r->S * r->D);
+  if (reinterpret_cast<uintptr_t>(r->ws) & 15) return fail(NGDN_EINVAL, "%s: ws must be 16-byte aligned", what);
   // the largest grid: 512 work-items for 128 tokens of 64 channels (and so a row of
   // D is under 2^31 bytes)
   const long long tiles = (r->D + 63LL) / 64 * ((r->T + 127LL) / 128) * r->B;

@@ -62,6 +62,7 @@ def _compute_dtype(x):
 _EMBED = (torch.bfloat16, torch.float32)                     # the kernels' types
 _TABLES = (torch.bfloat16, torch.float16, torch.float32)     # fp16 runs in fp32
 _EMBED_MOST = 1 << 24                                        # ids, and rows of the table
+_EMBED_WIDTH, _EMBED_VALUES = 1 << 20, 1 << 35               # and its columns, ids times columns
 
 
 def _embed(t):
@@ -146,6 +147,8 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     ydt = weight.dtype if out_dtype is None else out_dtype
     if ydt not in _TABLES:
         raise ValueError(f"embedding: out_dtype {ydt} (bf16, fp16 or fp32)")
+    if max(weight.shape) > (1 << 31) - 1:
+        raise ValueError(f"embedding: weight {tuple(weight.shape)} (sizes up to 2^31 - 1)")
     _on_gpu("embedding", weight, ids)
     if ids.dtype != torch.int64:
         ids = ids.to(torch.int64)
@@ -158,16 +161,19 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
 
 class Embedding(nn.Embedding):
     """nn.Embedding whose lookup on the GPU and its gradient are kernels of the
-    library. With max_norm, scale_grad_by_freq or sparse, off the GPU, for
-    tensor subclasses and under functorch, forward-mode differentiation or
-    tracing it is nn.Embedding's own."""
+    library. With max_norm, scale_grad_by_freq or sparse, off the GPU, in other
+    types than bfloat16 and float32, beyond the kernels' sizes, for tensor
+    subclasses and under functorch, forward-mode differentiation or tracing it
+    is nn.Embedding's own (which on the GPU ends the process on an id outside
+    the table, where ``embedding`` gives NaN)."""
 
     def forward(self, ids):
         w = self.weight
-        plain = (w.is_cuda and ids.device == w.device and w.dim() == 2 and w.dtype in _TABLES
-                 and ids.dtype in (torch.int32, torch.int64) and type(ids) is torch.Tensor
-                 and type(w) in (torch.Tensor, nn.Parameter)
-                 and w.shape[0] < _EMBED_MOST and ids.numel() <= _EMBED_MOST
+        plain = (type(ids) is torch.Tensor and type(w) in (torch.Tensor, nn.Parameter)
+                 and w.is_cuda and ids.device == w.device and w.dim() == 2 and w.numel() > 0
+                 and w.dtype in _EMBED and ids.dtype in (torch.int32, torch.int64)
+                 and w.shape[0] < _EMBED_MOST and w.shape[1] <= _EMBED_WIDTH
+                 and ids.numel() <= min(_EMBED_MOST, _EMBED_VALUES // w.shape[1])
                  and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse)
         if (not plain or torch.compiler.is_compiling() or torch.jit.is_tracing()
                 or forward_ad._current_level >= 0

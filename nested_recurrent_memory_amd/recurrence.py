@@ -14,8 +14,8 @@ prologue (``NestedGDN2Attention.A_log``, ``dt_bias``):
   or packed sequences, a state in and out.
 * ``step_gated_recurrence``: one token, for decoding. Forward only.
 
-Inputs in bfloat16 or float32 run on the kernels as they are, float16 in
-float32; states and the decay parameters are float32 in the kernels. There is
+Inputs all in bfloat16 or all in float32 run on the kernels as they are, float16
+and mixed types in float32; states and the decay parameters are float32 in the kernels. There is
 no fallback: without the library (or on tensors off the GPU) the calls raise.
 """
 
@@ -24,6 +24,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -60,8 +61,14 @@ def _f32(t):
     return t if t.is_contiguous() else t.contiguous()
 
 
-_WORK = (torch.bfloat16, torch.float32)                     # the kernels' types
-_TYPES = (torch.bfloat16, torch.float16, torch.float32)     # fp16 runs in fp32
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_MOST = (1 << 31) - 1           # of any size, which the library takes in 32 bits
+
+
+def _work_type(x, f, wz):
+    """The kernels' type: a narrower one than a tensor's own would lose its bits."""
+    same = x.dtype == f.dtype == wz.dtype == torch.bfloat16
+    return torch.bfloat16 if same else torch.float32
 
 
 def _token_args(B, T, D, x, f, wz, A_log, dt_bias):
@@ -83,33 +90,39 @@ def _sequence_args(x, f, wz, A_log, dt_bias, h0, cu):
     return a
 
 
+def _forward(x, f, wz, A_log, dt_bias, h0, cu, want_final, train):
+    """y in the work type, the final state, and what the backward reads."""
+    B, T, D = x.shape
+    wd = _work_type(x, f, wz)
+    xw, fw, ww = _rows(x, wd), _rows(f, wd), _rows(wz, wd)
+    A, dt, h = _f32(A_log), _f32(dt_bias), _f32(h0)
+    if cu is not None:
+        cu = cu.to(torch.int32).contiguous()
+    rows = B if cu is None else cu.shape[0] - 1
+    dev = x.device
+    y = torch.empty((B, T, D), device=dev, dtype=wd)
+    final = torch.empty((rows, D), device=dev, dtype=torch.float32) if want_final else None
+    hs = None
+    if y.numel() == 0 or rows == 0:       # no token: the states stay
+        y.zero_()
+        if want_final:
+            final.copy_(h) if h is not None else final.zero_()
+    else:
+        a = _sequence_args(xw, fw, ww, A, dt, h, cu)
+        ws = torch.empty(_lib.lib().ngdn_recurrence_ws(B, T, D, 0), device=dev, dtype=torch.float32)
+        a.y, a.final_state, a.ws = y.data_ptr(), _lib.ptr(final), ws.data_ptr()
+        if train:
+            hs = torch.empty((B, -(-T // _lib.REC_RUN), D), device=dev, dtype=torch.float32)
+            a.hs = hs.data_ptr()
+        _lib.on_device(y, "ngdn_recurrence_fwd", _code(wd), ctypes.byref(a))
+    return y, final, (xw, fw, ww, A, dt, h, cu, hs)
+
+
 class _RecurrenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, wz, A_log, dt_bias, h0, cu, want_final):
-        B, T, D = x.shape
-        wd = x.dtype if x.dtype in _WORK else torch.float32
-        xw, fw, ww = _rows(x, wd), _rows(f, wd), _rows(wz, wd)
-        A, dt, h = _f32(A_log), _f32(dt_bias), _f32(h0)
-        if cu is not None:
-            cu = cu.to(torch.int32).contiguous()
-        rows = B if cu is None else cu.shape[0] - 1
-        dev = x.device
-        y = torch.empty((B, T, D), device=dev, dtype=wd)
-        final = torch.empty((rows, D), device=dev, dtype=torch.float32) if want_final else None
-        hs = None
-        if y.numel() == 0 or rows == 0:       # no token: the states stay
-            y.zero_()
-            if want_final:
-                final.copy_(h) if h is not None else final.zero_()
-        else:
-            a = _sequence_args(xw, fw, ww, A, dt, h, cu)
-            ws = torch.empty(_lib.lib().ngdn_recurrence_ws(B, T, D, 0), device=dev, dtype=torch.float32)
-            a.y, a.final_state, a.ws = y.data_ptr(), _lib.ptr(final), ws.data_ptr()
-            if any(ctx.needs_input_grad):
-                hs = torch.empty((B, -(-T // _lib.REC_RUN), D), device=dev, dtype=torch.float32)
-                a.hs = hs.data_ptr()
-            _lib.on_device(y, "ngdn_recurrence_fwd", _code(wd), ctypes.byref(a))
-        ctx.save_for_backward(xw, fw, ww, A, dt, h, cu, hs)
+        y, final, saved = _forward(x, f, wz, A_log, dt_bias, h0, cu, want_final, True)
+        ctx.save_for_backward(*saved)
         ctx.dtypes = (x.dtype, f.dtype, wz.dtype, A_log.dtype, dt_bias.dtype,
                       h0.dtype if h0 is not None else None)
         ctx.set_materialize_grads(False)
@@ -154,6 +167,8 @@ def _check(name, x, f, wz, A_log, dt_bias, dims):
     if D < 1 or dt_bias.shape != (D,) or A_log.dim() != 1 or A_log.shape[0] < 1 or D % A_log.shape[0]:
         raise ValueError(f"{name}: dt_bias {tuple(dt_bias.shape)}, A_log {tuple(A_log.shape)} for "
                          f"D={D} (dt_bias [D], A_log [H] with D a multiple of H)")
+    if max(x.shape) > _MOST:
+        raise ValueError(f"{name}: x {tuple(x.shape)} (sizes up to {_MOST})")
     for n, t in (("x", x), ("f", f), ("wz", wz), ("A_log", A_log), ("dt_bias", dt_bias)):
         if t.dtype not in _TYPES:
             raise ValueError(f"{name}: {n} is {t.dtype} (bf16, fp16 or fp32)")
@@ -174,13 +189,15 @@ def gated_recurrence(x, f, wz, A_log, dt_bias, initial_state=None, output_final_
     sequence s; the states are [S,D], and an empty sequence keeps its state.
     Tokens in no sequence have y = 0 and no effect on anything.
 
-    Differentiable once in every tensor; gradients have the bits of every
-    other run on the same inputs."""
+    Differentiable once in every tensor (not forward-mode); gradients have the
+    bits of every other run on the same inputs. To capture the backward into a
+    graph, let no eager graph of the same leaves live: autograd would then
+    leave the captured stream."""
     _check("gated_recurrence", x, f, wz, A_log, dt_bias, 3)
     B, T, D = x.shape
     rows = B
     if cu_seqlens is not None:
-        if (B != 1 or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1
+        if (B != 1 or cu_seqlens.dim() != 1 or not 1 <= cu_seqlens.shape[0] <= _MOST
                 or cu_seqlens.dtype not in (torch.int32, torch.int64)):
             raise ValueError(f"gated_recurrence: cu_seqlens {cu_seqlens.dtype} {tuple(cu_seqlens.shape)} "
                              f"with B={B} (int32 or int64 [S+1], B = 1)")
@@ -189,8 +206,12 @@ def gated_recurrence(x, f, wz, A_log, dt_bias, initial_state=None, output_final_
         raise ValueError(f"gated_recurrence: initial_state {tuple(initial_state.shape)}, expected "
                          f"{(rows, D)}")
     _on_gpu("gated_recurrence", x, f, wz, A_log, dt_bias, initial_state, cu_seqlens)
-    return _RecurrenceFn.apply(x, f, wz, A_log, dt_bias, initial_state, cu_seqlens,
-                               bool(output_final_state))
+    args = (x, f, wz, A_log, dt_bias, initial_state, cu_seqlens, bool(output_final_state))
+    if forward_ad._current_level < 0 and not (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in args[:6])):
+        y, final, _ = _forward(*args, False)
+        return y if y.dtype == x.dtype else y.to(x.dtype), final
+    return _RecurrenceFn.apply(*args)
 
 
 def step_gated_recurrence(x, f, wz, A_log, dt_bias, state, *, inplace=False):
@@ -207,13 +228,15 @@ def step_gated_recurrence(x, f, wz, A_log, dt_bias, state, *, inplace=False):
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, f, wz, A_log, dt_bias, state)):
         raise RuntimeError(f"{name} is forward-only (decoding); call it under torch.no_grad() or on "
                            "tensors that do not require grad")
-    wd = x.dtype if x.dtype in _WORK else torch.float32
+    wd = _work_type(x, f, wz)
     xw, fw, ww = _rows(x, wd), _rows(f, wd), _rows(wz, wd)
     A, dt = _f32(A_log), _f32(dt_bias)
     if inplace:
         if state.dtype != torch.float32 or not state.is_contiguous():
             raise ValueError(f"{name}: inplace=True needs a contiguous fp32 state")
         s_in = s_out = state
+        if not state.is_inference():        # a graph that saved it must not use the new values
+            torch.autograd.graph.increment_version(state)
     else:
         s_in = _f32(state)
         s_out = torch.empty_like(s_in)

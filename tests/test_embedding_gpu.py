@@ -298,3 +298,14 @@ def test_a_recurrent_language_model_step():
                                           inplace=True)
             # one fp32 product of 32 terms in another order each side, through 20 tokens
             assert (yt - y[:, t]).abs().max() < 1e-4
+
+
+def test_module_beyond_the_kernels_is_nn_embedding():
+    """fp16 and an empty table go to nn.Embedding, int32 ids do not."""
+    h = Embedding(50, 24).cuda().half()
+    ids = torch.randint(0, 50, (4, 30), device="cuda")
+    h(ids).sum().backward()
+    assert torch.equal(h(ids), F.embedding(ids, h.weight)) and h.weight.grad.dtype == torch.float16
+    assert Embedding(0, 24).cuda()(ids[:0]).shape == (0, 30, 24)
+    m = Embedding(50, 24).cuda()
+    assert torch.equal(m(ids.int()), F.embedding(ids, m.weight))

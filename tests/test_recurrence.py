@@ -168,3 +168,31 @@ def test_recurrence_struct_matches_header():
     ct = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "ptr": ctypes.c_void_p}
     assert [(n, ct[t]) for n, t in fields] == list(_lib.RecurrenceArgs._fields_)
     assert int(re.search(r"#define NGDN_REC_RUN (\d+)", text).group(1)) == _lib.REC_RUN
+
+
+def test_sizes_beyond_the_library_are_refused():
+    """Sizes are 32 bits in the library: a larger one must not wrap on its way."""
+    e = torch.zeros(1)
+    x = e.expand(1, 1 << 31, 1)
+    with pytest.raises(ValueError, match="sizes up to"):
+        gated_recurrence(x, x, x, e, e)
+    with pytest.raises(ValueError, match="sizes up to"):
+        step_gated_recurrence(x[0], x[0], x[0], e, e, x[0])
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        gated_recurrence(e.view(1, 1, 1), e.view(1, 1, 1), e.view(1, 1, 1), e, e,
+                         cu_seqlens=torch.zeros(1, dtype=torch.int32).expand((1 << 31) + 5))
+    with pytest.raises(ValueError, match="sizes up to"):
+        embedding(torch.zeros(1, dtype=torch.long), e.expand(1, (1 << 31) + 5))
+
+
+def test_recurrence_workspace_alignment_is_refused():
+    so = _lib.lib()
+    for name in ("ngdn_recurrence_fwd", "ngdn_recurrence_bwd"):
+        assert getattr(so, name)(1, ctypes.byref(_args(ws=4100)), None) == 1
+        assert b"aligned" in so.ngdn_last_error()
+
+
+def test_embedding_module_is_traced_as_torchs():
+    m = torch.nn.Sequential(Embedding(7, 3))
+    ids = torch.tensor([1, 6])
+    assert torch.equal(torch.fx.symbolic_trace(m)(ids), m(ids))

@@ -396,3 +396,92 @@ def test_prompt_then_tokens():
         ys.append(out.clone()[:, None])
     check("y", torch.cat(ys, 1), want["y"], torch.float32)
     check("final", state, want["final"], torch.float32)
+
+
+# ---------------------------------------------------------------- rows of many tiles, types, streams
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,D,H,S", [(3100, 70, 7, 60), (2500, 130, 2, 3), (4000, 9, 9, 900)])
+def test_long_packed_rows(T, D, H, S, dtype):
+    """Sequences over many workgroups' tiles, some empty, tokens before the first
+    and behind the last."""
+    g = torch.Generator().manual_seed(T + S)
+    cu = torch.sort(torch.randint(5, T - 40, (S + 1,), generator=g)).values
+    cu[S // 2] = cu[S // 2 - 1]
+    p, dy, dfinal = make(1, T, D, H, dtype, rows=S)
+    run_and_check(p, dy, dfinal, cu=cu.tolist())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,D,H", [(2, 5000, 66, 3), (1, 1024, 128, 1), (1, 1025, 64, 64)])
+def test_long_rows(B, T, D, H, dtype):
+    p, dy, dfinal = make(B, T, D, H, dtype)
+    run_and_check(p, dy, dfinal)
+
+
+@pytest.mark.parametrize("types", [(torch.bfloat16, torch.float32, torch.float32),
+                                   (torch.float32, torch.bfloat16, torch.float16),
+                                   (torch.float16, torch.bfloat16, torch.bfloat16)])
+def test_mixed_types_lose_nothing(types):
+    p, dy, dfinal = make(2, 150, 64, 4, torch.float32)
+    for n, t in zip(("x", "f", "wz"), types):
+        p[n] = p[n].to(t)
+    run_and_check(p, dy.to(types[0]), dfinal)
+    want = oracle.recurrence(*(p[n][:, :1] for n in NAMES[:3]), p["A_log"], p["dt_bias"], p["initial_state"])
+    s = gpu(p, grad=False)
+    y, state = step_gated_recurrence(*(s[n][:, 0] for n in NAMES[:3]), s["A_log"], s["dt_bias"],
+                                     s["initial_state"])
+    check("y", y[:, None], want["y"], types[0])
+    check("state", state, want["final"], torch.float32)
+
+
+def test_without_gradients_the_same_bits():
+    """Under no_grad (parameters that require it) and in inference mode."""
+    p, _, _ = make(2, 700, 66, 6, torch.bfloat16)
+    q = gpu(p)
+    args = [q[n] for n in NAMES]
+    y, f = gated_recurrence(*args, output_final_state=True)
+    with torch.no_grad():
+        y1, f1 = gated_recurrence(*args, output_final_state=True)
+    with torch.inference_mode():
+        y2, f2 = gated_recurrence(*args, output_final_state=True)
+        s = torch.zeros(2, 66, device="cuda")
+        step_gated_recurrence(*(q[n][:, 0] for n in NAMES[:3]), q["A_log"], q["dt_bias"], s, inplace=True)
+    assert y.requires_grad and not y1.requires_grad
+    assert torch.equal(y, y1) and torch.equal(f, f1) and torch.equal(y, y2) and torch.equal(f, f2)
+
+
+def test_calls_on_two_streams_at_once():
+    """Two long rows whose tiles wait for one another, each on a stream of its
+    own, forward and backward, against the same calls alone."""
+    def work(q, dy):
+        y, f = gated_recurrence(*(q[n] for n in NAMES), output_final_state=True)
+        return (y.detach(), f.detach(), *torch.autograd.grad([y, f], [q[n] for n in NAMES], [dy, torch.ones_like(f)]))
+
+    qs, dys = [], []
+    for k in range(2):
+        p, dy, _ = make(1, 20000, 512, 8, torch.bfloat16, seed=k)
+        qs.append(gpu(p))
+        dys.append(dy.cuda())
+    alone = [work(q, dy) for q, dy in zip(qs, dys)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    outs = [None, None]
+    for _ in range(4):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[k] = work(qs[k], dys[k])
+    torch.cuda.synchronize()
+    for a, b in zip(alone, outs):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_a_state_saved_by_a_graph_is_not_updated_behind_it():
+    p, _, _ = make(2, 1, 64, 4, torch.float32)
+    s = gpu(p, grad=False)
+    state = s["initial_state"]
+    w = torch.ones_like(state).requires_grad_()
+    out = (w * state).sum()
+    step_gated_recurrence(*(s[n][:, 0] for n in NAMES[:3]), s["A_log"], s["dt_bias"], state, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward()
