@@ -123,42 +123,52 @@ class _RecurrenceFn(torch.autograd.Function):
     def forward(ctx, x, f, wz, A_log, dt_bias, h0, cu, want_final):
         y, final, saved = _forward(x, f, wz, A_log, dt_bias, h0, cu, want_final, True)
         ctx.save_for_backward(*saved)
-        ctx.dtypes = (x.dtype, f.dtype, wz.dtype, A_log.dtype, dt_bias.dtype,
-                      h0.dtype if h0 is not None else None)
+        wd, f32 = y.dtype, torch.float32
+        types = (x.dtype, f.dtype, wz.dtype, A_log.dtype, dt_bias.dtype, f32 if h0 is None else h0.dtype)
+        ctx.dtypes = None if types == (wd, wd, wd, f32, f32, f32) else types
         ctx.set_materialize_grads(False)
         return y if y.dtype == x.dtype else y.to(x.dtype), final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy, dfinal):
-        xw, fw, ww, A, dt, h, cu, hs = ctx.saved_tensors
-        B, T, D = xw.shape
-        wd, dev = xw.dtype, xw.device
-        rows = B if cu is None else cu.shape[0] - 1
-        dh0 = torch.empty((rows, D), device=dev, dtype=torch.float32) if ctx.needs_input_grad[5] else None
-        dx = torch.empty((B, T, D), device=dev, dtype=wd)
-        df, dw = torch.empty_like(dx), torch.empty_like(dx)
-        dA, ddt = torch.empty_like(A), torch.empty_like(dt)
-        dfinal = _f32(dfinal)
-        if hs is None:
-            for t in (dx, df, dw, dA, ddt):
-                t.zero_()
-            if dh0 is not None:
-                dh0.copy_(dfinal) if dfinal is not None else dh0.zero_()
-        else:
-            dyw = _rows(dy, wd) if dy is not None else torch.zeros_like(dx)
-            a = _sequence_args(xw, fw, ww, A, dt, h, cu)
-            ws = torch.empty(_lib.lib().ngdn_recurrence_ws(B, T, D, 1), device=dev, dtype=torch.float32)
-            a.hs, a.ws, a.dy, a.dfinal = hs.data_ptr(), ws.data_ptr(), dyw.data_ptr(), _lib.ptr(dfinal)
-            a.dy_b, a.dy_t = dyw.stride(0), dyw.stride(1)
-            a.dx, a.df, a.dwz = dx.data_ptr(), df.data_ptr(), dw.data_ptr()
-            a.dA_log, a.ddt_bias, a.dh0 = dA.data_ptr(), ddt.data_ptr(), _lib.ptr(dh0)
-            _lib.on_device(dx, "ngdn_recurrence_bwd", _code(wd), ctypes.byref(a))
-        return (*(g if g is None or g.dtype == d else g.to(d)
-                  for g, d in zip((dx, df, dw, dA, ddt, dh0), ctx.dtypes)), None, None)
+        # once_differentiable's wrapping costs 3 us and is for a backward that a graph is made of
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, dy, dfinal)
 
 
-def _check(name, x, f, wz, A_log, dt_bias, dims):
+def _backward(ctx, dy, dfinal):
+    xw, fw, ww, A, dt, h, cu, hs = ctx.saved_tensors
+    B, T, D = xw.shape
+    wd, dev = xw.dtype, xw.device
+    rows = B if cu is None else cu.shape[0] - 1
+    dh0 = torch.empty((rows, D), device=dev, dtype=torch.float32) if ctx.needs_input_grad[5] else None
+    dx = torch.empty((B, T, D), device=dev, dtype=wd)
+    df, dw = torch.empty_like(dx), torch.empty_like(dx)
+    dA, ddt = torch.empty_like(A), torch.empty_like(dt)
+    dfinal = _f32(dfinal)
+    if hs is None:
+        for t in (dx, df, dw, dA, ddt):
+            t.zero_()
+        if dh0 is not None:
+            dh0.copy_(dfinal) if dfinal is not None else dh0.zero_()
+    else:
+        dyw = _rows(dy, wd) if dy is not None else torch.zeros_like(dx)
+        a = _sequence_args(xw, fw, ww, A, dt, h, cu)
+        ws = torch.empty(_lib.lib().ngdn_recurrence_ws(B, T, D, 1), device=dev, dtype=torch.float32)
+        a.hs, a.ws, a.dy, a.dfinal = hs.data_ptr(), ws.data_ptr(), dyw.data_ptr(), _lib.ptr(dfinal)
+        a.dy_b, a.dy_t = dyw.stride(0), dyw.stride(1)
+        a.dx, a.df, a.dwz = dx.data_ptr(), df.data_ptr(), dw.data_ptr()
+        a.dA_log, a.ddt_bias, a.dh0 = dA.data_ptr(), ddt.data_ptr(), _lib.ptr(dh0)
+        _lib.on_device(dx, "ngdn_recurrence_bwd", _code(wd), ctypes.byref(a))
+    grads = (dx, df, dw, dA, ddt, dh0)
+    if ctx.dtypes:
+        grads = (g if g is None else g.to(d) for g, d in zip(grads, ctx.dtypes))
+    return *grads, None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
+def _check(name, x, f, wz, A_log, dt_bias, state, dims):
     if x.dim() != dims or f.shape != x.shape or wz.shape != x.shape:
         want = "[B,T,D]" if dims == 3 else "[B,D]"
         raise ValueError(f"{name}: x {tuple(x.shape)}, f {tuple(f.shape)}, wz {tuple(wz.shape)} "
@@ -169,8 +179,8 @@ def _check(name, x, f, wz, A_log, dt_bias, dims):
                          f"D={D} (dt_bias [D], A_log [H] with D a multiple of H)")
     if max(x.shape) > _MOST:
         raise ValueError(f"{name}: x {tuple(x.shape)} (sizes up to {_MOST})")
-    for n, t in (("x", x), ("f", f), ("wz", wz), ("A_log", A_log), ("dt_bias", dt_bias)):
-        if t.dtype not in _TYPES:
+    for n, t in (("x", x), ("f", f), ("wz", wz), ("A_log", A_log), ("dt_bias", dt_bias), ("the state", state)):
+        if t is not None and t.dtype not in _TYPES:
             raise ValueError(f"{name}: {n} is {t.dtype} (bf16, fp16 or fp32)")
 
 
@@ -193,7 +203,7 @@ def gated_recurrence(x, f, wz, A_log, dt_bias, initial_state=None, output_final_
     bits of every other run on the same inputs. To capture the backward into a
     graph, let no eager graph of the same leaves live: autograd would then
     leave the captured stream."""
-    _check("gated_recurrence", x, f, wz, A_log, dt_bias, 3)
+    _check("gated_recurrence", x, f, wz, A_log, dt_bias, initial_state, 3)
     B, T, D = x.shape
     rows = B
     if cu_seqlens is not None:
@@ -220,7 +230,7 @@ def step_gated_recurrence(x, f, wz, A_log, dt_bias, state, *, inplace=False):
     modified, or with ``inplace=True`` (fp32, contiguous) updated and
     returned, which keeps the buffer fixed for graph capture. Forward only."""
     name = "step_gated_recurrence"
-    _check(name, x, f, wz, A_log, dt_bias, 2)
+    _check(name, x, f, wz, A_log, dt_bias, state, 2)
     B, D = x.shape
     if tuple(state.shape) != (B, D):
         raise ValueError(f"{name}: state {tuple(state.shape)}, expected {(B, D)}")

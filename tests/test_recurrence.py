@@ -196,3 +196,12 @@ def test_embedding_module_is_traced_as_torchs():
     m = torch.nn.Sequential(Embedding(7, 3))
     ids = torch.tensor([1, 6])
     assert torch.equal(torch.fx.symbolic_trace(m)(ids), m(ids))
+
+
+def test_states_of_other_types_are_refused():
+    x, h = torch.zeros(1, 2, 4), torch.zeros(1, 4)
+    for bad in (h.double(), h.long()):
+        with pytest.raises(ValueError, match="the state is"):
+            gated_recurrence(x, x, x, h[0, :2], h[0], initial_state=bad)
+        with pytest.raises(ValueError, match="the state is"):
+            step_gated_recurrence(h, h, h, h[0, :2], h[0], bad)
