@@ -141,12 +141,11 @@ __device__ __forceinline__ void params(const RecArgs& a, unsigned d, float& bias
 // A workgroup has W waves, each a run of N tokens of 64 channels (a strip): a
 // tile of W runs. The state that enters a tile comes from the tiles before it (in
 // the backward: behind it) while those are still running, through device memory:
-// every tile publishes its (A, H) as soon as it has them; the last of a group of W
-// also the state behind it. A tile takes the state at its group's start and the
-// (A, H) of the tiles between, a wave each, so the chain over a long row has a
-// link a group, and the order of the arithmetic does not depend on timing. Groups
-// of 2 W: 16384 x 512 forward 25.0 us against 26.2, 4 x 6000 x 2048 98.3 against
-// 97.4, within noise elsewhere.
+// every tile publishes its (A, H) as soon as it has them; the last of a group of
+// W EACH also the state behind it. A tile takes the state at its group's start and
+// the (A, H) of the tiles between, so the chain over a long row has a link a
+// group, and the order of the arithmetic does not depend on timing. EACH 1, 2, 4,
+// both passes: 65536 x 64 100, 70, 59 us; 4 x 8192 x 2048 323, 327, 332.
 // One 64-bit (32-bit) value is its own flag: all bits set before it is
 // published, which no published value has (a NaN of that pattern is changed).
 // A strip's tiles are handed out by a counter, so all a tile waits for was
@@ -163,6 +162,7 @@ __device__ __forceinline__ void params(const RecArgs& a, unsigned d, float& bias
 
 constexpr int W = REC_WAVES;
 constexpr int LINE = 32;            // ints in a cache line
+constexpr int EACH = 2;             // tiles that a wave looks at, W EACH of them a group
 
 struct Sync {
   int* ticket;                      // [nstrip] counters, LINE apart (NULL: one tile a row, nothing to join)
@@ -268,8 +268,9 @@ __device__ __forceinline__ float join_tiles(Joint& s, const Sync& y, int step, i
   lds_barrier();
   float h = first;
   if (y.ticket) {
-    const int group = step / W, n = step - group * W;         // n tiles from the group's start
-    const bool go = step + 1 < y.nchunk, link = n == W - 1 && go;
+    constexpr int per = W * EACH;
+    const int group = step / per, n = step - group * per;      // n tiles from the group's start
+    const bool go = step + 1 < y.nchunk, link = n == per - 1 && go;
     auto agg = [&](int k) { return y.agg + ((long long)k * y.nstrip + strip) * 64 + l; };
     auto base = [&](int k) { return y.base + ((long long)k * y.nstrip + strip) * 64 + l; };
     float tA = 1.f, tH = 0.f;                                 // the whole tile
@@ -279,21 +280,26 @@ __device__ __forceinline__ float join_tiles(Joint& s, const Sync& y, int step, i
       publish(agg(step), tA, tH);
     }
     if (step > 0) {
-      // each wave one of the n tiles, the last, which has none, the state at the
-      // group's start, which it looks at before it waits for the tiles
-      const bool one = wv < n, far = wv == W - 1 && group > 0;
+      // each wave EACH of the n tiles in order; the last wave also the state at the
+      // group's start. All are looked at before the first is waited for
+      const int k0 = wv * EACH, k1 = k0 + EACH < n ? k0 + EACH : n;
+      const bool far = wv == W - 1 && group > 0;
       const unsigned hb = far ? peek(base(group)) : bits(first);
-      if (one) {
-        const unsigned long long* p = agg(group * W + wv);
-        s.before[wv][l] = pair(await(p, peek(p)));
-      }
+      unsigned long long v[EACH];
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) v[i] = k0 + i < k1 ? peek(agg(group * per + k0 + i)) : 0;
+      float bA = 1.f, bH = 0.f;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+        if (k0 + i < k1) join<PACKED>(bA, bH, pair(await(agg(group * per + k0 + i), v[i])));
+      s.before[wv][l] = make_float2(bA, bH);
       // the group's last tile is a link of the chain: everything up to its own end is
       // joined before the state at its start is there, which then goes on in one operation
       if (link) lds_barrier();
       if (wv == W - 1) {
         float gA = 1.f, gH = 0.f;
         if (link) {
-          for (int k = 0; k < n; ++k) join<PACKED>(gA, gH, s.before[k][l]);
+          for (int k = 0; k * EACH < n; ++k) join<PACKED>(gA, gH, s.before[k][l]);
           join<PACKED>(gA, gH, make_float2(tA, tH));
         }
         h = __uint_as_float(far ? await(base(group), hb) : hb);
@@ -302,7 +308,7 @@ __device__ __forceinline__ float join_tiles(Joint& s, const Sync& y, int step, i
       }
       lds_barrier();
       h = s.base[l];
-      for (int k = 0; k < n; ++k) h = pass<PACKED>(h, s.before[k][l]);
+      for (int k = 0; k * EACH < n; ++k) h = pass<PACKED>(h, s.before[k][l]);
     }
   }
   for (int k = 0; k < wv; ++k) h = pass<PACKED>(h, s.wave[k][l]);
@@ -689,7 +695,7 @@ Space space(long long B, long long T, long long D, bool backward) {
   const bool many = s.nchunk > 1;
   s.agg = many ? wide / 64 * LINE : 16;
   s.base = s.agg + (many ? 2 * s.nchunk * wide : 0);
-  s.runs = s.base + (many ? (s.nchunk / W + 1) * wide : 0);
+  s.runs = s.base + (many ? (s.nchunk / (W * EACH) + 1) * wide : 0);
   s.parts = s.runs + (B == 1 ? 4 * ((T + N - 1) / N) : 0);
   s.sums = s.parts + (backward ? 2 * B * s.nchunk * D : 0);
   s.all = s.sums + (backward ? 2 * REC_SLICES * D : 0);
