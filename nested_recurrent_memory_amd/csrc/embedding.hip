@@ -26,7 +26,8 @@ __device__ __forceinline__ void put(E* p, const float* x) {
 }  // namespace
 
 // 2^lg lanes a row (the least that hold it in one pass, at most a wave), each
-// taking VEC values at a time.
+// taking VEC values at a time. Bound by HBM: 32768 x 1024 from fp32 to bf16 20 us
+// (102 MB with the distinct rows of the table), 131072 x 2048 175 us (870 MB).
 template <typename W, typename Y, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a, int lg) {
   constexpr int AHEAD = 4;                   // loads before the first store; 131072 x 2048 fp32 to bf16 184 -> 175 us
@@ -159,7 +160,9 @@ __device__ __forceinline__ int scan_digits(int v, int* s_part) {
 
 }  // namespace
 
-// The whole sort of at most ONE ids (block 0); the other blocks clear dw.
+// The whole sort of at most ONE ids (block 0); the other blocks clear dw. 8192 ids
+// of a table of 32000 rows: 21.5 us, two passes' latency in one workgroup, beside
+// which 128 MiB are cleared.
 __global__ __launch_bounds__(ST) void embed_sort_one(SortArgs s) {
   __shared__ int s_key[ONE], s_pos[ONE], s_count[SW][BUCKETS], s_total[BUCKETS], s_part[SW];
   if (blockIdx.x > 0) {
@@ -207,7 +210,7 @@ __device__ __forceinline__ int pass_key(const SortArgs& s, int i) {
   return i >= s.N ? FILLER : s.shift == 0 ? key_of(s, s.ids[i]) : s.key[0][i];
 }
 
-// One pass over blocks: their counts of every digit.
+// One pass over blocks: their counts of every digit. 131072 ids 9 us, the scatter 15.
 __global__ __launch_bounds__(ST) void embed_count(SortArgs s) {
   __shared__ int s_count[BUCKETS];
   if ((int)blockIdx.x >= s.nblock) {
@@ -284,6 +287,9 @@ __global__ __launch_bounds__(ST) void embed_scatter(SortArgs s) {
 // segment is summed there; of one that crosses segments each leaves its part
 // (parts[2 k] what came into segment k from before, [2 k + 1] what starts in it
 // and goes on), added in order by embed_join.
+// 131072 x 2048 in bf16 into 131072 rows of fp32: 315 us, 0.54 GB read and 0.94 GB
+// written (rows without a sum are cleared here), at 4.7 TB/s; clearing first or
+// mixed among the sums 342 and 334, with non-temporal stores 470.
 
 struct EmbedSum {
   const int* key; const int* pos;
@@ -382,7 +388,8 @@ __global__ __launch_bounds__(256) void embed_sum(EmbedSum a) {
 
 // The ids that cross segments: the part of the segment they start in and of
 // those behind it, each of the workgroup's waves a stretch of them in order.
-// The list of segments is in any order, what is added for one is not.
+// The list of segments is in any order, what is added for one is not. 20 us at
+// the same size: the most frequent ids' parts, one after another.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void embed_join(EmbedSum a) {
   __shared__ float s_acc[4][WAVE * VEC];
@@ -428,7 +435,9 @@ __global__ __launch_bounds__(256) void embed_join(EmbedSum a) {
 
 // The whole gradient of at most FEW ids in one launch: a workgroup has HAND rows
 // of dw, looks all ids over for them, and its waves take the rows' tiles of 64
-// VEC columns in turn, to clear them or to add what points at them.
+// VEC columns in turn, to clear them or to add what points at them. 256 ids into
+// 32000 x 1024: 25 us (131 MB cleared), 33 sorted; every workgroup reads all ids, so
+// not beyond the ids that a workgroup has threads for.
 constexpr int FEW = 256, HAND = 16;
 template <typename G, typename T, int VEC>
 __global__ __launch_bounds__(FEW) void embed_few(EmbedArgs a) {
