@@ -23,32 +23,40 @@ constexpr int N = REC_RUN;          // tokens a run, which a wave has in registe
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-// e^(ln2 p) - 1 = ln2 p (1 + ...): the coefficients of -(2^p - 1) / p
-constexpr float EM1 = 0.69314718055994531f, EM2 = 0.24022650695910071f, EM3 = 0.05550410866482158f,
-                EM4 = 0.00961812910762848f;
+// (1 - 4^p) / -p by its series: with p = g log2(e) 1 - e^2g
+constexpr float Q1 = 1.3862943611198906f, Q2 = 0.96090602783640278f, Q3 = 0.44403286931857261f,
+                Q4 = 0.15389006572205563f, Q5 = 0.042667386068571012f;
 
-// What a token's decay needs: a = e^g, q = 1 - a^2, g2 = g log2(e), and the
-// sigmoid's parts (e = e^-|z|, up = z >= 0).
+// What a token's decay needs: a = e^g, q = 1 - a^2, g2 = g log2(e), and ls = log2
+// of sigmoid(z).
 struct Decay {
-  float a, q, g2, e;
-  bool up;
+  float a, q, g2, ls;
 };
 
+// The first coefficients of both polynomials. An instruction takes one constant:
+// held in registers, where there are any left, they save two moves a token.
+struct First {
+  float p, q;
+};
+constexpr First FIRST{-0.012319466099143028f, Q5};
+__device__ __forceinline__ First held() {
+  First k = FIRST;
+  asm volatile("" : "+v"(k.p), "+v"(k.q));
+  return k;
+}
+
 // z2 = z log2(e) = f log2(e) + bias2, nrate = -exp(A_log).
-// softplus(z) log2(e) = max(z2, 0) + log2(1 + e): the logarithm as e P(e), P
-// the degree-7 polynomial of least relative error on [0, 1] (3e-7 in fp32),
-// which keeps its relative precision for the small e where decays usually sit;
-// log2(1 + e) itself loses e's low bits there.
-// 1 - a from the series of e^g - 1 for -g < 1/16 (relative error 1e-7), where
-// the subtraction would cancel, and q = (1 - a)(1 + a).
-__device__ __forceinline__ Decay decay(float f, float bias2, float nrate) {
+// softplus(z) log2(e) = max(z2, 0) + log2(1 + e), e = e^-|z|: the logarithm as
+// e P(e), P the degree-7 polynomial of least relative error on [0, 1] (3e-7 in
+// fp32), which keeps its relative precision for the small e where decays usually
+// sit; log2(1 + e) itself loses e's low bits there. And log2 sigmoid(z) =
+// min(z2, 0) - e P(e), in one instruction where a reciprocal took six.
+// q from the series for -g < 1/16 (its error 4e-8), where 1 - a^2 would cancel.
+__device__ __forceinline__ Decay decay(float f, float bias2, float nrate, const First& k) {
   Decay d;
   const float z2 = fmaf(f, LOG2E, bias2);
-  d.up = z2 >= 0.f;
-  d.e = __builtin_amdgcn_exp2f(-fabsf(z2));
-  const float e = d.e;
-  float p = -0.012319466099143028f;
-  p = fmaf(p, e, 0.06360787153244019f);
+  const float e = __builtin_amdgcn_exp2f(-fabsf(z2));
+  float p = fmaf(k.p, e, 0.06360787153244019f);
   p = fmaf(p, e, -0.15535186231136322f);
   p = fmaf(p, e, 0.2560097277164459f);
   p = fmaf(p, e, -0.35339483618736267f);
@@ -56,23 +64,16 @@ __device__ __forceinline__ Decay decay(float f, float bias2, float nrate) {
   p = fmaf(p, e, -0.7213100790977478f);
   p = fmaf(p, e, 1.4426947832107544f);
   d.g2 = nrate * fmaf(p, e, fmaxf(z2, 0.f));
+  d.ls = fmaf(-p, e, fminf(z2, 0.f));
   d.a = __builtin_amdgcn_exp2f(d.g2);
   const float g2 = d.g2;
-  const float s = -g2 * fmaf(g2, fmaf(g2, fmaf(g2, EM4, EM3), EM2), EM1);
-  const float t = g2 > -LOG2E / 16.f ? s : 1.f - d.a;
-  d.q = t * (2.f - t);
+  const float s = -g2 * fmaf(g2, fmaf(g2, fmaf(g2, fmaf(g2, k.q, Q4), Q3), Q2), Q1);
+  d.q = g2 > -LOG2E / 16.f ? s : fmaf(-d.a, d.a, 1.f);
   return d;
 }
 
 __device__ __forceinline__ float sigmoid2(float w) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * w));
-}
-
-// beta and 1 / beta. A q of 0 (a decay that rounds to 1) is lifted so that
-// 1 / beta stays finite: it is multiplied by e, which is 0 there.
-__device__ __forceinline__ void root(float q, float& beta, float& inv) {
-  inv = __builtin_amdgcn_rsqf(fmaxf(q, 1e-37f));
-  beta = q * inv;
 }
 
 // Where the tokens [t0, t0 + n) of a packed row stand: bit j of start / end /
@@ -236,6 +237,15 @@ template <typename E>
 __device__ __forceinline__ void store_at(E* row, unsigned bytes, float x) {
   *(Device<E>*)((Device<char>*)row + bytes) = from_f<E>(x);
 }
+// Two tokens' rows, one conversion.
+template <typename E>
+__device__ __forceinline__ void store_two(E* r0, E* r1, unsigned bytes, float x0, float x1) {
+  typedef E Pair __attribute__((ext_vector_type(2)));
+  typedef float Two __attribute__((ext_vector_type(2)));
+  const Pair p = __builtin_convertvector((Two{x0, x1}), Pair);
+  *(Device<E>*)((Device<char>*)r0 + bytes) = p.x;
+  *(Device<E>*)((Device<char>*)r1 + bytes) = p.y;
+}
 // The compiler takes that form only where it sees the 32 bits widened in the same block.
 __device__ __forceinline__ unsigned here(unsigned bytes) {
   asm volatile("" : "+v"(bytes));
@@ -374,8 +384,9 @@ __global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long lon
 // h_t = H_t + P_t h_in from one pass, then y.
 // Three values of a token and channel are read and one written, in bf16 8 bytes:
 // 65536 x 2048 in 225 us, 4.8 TB/s where a large copy reaches 5.2. Behind that
-// bound lies the next: vector instructions are issued 3/4 of the time (43 a token,
-// 5 of them transcendental). 333 x 1024: 7.5 us, three tiles' loads and joins.
+// bound lies the next: vector instructions are issued 4/5 of the time (42 a token, 5
+// of them transcendental). More waves a CU (64 registers, a few spilled) took 251 us.
+// 333 x 1024: 7.5 us, three tiles' loads and joins.
 template <typename E, bool PACKED>
 __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) {
   __shared__ Joint s_join;
@@ -396,10 +407,11 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
   const float first = a.h0 && !PACKED ? a.h0[(long long)b * a.D + dl] : 0.f;
   Run r{0u, 0u, 0u, 0, 0};
   if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
+  const First c0 = FIRST;
   float P[N], H[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const Decay k = decay(to_f(v[0][j]), bias2, nrate);
+    const Decay k = decay(to_f(v[0][j]), bias2, nrate, c0);
     P[j] = k.a;
     H[j] = __builtin_amdgcn_sqrtf(k.q) * sigmoid2(to_f(v[1][j])) * to_f(v[2][j]);
   }
@@ -448,7 +460,7 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
   if (n >= N) {
     const unsigned o = here(lane);
 #pragma unroll
-    for (int j = 0; j < N; ++j, yp += a.D) store_at(yp, o, H[j]);
+    for (int j = 0; j < N; j += 2, yp += 2LL * a.D) store_two(yp, yp + a.D, o, H[j], H[j + 1]);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j, yp += a.D)
@@ -477,12 +489,14 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
 // One pass over the run's tokens in order forms the gates again, the states from
 // hs, what lam_t multiplies in each gradient, and (A, C) with c = A c_in + C for
 // what flows out of the run backwards (c_t = a_t lam_t). The parameter gradients'
-// sums over tokens, sum lam_t k_t, need no second array: with
-// G_t = a_t G_(t-1) + k_t they are sum dy_t G_t + c_in G_last.
+// sums over tokens: dt_bias' of df as it is formed; A_log's, sum lam_t k_t with k_t =
+// ki_t g_t, needs no second array: with G_t = a_t G_(t-1) + k_t it is
+// sum dy_t G_t + c_in G_last.
 // Four values of a token and channel are read, three written: 4 x 8192 x 2048 in
-// bf16 195 us, 4.8 TB/s. A branch a token where a row or sequence may end: without
-// (straight code, rows of whole runs) 16 % fewer vector instructions took the same
-// 203 us then, as the loads bound it, and two copies of the loop spill.
+// bf16 195 us, 4.8 TB/s. Its 75 vector instructions a token are issued 4/5 of the
+// time; a tenth fewer (sigmoid(z) from its logarithm, df summed as it is formed)
+// took 1 % off. A branch a token where a row or sequence may end: straight code for
+// rows of whole runs was no faster, and two copies of the loop spill.
 template <typename E, bool PACKED>
 __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, float* parts) {
   __shared__ Joint s_join;
@@ -506,7 +520,8 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
   Run r{0u, 0u, 0u, 0, 0};
   if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
   float aa[N], bs[N], kw[N], kf[N], dy[N];
-  float A = 1.f, C = 0.f, Gb = 0.f, Ga = 0.f, sb = 0.f, sa = 0.f;
+  const First c0 = held();
+  float A = 1.f, C = 0.f, Ga = 0.f, sb = 0.f, sa = 0.f;
   int cur = r.cur;
   bool open = true;                        // no sequence has ended in the run yet
 #pragma unroll
@@ -516,32 +531,28 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
     if (!us) {
       aa[j] = PACKED ? 0.f : 1.f;          // behind the row the gradient passes
       bs[j] = kw[j] = kf[j] = dy[j] = 0.f;
-      if (PACKED) Gb = Ga = 0.f;
+      if (PACKED) Ga = 0.f;
       continue;
     }
     if (PACKED && (st || en)) {
       if (st) cur = seq_from(a.cu, a.S, cur, t0 + j);
       if (cur < 0) cur = 0;
     }
-    const float xv = to_f(v[2][j]);
-    const Decay k = decay(to_f(v[0][j]), bias2, nrate);
-    float beta, inv;
-    root(k.q, beta, inv);
-    const float s = sigmoid2(to_f(v[1][j]));
-    const float one = __builtin_amdgcn_rcpf(1.f + k.e), sz = k.up ? one : k.e * one;
+    const Decay k = decay(to_f(v[0][j]), bias2, nrate, c0);
+    // 1 / beta; a q of 0 (a decay that rounds to 1) is lifted so that it stays finite
+    const float inv = __builtin_amdgcn_rsqf(fmaxf(k.q, 1e-37f));
+    const float xv = to_f(v[2][j]), s = sigmoid2(to_f(v[1][j])), si = s * inv;
     if (st) h = a.h0 ? a.h0[(long long)cur * a.D + dl] : 0.f;
-    const float u = beta * s * xv, ah = k.a * h;
-    const float ki = ah - k.a * k.a * inv * (s * xv);       // dg = lam ki
     aa[j] = k.a;
-    bs[j] = beta * s;
-    kw[j] = u * (1.f - s);
-    kf[j] = nrate * sz * ki;
+    bs[j] = k.q * si;
+    const float u = bs[j] * xv;
+    const float ki = fmaf(k.a, h, -(k.a * k.a) * (si * xv));        // dg = lam ki
+    kw[j] = fmaf(-u, s, u);
+    kf[j] = nrate * __builtin_amdgcn_exp2f(k.ls) * ki;
     dy[j] = to_f(v[3][j]);
     if (en && a.dfinal) dy[j] += a.dfinal[(long long)cur * a.D + dl];
-    h = ah + u;
-    Gb = st ? kf[j] : fmaf(k.a, Gb, kf[j]);
+    h = fmaf(k.a, h, u);
     Ga = st ? ki * k.g2 : fmaf(k.a, Ga, ki * k.g2);
-    sb = fmaf(dy[j], Gb, sb);
     sa = fmaf(dy[j], Ga, sa);
     if (open) {
       A *= k.a;
@@ -555,7 +566,6 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
   // what comes from behind a run whose last token is the last of its sequence
   // (or in none) is not for it
   if (PACKED && (n < N || (r.end >> (N - 1) & 1) || !(r.used >> (N - 1) & 1))) c = 0.f;
-  sb = fmaf(c, Gb, sb);
   sa = fmaf(c, Ga, sa);
   if (live) {
     const long long o = ((long long)b * a.T + t0) * a.D;
@@ -564,12 +574,14 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
       E* dw = static_cast<E*>(a.dwz) + o + (N - 1LL) * a.D;
       const unsigned l = here(lane);
 #pragma unroll
-      for (int j = N - 1; j >= 0; --j, dx -= a.D, df -= a.D, dw -= a.D) {
-        const float lam = dy[j] + c;
-        c = aa[j] * lam;
-        store_at(dx, l, lam * bs[j]);
-        store_at(df, l, lam * kf[j]);
-        store_at(dw, l, lam * kw[j]);
+      for (int j = N - 1; j > 0; j -= 2, dx -= 2LL * a.D, df -= 2LL * a.D, dw -= 2LL * a.D) {
+        const float l1 = dy[j] + c, l0 = fmaf(aa[j], l1, dy[j - 1]), f1 = l1 * kf[j], f0 = l0 * kf[j - 1];
+        c = aa[j - 1] * l0;
+        sb += f1;
+        sb += f0;
+        store_two(dx, dx - a.D, l, l1 * bs[j], l0 * bs[j - 1]);
+        store_two(df, df - a.D, l, f1, f0);
+        store_two(dw, dw - a.D, l, l1 * kw[j], l0 * kw[j - 1]);
       }
     } else {
       cur = r.last;
@@ -582,7 +594,9 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
         if (j < n) {
           const long long q = o + (long long)j * a.D + d;
           static_cast<E*>(a.dx)[q] = from_f<E>(lam * bs[j]);
-          static_cast<E*>(a.df)[q] = from_f<E>(lam * kf[j]);
+          const float fj = lam * kf[j];
+          sb += fj;
+          static_cast<E*>(a.df)[q] = from_f<E>(fj);
           static_cast<E*>(a.dwz)[q] = from_f<E>(lam * kw[j]);
           if (PACKED && st && us && a.dh0) {
             cur = seq_before(a.cu, a.S, cur, t0 + j);
@@ -684,7 +698,7 @@ __global__ __launch_bounds__(256) void rec_step_kernel(RecArgs a) {
   const float w = to_f(static_cast<const E*>(a.wz)[b * a.w_b + d]);
   float bias2, nrate;
   params(a, d, bias2, nrate);
-  const Decay k = decay(f, bias2, nrate);
+  const Decay k = decay(f, bias2, nrate, FIRST);
   const float h = fmaf(k.a, a.h0[i], __builtin_amdgcn_sqrtf(k.q) * sigmoid2(w) * x);
   a.final_state[i] = h;
   static_cast<E*>(a.y)[i] = from_f<E>(h);
