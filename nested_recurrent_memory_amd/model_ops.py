@@ -72,6 +72,12 @@ def _embed(t):
 
 
 def _lookup(ids, weight, scale, ydt):
+    if weight.dtype == torch.float16:
+        # the rows' bits through the kernel, which at scale 1 moves bfloat16 as it is (its
+        # infinities and NaN are NaN in float16 too), then their values in float32: not
+        # the whole table's
+        rows = _lookup(ids, weight.view(torch.bfloat16), 1.0, torch.bfloat16).view(torch.float16)
+        return rows.float().mul_(scale).to(ydt)
     w = _embed(weight)
     V, D = w.shape
     y = w.new_empty((*ids.shape, D), dtype=ydt if ydt in _EMBED else torch.float32)

@@ -309,3 +309,15 @@ def test_module_beyond_the_kernels_is_nn_embedding():
     assert Embedding(0, 24).cuda()(ids[:0]).shape == (0, 30, 24)
     m = Embedding(50, 24).cuda()
     assert torch.equal(m(ids.int()), F.embedding(ids, m.weight))
+
+
+@pytest.mark.parametrize("D", [8, 13])
+def test_fp16_rows_keep_every_value(D):
+    """All 65536 values of fp16 at scale 1, bit for bit but for the NaN's payloads."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16)
+    w = torch.cat((bits, bits[:-65536 % D])) if 65536 % D else bits
+    w = w.view(torch.float16).view(-1, D).cuda()
+    ids = torch.arange(w.shape[0], device="cuda").flip(0)
+    y, want = embedding(ids, w), w.flip(0)
+    same = (y.view(torch.int16) == want.view(torch.int16)) | (y.isnan() & want.isnan())
+    assert y.dtype == torch.float16 and same.all()

@@ -485,3 +485,31 @@ def test_a_state_saved_by_a_graph_is_not_updated_behind_it():
     step_gated_recurrence(*(s[n][:, 0] for n in NAMES[:3]), s["A_log"], s["dt_bias"], state, inplace=True)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.backward()
+
+
+def test_a_long_row_captured_in_a_graph():
+    """More tiles than a link of the chain joins; replays with new inputs between
+    eager calls, each against the eager result."""
+    p, dy, dfinal = make(1, 4500, 130, 2, torch.bfloat16)
+    s = gpu(p, grad=False)
+    dy, dfinal = dy.cuda(), dfinal.cuda()
+
+    def work():
+        q = [s[n].detach().requires_grad_(True) for n in NAMES]
+        y, f = gated_recurrence(*q, output_final_state=True)
+        return (y.detach(), f.detach(), *torch.autograd.grad([y, f], q, [dy, dfinal]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = work()
+    for i in range(4):
+        for name, t in make(1, 4500, 130, 2, torch.bfloat16, seed=20 + i)[0].items():
+            s[name].copy_(t)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, work())), i
