@@ -343,11 +343,10 @@ __device__ __forceinline__ int take(const Sync& y, int strip, Joint& s) {
   return __builtin_amdgcn_readfirstlane(s.step);
 }
 
-// (2 to 6 us, the launch and the flags' bytes, 0.8 % of the pass's.)
 // Before either pass: the flags' patterns, the counters, where the boundaries of
 // packed sequences fall in each run, and sequences without tokens (out = in or
 // 0: their final state is their initial one, their initial state's gradient the
-// final one's).
+// final one's). 2 to 6 us, a launch and 0.8 % of the pass's bytes.
 __global__ __launch_bounds__(256) void rec_init(RecArgs a, uint4* fill, long long n16, int* ticket, int tickets,
                                                 int4* runs, const float* in, float* out) {
   const unsigned i0 = blockIdx.x * 256 + threadIdx.x, step = gridDim.x * 256;
@@ -393,7 +392,8 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
   const int strip = strip_of(sy), chunk = take(sy, strip, s_join), wv = wave_id(), b = strip / sy.strips;
   const int d = strip % sy.strips * 64 + lane_id();
   const bool live = d < a.D;
-  const unsigned dl = live ? d : 0, lane = dl * (unsigned)sizeof(E);                        // lanes behind D work on channel 0 and store nothing
+  // lanes behind D work on channel 0 and store nothing
+  const unsigned dl = live ? d : 0, lane = dl * (unsigned)sizeof(E);
   const int t0 = (chunk * W + wv) * N, n = a.T - t0 < N ? a.T - t0 : N;     // n <= 0: no token
   const long long ts = n > 0 ? t0 : a.T - 1;
   E v[3][N];                                          // f, wz, x
