@@ -513,3 +513,12 @@ def test_a_long_row_captured_in_a_graph():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, work())), i
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,D,H", [(1, 256, 70, 7), (3, 257, 64, 1), (2, 250, 9, 9), (4, 300, 4096, 64),
+                                     (4, 512, 4095, 5), (5, 513, 3333, 1)])
+def test_rows_of_few_tiles(B, T, D, H, dtype):
+    """Around the sizes of one, two and a few tiles, with many strips too."""
+    p, dy, dfinal = make(B, T, D, H, dtype)
+    run_and_check(p, dy, dfinal)
