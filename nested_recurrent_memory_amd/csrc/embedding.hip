@@ -12,15 +12,33 @@ namespace ngdn {
 
 namespace {
 
+// VEC values at p, aligned to their size
 template <typename E, int VEC>
 __device__ __forceinline__ void get(const E* p, float* o) {
-  if constexpr (VEC == 8) load8f(p, o);
-  else o[0] = to_f(*p);
+  typedef E Vec __attribute__((ext_vector_type(4)));
+  if constexpr (VEC == 8) {
+    load8f(p, o);
+  } else if constexpr (VEC == 4) {
+    const Vec v = *reinterpret_cast<const Vec*>(p);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (float)v[e];
+  } else {
+    o[0] = to_f(*p);
+  }
 }
 template <typename E, int VEC>
 __device__ __forceinline__ void put(E* p, const float* x) {
-  if constexpr (VEC == 8) store8f(p, x);
-  else *p = from_f<E>(x[0]);
+  typedef E Vec __attribute__((ext_vector_type(4)));
+  if constexpr (VEC == 8) {
+    store8f(p, x);
+  } else if constexpr (VEC == 4) {
+    Vec v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (E)x[e];
+    *reinterpret_cast<Vec*>(p) = v;
+  } else {
+    *p = from_f<E>(x[0]);
+  }
 }
 
 }  // namespace
@@ -30,7 +48,9 @@ __device__ __forceinline__ void put(E* p, const float* x) {
 // (102 MB with the distinct rows of the table), 131072 x 2048 175 us (870 MB).
 template <typename W, typename Y, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a, int lg) {
-  constexpr int AHEAD = 4;                   // loads before the first store; 131072 x 2048 fp32 to bf16 184 -> 175 us
+  // loads before the first store: 131072 x 2048 from fp32 to bf16 184 us one at a
+  // time, 181 two, 175 four; bf16 189 us four, 186 two
+  constexpr int AHEAD = sizeof(W) * VEC > 16 ? 4 : 2;
   const long long n = ((long long)blockIdx.x * 256 + threadIdx.x) >> lg;
   if (n >= a.N) return;
   const long long v = a.ids[n];
@@ -531,11 +551,15 @@ template <typename W, typename Y>
 hipError_t fwd(const EmbedArgs& a, hipStream_t st) {
   if (a.N == 0) return hipSuccess;
   const uintptr_t at = reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.y);
-  const int vec = a.D % 8 == 0 && at % 16 == 0 ? 8 : 1;
+  // 16 bytes a lane each way; 8 values of fp32 are two loads, which pays where they
+  // are one store (32768 x 2048 fp32 90 us with 8 values, 81.5 with 4; to bf16 59.8
+  // and 59.7, 32768 x 256 9.0 and 9.6)
+  constexpr int WIDE = sizeof(W) == 4 && sizeof(Y) == 4 ? 4 : 8;
+  const int vec = a.D % 8 == 0 && at % 16 == 0 ? WIDE : 1;
   int lg = 0;
   while (lg < 6 && (vec << lg) < a.D) ++lg;
   const dim3 grid((unsigned)(((a.N << lg) + 255) / 256));
-  if (vec == 8) hipLaunchKernelGGL((embed_fwd_kernel<W, Y, 8>), grid, dim3(256), 0, st, a, lg);
+  if (vec > 1) hipLaunchKernelGGL((embed_fwd_kernel<W, Y, WIDE>), grid, dim3(256), 0, st, a, lg);
   else hipLaunchKernelGGL((embed_fwd_kernel<W, Y, 1>), grid, dim3(256), 0, st, a, lg);
   return hipGetLastError();
 }
