@@ -321,3 +321,21 @@ def test_fp16_rows_keep_every_value(D):
     y, want = embedding(ids, w), w.flip(0)
     same = (y.view(torch.int16) == want.view(torch.int16)) | (y.isnan() & want.isnan())
     assert y.dtype == torch.float16 and same.all()
+
+
+@pytest.mark.parametrize("N", [1, 300, 9000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_module_in_training_and_not(N, dtype):
+    """The kernels where a gradient is wanted (its bound, and the same bits every
+    time), nn.Embedding elsewhere, with the same values."""
+    torch.manual_seed(2)
+    m = Embedding(300, 72, padding_idx=7).cuda().to(dtype)
+    ids, dy = torch.randint(0, 300, (N,)), torch.randn(N, 72).to(dtype)
+    y = m(ids.cuda())
+    assert torch.equal(y, F.embedding(ids.cuda(), m.weight)) and "_EmbeddingFn" in type(y.grad_fn).__name__
+    grads = [torch.autograd.grad(m(ids.cuda()), m.weight, dy.cuda())[0] for _ in range(3)]
+    check_grad(grads[0], ids, dy, 300, 1.0, 7)
+    assert all(torch.equal(grads[0], g) for g in grads)
+    with torch.no_grad():
+        assert torch.equal(m(ids.cuda()), y)
+    assert torch.equal(m.requires_grad_(False)(ids.cuda()), y)
