@@ -113,10 +113,12 @@ __device__ Run run_of(const int* cu, int S, int t0, int n, int T) {
 __device__ __forceinline__ int4 pack(const Run& r) {
   return make_int4((int)(r.start | r.end << 16), (int)r.used, r.cur, r.last);
 }
-__device__ __forceinline__ Run unpack(const int4& v) {
-  const unsigned m = __builtin_amdgcn_readfirstlane(v.x);
-  return Run{m & 0xffffu, m >> 16, (unsigned)__builtin_amdgcn_readfirstlane(v.y),
-             __builtin_amdgcn_readfirstlane(v.z), __builtin_amdgcn_readfirstlane(v.w)};
+// A wave's run, by a scalar load: it does not queue behind the tokens' loads.
+__device__ __forceinline__ Run unpack(const int4* at) {
+  typedef int I4 __attribute__((ext_vector_type(4)));
+  const I4 v = *(const __attribute__((address_space(4))) I4*)at;
+  const unsigned m = v.x;
+  return Run{m & 0xffffu, m >> 16, (unsigned)v.y, v.z, v.w};
 }
 // the sequence that token t starts: the last one with that boundary, from
 // sequence cur on
@@ -406,7 +408,7 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
   params(a, dl, bias2, nrate);
   const float first = a.h0 && !PACKED ? a.h0[(long long)b * a.D + dl] : 0.f;
   Run r{0u, 0u, 0u, 0, 0};
-  if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
+  if (PACKED && n > 0) r = unpack(sy.runs + t0 / N);
   const First c0 = FIRST;
   float P[N], H[N];
 #pragma unroll
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
   const float last = a.dfinal && !PACKED ? a.dfinal[(long long)b * a.D + dl] : 0.f;
   float h = n > 0 ? a.hs[(b * ((a.T + N - 1LL) / N) + t0 / N) * a.D + dl] : 0.f;
   Run r{0u, 0u, 0u, 0, 0};
-  if (PACKED && n > 0) r = unpack(sy.runs[t0 / N]);
+  if (PACKED && n > 0) r = unpack(sy.runs + t0 / N);
   float aa[N], bs[N], kw[N], kf[N], dy[N];
   const First c0 = held();
   float A = 1.f, C = 0.f, Ga = 0.f, sb = 0.f, sa = 0.f;
