@@ -122,13 +122,16 @@ __device__ __forceinline__ Run unpack(const int4* at) {
 }
 // the sequence that token t starts: the last one with that boundary, from
 // sequence cur on
-__device__ __forceinline__ int seq_from(const int* cu, int S, int cur, int t) {
+using Scalar = const __attribute__((address_space(4))) int;
+__device__ __forceinline__ int seq_from(const int* boundaries, int S, int cur, int t) {
+  Scalar* cu = (Scalar*)boundaries;
   if (cur < 0) cur = 0;
   while (cur + 1 <= S && cu[cur + 1] <= t) ++cur;
   return cur < S ? cur : S - 1;
 }
 // the sequence of token t, from sequence cur (behind it) down
-__device__ __forceinline__ int seq_before(const int* cu, int S, int cur, int t) {
+__device__ __forceinline__ int seq_before(const int* boundaries, int S, int cur, int t) {
+  Scalar* cu = (Scalar*)boundaries;
   while (cur > 0 && cu[cur] > t) --cur;
   return cur < S ? cur : S - 1;
 }
