@@ -186,8 +186,7 @@ class Embedding(nn.Embedding):
                  and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse)
         if (not plain or torch.compiler.is_compiling() or torch.jit.is_tracing()
                 or forward_ad._current_level >= 0
-                or torch._C._functorch.is_functorch_wrapped_tensor(w)
-                or torch._C._functorch.is_functorch_wrapped_tensor(ids)):
+                or torch._C._are_functorch_transforms_active()):
             return super().forward(ids)
         return embedding(ids, w, padding_idx=self.padding_idx)
 

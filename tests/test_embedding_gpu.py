@@ -339,3 +339,11 @@ def test_module_in_training_and_not(N, dtype):
     with torch.no_grad():
         assert torch.equal(m(ids.cuda()), y)
     assert torch.equal(m.requires_grad_(False)(ids.cuda()), y)
+
+
+def test_module_inside_a_function_transform():
+    """A transform of another input, the table closed over, is nn.Embedding's."""
+    m = Embedding(30, 8).cuda()
+    ids, h = torch.tensor([1, 5, 5], device="cuda"), torch.randn(3, 8, device="cuda")
+    got = torch.func.grad(lambda h: (m(ids) * h).sum())(h)
+    assert torch.equal(got, F.embedding(ids, m.weight))
