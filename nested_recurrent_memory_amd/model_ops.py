@@ -130,7 +130,10 @@ class _EmbeddingGradFn(torch.autograd.Function):
         if padding_idx is not None:
             ddw = ddw.clone()
             ddw[padding_idx] = 0
-        return None, _EmbeddingFn.apply(ids, ddw, scale, padding_idx, gdt), None, None, None, None
+        g = _EmbeddingFn.apply(ids, ddw, scale, padding_idx, gdt)
+        # an id outside the table, whose lookup is NaN, was in no sum
+        g = g.masked_fill(((ids < 0) | (ids >= ddw.shape[0])).unsqueeze(-1), 0)
+        return None, g, None, None, None, None
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):

@@ -347,3 +347,19 @@ def test_module_inside_a_function_transform():
     ids, h = torch.tensor([1, 5, 5], device="cuda"), torch.randn(3, 8, device="cuda")
     got = torch.func.grad(lambda h: (m(ids) * h).sum())(h)
     assert torch.equal(got, F.embedding(ids, m.weight))
+
+
+def test_gradient_of_the_gradient_outside_the_table():
+    """No gradient reaches the table from there, so none comes back, nor NaN."""
+    ids = torch.tensor([0, -1, 5, 3, 1 << 40, 3], device="cuda")
+    w = torch.zeros(5, 12, device="cuda", requires_grad=True)
+    v, t = torch.randn(6, 12, device="cuda", requires_grad=True), torch.randn(5, 12, device="cuda")
+    t.requires_grad_(True)
+    dw, = torch.autograd.grad(embedding(ids, w, scale=2.0, padding_idx=3), w, v, create_graph=True)
+    dv, = torch.autograd.grad(dw, v, t, create_graph=True)
+    want = torch.zeros(6, 12, device="cuda")
+    want[0] = 2 * t[0]
+    assert torch.equal(dv, want)
+    # and once more: linear in t
+    dt, = torch.autograd.grad(dv, t, torch.ones_like(dv))
+    assert torch.equal(dt, torch.tensor([2.0, 0, 0, 0, 0], device="cuda")[:, None].expand(5, 12))
