@@ -175,7 +175,8 @@ class Embedding(nn.Embedding):
     card and with 2 us less host work; so is one with max_norm,
     scale_grad_by_freq or sparse, off the GPU, in other types than bfloat16 and
     float32, beyond the kernels' sizes, of tensor subclasses and under functorch,
-    forward-mode differentiation or tracing. (nn.Embedding ends the process on an
+    forward-mode differentiation, tracing or any dispatch mode (a tracer sees
+    torch's operations, not the kernels). (nn.Embedding ends the process on an
     id outside the table, where ``embedding`` gives NaN.)"""
 
     def forward(self, ids):
@@ -188,7 +189,7 @@ class Embedding(nn.Embedding):
                  and ids.numel() <= min(_EMBED_MOST, _EMBED_VALUES // w.shape[1])
                  and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse)
         if (not plain or torch.compiler.is_compiling() or torch.jit.is_tracing()
-                or forward_ad._current_level >= 0
+                or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
                 or torch._C._are_functorch_transforms_active()):
             return super().forward(ids)
         return embedding(ids, w, padding_idx=self.padding_idx)

@@ -363,3 +363,24 @@ def test_gradient_of_the_gradient_outside_the_table():
     # and once more: linear in t
     dt, = torch.autograd.grad(dv, t, torch.ones_like(dv))
     assert torch.equal(dt, torch.tensor([2.0, 0, 0, 0, 0], device="cuda")[:, None].expand(5, 12))
+
+
+def test_module_under_a_tracer_is_nn_embedding():
+    """A trace of a training pass computes with its own inputs when it is run."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    m = Embedding(30, 8).cuda()
+
+    def work(w, ids, dy):
+        y = torch.func.functional_call(m, {"weight": w}, ids)
+        return y, torch.autograd.grad(y, w, dy)[0]
+
+    def inputs(seed):
+        g = torch.Generator().manual_seed(seed)
+        return (torch.randn(30, 8, generator=g).cuda().requires_grad_(True),
+                torch.randint(0, 30, (20,), generator=g).cuda(), torch.randn(20, 8, generator=g).cuda())
+
+    traced = make_fx(work)(*inputs(1))
+    w, ids, dy = inputs(2)
+    y, dw = traced(w, ids, dy)
+    assert torch.equal(y, F.embedding(ids, w))
+    check_grad(dw, ids.cpu(), dy.cpu(), 30, 1.0)
