@@ -178,8 +178,9 @@ def on_device(t, name, *args):
             call(name, *args, _raw_stream(i))
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# a torch built without a GPU has neither (and no tensor that reaches them)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def ptr_of_stream(st):
