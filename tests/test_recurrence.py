@@ -209,16 +209,15 @@ def test_states_of_other_types_are_refused():
 
 def test_import_without_torchs_gpu_names():
     """A torch built without a GPU has none of the names that read its streams:
-    the package (schedules, configurations, the modules on the CPU) imports."""
+    the package (schedules, the layer's configuration, modules on the CPU) imports."""
     import os
     import subprocess
     import sys
     code = ("import torch\n"
             "del torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice\n"
-            "from nested_recurrent_memory_amd import n_firings\n"
-            "from nested_recurrent_memory_amd.model import NestedGDN2Config\n"
+            "from nested_recurrent_memory_amd import NestedGDN2LayerConfig, n_firings\n"
             "from nested_recurrent_memory_amd.model_ops import Embedding\n"
-            "NestedGDN2Config()\n"
+            "NestedGDN2LayerConfig()\n"
             "assert Embedding(3, 2)(torch.tensor([1])).shape == (1, 2)\n")
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
