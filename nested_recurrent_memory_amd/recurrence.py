@@ -228,12 +228,16 @@ def step_gated_recurrence(x, f, wz, A_log, dt_bias, state, *, inplace=False):
     """One token of B sequences: x, f, wz [B,D], state [B,D]. Returns (y [B,D]
     in x's dtype, the new state [B,D] fp32). The state passed in is not
     modified, or with ``inplace=True`` (fp32, contiguous) updated and
-    returned, which keeps the buffer fixed for graph capture. Forward only."""
+    returned, which keeps the buffer fixed for graph capture. Forward only: inputs
+    that want a gradient or carry a forward-mode tangent are refused."""
     name = "step_gated_recurrence"
     _check(name, x, f, wz, A_log, dt_bias, state, 2)
     B, D = x.shape
     if tuple(state.shape) != (B, D):
         raise ValueError(f"{name}: state {tuple(state.shape)}, expected {(B, D)}")
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(t).tangent is not None for t in (x, f, wz, A_log, dt_bias, state)):
+        raise RuntimeError(f"{name} is forward-only (decoding): no tangent goes through it")
     _on_gpu(name, x, f, wz, A_log, dt_bias, state)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (x, f, wz, A_log, dt_bias, state)):
         raise RuntimeError(f"{name} is forward-only (decoding); call it under torch.no_grad() or on "

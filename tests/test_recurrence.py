@@ -222,3 +222,21 @@ def test_import_without_torchs_gpu_names():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
+
+
+def test_step_refuses_forward_mode():
+    """Forward-mode tangents have no way through the step: refused, not dropped.
+    A dual level without tangents changes nothing."""
+    from torch.autograd import forward_ad
+    x, A, h = torch.zeros(1, 4), torch.zeros(2), torch.zeros(1, 4)
+    args = [x, x, x, A, h[0], h]
+    with forward_ad.dual_level():
+        for i in range(6):
+            a = list(args)
+            a[i] = forward_ad.make_dual(a[i], torch.ones_like(a[i]))
+            with pytest.raises(RuntimeError, match="forward-only"):
+                step_gated_recurrence(*a)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-only"):
+                step_gated_recurrence(*a)
+        with pytest.raises(ValueError, match="no CPU path"):
+            step_gated_recurrence(*args)
