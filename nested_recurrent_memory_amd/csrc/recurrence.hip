@@ -75,6 +75,14 @@ __device__ __forceinline__ Decay decay(float f, float bias2, float nrate, const 
 __device__ __forceinline__ float sigmoid2(float w) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * w));
 }
+// s = sigmoid(w) and 1 - s = e^-w s, which a subtraction loses where the gate is open
+// (all of it from w = 17). e^-w is held below 2^126 there: where it is more, s may be
+// 0, and so is what 1 - s multiplies.
+__device__ __forceinline__ float sigmoid2(float w, float& rest) {
+  const float e = __builtin_amdgcn_exp2f(-LOG2E * w), s = __builtin_amdgcn_rcpf(1.f + e);
+  rest = fminf(e, 0x1p126f) * s;
+  return s;
+}
 
 // Where the tokens [t0, t0 + n) of a packed row stand: bit j of start / end /
 // used says whether token t0 + j is the first / the last of its sequence / in
@@ -546,13 +554,14 @@ __global__ __launch_bounds__(64 * W, 4) void rec_bwd_kernel(RecArgs a, Sync sy, 
     const Decay k = decay(to_f(v[0][j]), bias2, nrate, c0);
     // 1 / beta; a q of 0 (a decay that rounds to 1) is lifted so that it stays finite
     const float inv = __builtin_amdgcn_rsqf(fmaxf(k.q, 1e-37f));
-    const float xv = to_f(v[2][j]), s = sigmoid2(to_f(v[1][j])), si = s * inv;
+    float rest;
+    const float xv = to_f(v[2][j]), s = sigmoid2(to_f(v[1][j]), rest), si = s * inv;
     if (st) h = a.h0 ? a.h0[(long long)cur * a.D + dl] : 0.f;
     aa[j] = k.a;
     bs[j] = k.q * si;
     const float u = bs[j] * xv;
     const float ki = fmaf(k.a, h, -(k.a * k.a) * (si * xv));        // dg = lam ki
-    kw[j] = fmaf(-u, s, u);
+    kw[j] = u * rest;
     kf[j] = nrate * __builtin_amdgcn_exp2f(k.ls) * ki;
     dy[j] = to_f(v[3][j]);
     if (en && a.dfinal) dy[j] += a.dfinal[(long long)cur * a.D + dl];

@@ -15,7 +15,8 @@ and, for each, a bound on the fp32 error of any evaluation that
     more for exp(A_log), whose argument has u |A_log|;
   a = e^g: 2 u + |g| r_g;   1 - a: relative error 16 u r (the subtraction, from
     -g = 1/16) or r_g (the series): q = (1 - a)(1 + a): r_q = 20 u + r_g;
-  beta and 1 / beta: half of it and 3 u;  sigmoid: 4 u + 2 u |w|.
+  beta and 1 / beta: half of it and 3 u;  sigmoid: 4 u + 2 u |w|, and so is
+    1 - sigmoid(w) = sigmoid(-w), which no subtraction may form.
 """
 
 import torch
@@ -93,10 +94,10 @@ def recurrence(x, f, wz, A_log, dt_bias, h0=None, cu=None, dy=None, dfinal=None)
     bs = beta * s
     dx = lam * bs
     edx = elam * bs + (ru + 3 * U) * dx.abs()
-    k = xx * (1 - s)
+    w = wz.detach().double().cpu()
+    k = xx * torch.sigmoid(-w)
     dw = dx * k
-    # 1 - s: its error is s's, absolute
-    edw = edx * k.abs() + dx.abs() * xx.abs() * (6 + 2 * wz.double().cpu().abs().clamp(max=200)) * U
+    edw = edx * k.abs() + dw.abs() * (10 + 2 * w.abs().clamp(max=200)) * U
     safe = torch.where(beta > 0, a * a / beta, 0.0)
     p1, p2 = a * prev, safe * s * xx
     inner = p1 - p2

@@ -522,3 +522,18 @@ def test_rows_of_few_tiles(B, T, D, H, dtype):
     """Around the sizes of one, two and a few tiles, with many strips too."""
     p, dy, dfinal = make(B, T, D, H, dtype)
     run_and_check(p, dy, dfinal)
+
+
+def test_open_write_gates():
+    """Where the gate is open 1 - sigmoid(wz) is small and keeps its relative
+    precision: sigmoid(-wz), with the oracle's error of a sigmoid."""
+    p, dy, dfinal = make(1, 40, 64, 4, torch.float32)
+    p["wz"] = torch.linspace(-100, 80, 64).repeat(40, 1)[None]
+    q = gpu(p)
+    y, _ = gated_recurrence(*(q[n] for n in NAMES))
+    dx, dw = torch.autograd.grad(y, [q["x"], q["wz"]], dy.cuda())
+    v, b = oracle.recurrence(*(p[n] for n in NAMES[:5]), p["initial_state"], None, dy)["dx"]
+    k = p["x"].double() * torch.sigmoid(-p["wz"].double())
+    rel = (10 + 2 * p["wz"].double().abs()) * oracle.U
+    err = (dw.double().cpu() - v * k).abs()
+    assert (err <= b * k.abs() + rel * (v * k).abs() + 1e-37).all(), (err / (v * k).abs()).max()
