@@ -1130,7 +1130,7 @@ int32_t rec_rows(const ngdn_recurrence_args* r, const char* what) {
     return fail(NGDN_EINVAL, "%s: S*D = %lld exceeds 2^31 - 1", what, (long long)r->S * r->D);
   if (reinterpret_cast<uintptr_t>(r->ws) & 15) return fail(NGDN_EINVAL, "%s: ws must be 16-byte aligned", what);
   // the largest grid: 512 work-items for 128 tokens of 64 channels (and so a row of
-  // D is under 2^31 bytes)
+  // D is under 2^31 bytes); the sum over heads bounds its own
   const long long tiles = (r->D + 63LL) / 64 * ((r->T + 127LL) / 128) * r->B;
   if (tiles > (1LL << 23) - 1)
     return fail(NGDN_EINVAL, "%s: %lld workgroups exceed %lld (B*T*D is too large)", what, tiles,

@@ -661,40 +661,43 @@ __global__ __launch_bounds__(256) void rec_sum_runs(const float* parts, long lon
   }
 }
 
-// The last sum over n rows ([2][n][D]), a workgroup a head: dt_bias' gradient a
-// channel, A_log's the sum over the head's. Four waves have a quarter of the rows
-// of 64 channels each; a wide head has up to 16 waves, 256 channels at once (one
-// head of 2048 channels: 4000 tokens, both passes, 82 us with 4 waves, 71 with 16).
+// The last sum over n rows ([2][n][D]), a workgroup a head (several where there are
+// more than a grid can have): dt_bias' gradient a channel, A_log's the sum over the
+// head's. Four waves have a quarter of the rows of 64 channels each; a wide head has
+// up to 16 waves, 256 channels at once (one head of 2048 channels: 4000 tokens, both
+// passes, 82 us with 4 waves, 71 with 16).
 __global__ __launch_bounds__(1024) void rec_sum_heads(RecArgs a, const float* part, int n) {
   __shared__ float s[2][16][64], s_sum[4];
-  const int h = blockIdx.x, per = a.D / a.H, l = lane_id(), w = wave_id(), q = w % 4, sets = blockDim.x / (4 * WAVE);
-  float sum = 0.f;
-  for (int i0 = 0; i0 < per; i0 += 64 * sets) {
-    const int i = i0 + w / 4 * 64 + l;
-    const bool live = i < per;
-    const int d = h * per + (live ? i : 0);
-    float b = 0.f, g = 0.f;
+  const int per = a.D / a.H, l = lane_id(), w = wave_id(), q = w % 4, sets = blockDim.x / (4 * WAVE);
+  for (unsigned h = blockIdx.x; h < (unsigned)a.H; h += gridDim.x) {
+    float sum = 0.f;
+    for (int i0 = 0; i0 < per; i0 += 64 * sets) {
+      const int i = i0 + w / 4 * 64 + l;
+      const bool live = i < per;
+      const int d = (int)h * per + (live ? i : 0);
+      float b = 0.f, g = 0.f;
 #pragma unroll 8
-    for (int k = q; k < n; k += 4) {
-      b += part[(long long)k * a.D + d];
-      g += part[(long long)(n + k) * a.D + d];
+      for (int k = q; k < n; k += 4) {
+        b += part[(long long)k * a.D + d];
+        g += part[(long long)(n + k) * a.D + d];
+      }
+      __syncthreads();
+      s[0][w][l] = b;
+      s[1][w][l] = g;
+      __syncthreads();
+      if (q == 0 && live) {
+        a.ddt_bias[d] = s[0][w][l] + s[0][w + 1][l] + s[0][w + 2][l] + s[0][w + 3][l];
+        sum += s[1][w][l] + s[1][w + 1][l] + s[1][w + 2][l] + s[1][w + 3][l];
+      }
     }
-    __syncthreads();
-    s[0][w][l] = b;
-    s[1][w][l] = g;
-    __syncthreads();
-    if (q == 0 && live) {
-      a.ddt_bias[d] = s[0][w][l] + s[0][w + 1][l] + s[0][w + 2][l] + s[0][w + 3][l];
-      sum += s[1][w][l] + s[1][w + 1][l] + s[1][w + 2][l] + s[1][w + 3][l];
-    }
-  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
-  if (q == 0 && l == 0) s_sum[w / 4] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < sets; ++k) sum += s_sum[k];
-    a.dA_log[h] = sum * 0.69314718055994531f;     // g2 -> g
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
+    if (q == 0 && l == 0) s_sum[w / 4] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int k = 1; k < sets; ++k) sum += s_sum[k];
+      a.dA_log[h] = sum * 0.69314718055994531f;     // g2 -> g
+    }
   }
 }
 
@@ -788,13 +791,15 @@ hipError_t bwd(const RecArgs& a, hipStream_t st) {
   // many tiles: first slices of them, over the whole card
   const long long rows = s.nchunk * a.B;
   const unsigned wide = 4 * WAVE * (unsigned)std::min(4, (a.D / a.H + 63) / 64);
+  // a grid has under 2^32 work-items, and a decay for every channel may be 2^24 heads
+  const dim3 heads((unsigned)std::min<long long>(a.H, (1LL << 30) / wide));
   if (rows > REC_SLICES) {
     float* sums = a.ws + s.sums;
     hipLaunchKernelGGL(rec_sum_runs, dim3((a.D + 63) / 64, REC_SLICES), dim3(256), 0, st, (const float*)parts,
                        rows, a.D, REC_SLICES, sums);
-    hipLaunchKernelGGL(rec_sum_heads, dim3(a.H), dim3(wide), 0, st, a, (const float*)sums, REC_SLICES);
+    hipLaunchKernelGGL(rec_sum_heads, heads, dim3(wide), 0, st, a, (const float*)sums, REC_SLICES);
   } else {
-    hipLaunchKernelGGL(rec_sum_heads, dim3(a.H), dim3(wide), 0, st, a, (const float*)parts, (int)rows);
+    hipLaunchKernelGGL(rec_sum_heads, heads, dim3(wide), 0, st, a, (const float*)parts, (int)rows);
   }
   return hipGetLastError();
 }

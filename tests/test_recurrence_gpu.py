@@ -537,3 +537,23 @@ def test_open_write_gates():
     rel = (10 + 2 * p["wz"].double().abs()) * oracle.U
     err = (dw.double().cpu() - v * k).abs()
     assert (err <= b * k.abs() + rel * (v * k).abs() + 1e-37).all(), (err / (v * k).abs()).max()
+
+
+def test_as_many_decays_as_a_grid_has_no_room_for():
+    """2^24 heads of one channel: a workgroup each would be 2^32 work-items. Channels
+    do not meet, so every part has the bits of a call of its own."""
+    D = (1 << 24) + 5
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda: torch.randn(D, generator=g, device="cuda")  # noqa: E731
+    t = [r().view(1, 1, D) for _ in range(3)] + [r() * 0.1, r() - 3]
+
+    def grads(lo, hi):
+        q = [v[..., lo:hi].detach().requires_grad_(True) for v in t]
+        y, f = gated_recurrence(*q, output_final_state=True)
+        return [v.reshape(-1) for v in (y.detach(), *torch.autograd.grad(f.sum(), q))]
+
+    whole = grads(0, D)
+    for lo in (0, 1 << 22, (1 << 22) * 3 - 512, D - 1003):
+        for a, b in zip(whole, grads(lo, lo + 1003)):
+            assert torch.equal(a[lo:lo + 1003], b), lo
+    assert all(torch.isfinite(v).all() for v in whole)
