@@ -384,3 +384,23 @@ def test_module_under_a_tracer_is_nn_embedding():
     y, dw = traced(w, ids, dy)
     assert torch.equal(y, F.embedding(ids, w))
     check_grad(dw, ids.cpu(), dy.cpu(), 30, 1.0)
+
+
+# ---------------------------------------------------------------- sums without a rounding
+
+@pytest.mark.parametrize("N,V,D", [(20000, 5, 9), (70000, 500, 8),             # segments of 16 and 32
+                                   (262149, 3000, 8), (262149, 3000, 13),      # of 64
+                                   (8000, (1 << 18) + 3, 8), (9000, (1 << 18) + 3, 8)])   # three digits of the sort
+@pytest.mark.parametrize("hot", [0.0, 0.5, 1.0])
+def test_sums_are_whole(N, V, D, hot):
+    """Whole numbers below 2^24 in sum, exact in fp32 in any order: every row of
+    dy is in the sum of its id once, an id of thousands of segments too."""
+    g = torch.Generator().manual_seed(N + D)
+    p = 1.0 / torch.arange(1, V + 1)
+    ids = torch.multinomial(p, N, replacement=True, generator=g)
+    ids[torch.randperm(N, generator=g)[:int(N * hot)]] = V // 2
+    ids, dy = ids.cuda(), torch.randint(-8, 9, (N, D), generator=g).float().cuda()
+    w = torch.zeros(V, D, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(embedding(ids, w), w, dy)
+    want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, ids, dy.double())
+    assert torch.equal(dw.double(), want)

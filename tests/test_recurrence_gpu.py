@@ -557,3 +557,28 @@ def test_as_many_decays_as_a_grid_has_no_room_for():
         for a, b in zip(whole, grads(lo, lo + 1003)):
             assert torch.equal(a[lo:lo + 1003], b), lo
     assert all(torch.isfinite(v).all() for v in whole)
+
+
+@pytest.mark.parametrize("B,T,D,H", [(5, 513, 3333, 1), (4, 512, 4095, 5), (1, 40, 200, 2)])
+def test_a_wide_heads_decay_gradient_is_its_channels(B, T, D, H):
+    """dA_log of a head against the float64 sum of the same channels' as heads of
+    their own, which are the same bits up to that sum: at most D / (64 H) + 16
+    fp32 roundings in a row."""
+    p, dy, dfinal = make(B, T, D, H, torch.bfloat16)
+
+    def grad(A_log):
+        q = gpu(dict(p, A_log=A_log))
+        y, f = gated_recurrence(*(q[n] for n in NAMES), output_final_state=True)
+        return torch.autograd.grad([y, f], q["A_log"], [dy.cuda(), dfinal.cuda()])[0].double().view(H, -1)
+
+    got, each = grad(p["A_log"])[:, 0], grad(p["A_log"].repeat_interleave(D // H))
+    assert ((got - each.sum(1)).abs() <= (D / (64 * H) + 16) * oracle.U * each.abs().sum(1)).all()
+
+
+def test_thousands_of_packed_sequences():
+    """More boundaries than the first launch keeps in shared memory, some together."""
+    T, S = 9000, 5000
+    g = torch.Generator().manual_seed(5)
+    cu = torch.sort(torch.randint(3, T - 10, (S + 1,), generator=g)).values
+    p, dy, dfinal = make(1, T, 6, 2, torch.float32, rows=S)
+    run_and_check(p, dy, dfinal, cu=cu.tolist())
