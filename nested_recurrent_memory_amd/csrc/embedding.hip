@@ -99,7 +99,7 @@ struct SortArgs {
   const long long* ids;
   int* key[2];            // sorted ids and their positions; a pass reads one and writes the other
   int* pos[2];
-  int* table;             // [nblock][BUCKETS] counts of a pass
+  int* table;             // [nblock][BUCKETS] counts of a pass (embed_offsets: their sums, and a row of totals)
   int* owners;            // count of runs that cross segments, then their segments
   uint4* dw;              // cleared: [w0, w1), by the workgroups that do not sort
   long long w0, w1;
@@ -254,6 +254,36 @@ __global__ __launch_bounds__(ST) void embed_count(SortArgs s) {
   if (threadIdx.x < BUCKETS) s.table[blockIdx.x * BUCKETS + threadIdx.x] = s_count[threadIdx.x];
 }
 
+// Above MANY blocks the counts are summed once, not by every block again, which grows
+// with their square: 64 columns of the table a workgroup, each of its waves a stretch of
+// the blocks. The gradient of 2^18 ids into 32000 x 16: 116 us, 119 with this launch;
+// 2^19 179 and 177, 2^20 305 and 286, 2^24 5127 and 1867.
+constexpr int MANY = 128;
+__global__ __launch_bounds__(ST) void embed_offsets(SortArgs s) {
+  __shared__ int s_sum[SW][WAVE];
+  const int w = wave_id(), l = lane_id(), per = (s.nblock + SW - 1) / SW, b0 = w * per;
+  const int b1 = b0 + per < s.nblock ? b0 + per : s.nblock;
+  int* t = s.table + blockIdx.x * WAVE + l;
+  int sum = 0;
+#pragma unroll 16
+  for (int b = b0; b < b1; ++b) sum += t[b * BUCKETS];
+  s_sum[w][l] = sum;
+  __syncthreads();
+  int at = 0;
+  for (int k = 0; k < w; ++k) at += s_sum[k][l];
+  for (int b = b0; b < b1; b += 16) {
+    int c[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) c[u] = b + u < b1 ? t[(b + u) * BUCKETS] : 0;
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      if (b + u < b1) t[(b + u) * BUCKETS] = at;
+      at += c[u];
+    }
+  }
+  if (w == SW - 1) t[s.nblock * BUCKETS] = at;
+}
+
 // One pass over blocks: every id to its place.
 __global__ __launch_bounds__(ST) void embed_scatter(SortArgs s) {
   __shared__ int s_count[SW][BUCKETS], s_total[BUCKETS], s_part[SW];
@@ -270,7 +300,12 @@ __global__ __launch_bounds__(ST) void embed_scatter(SortArgs s) {
     pos[r] = s.shift == 0 || i >= s.N ? i : s.pos[0][i];
   }
   int all = 0, before = 0;
-  if (threadIdx.x < BUCKETS) {
+  if (s.nblock > MANY) {
+    if (threadIdx.x < BUCKETS) {
+      all = s.table[s.nblock * BUCKETS + threadIdx.x];
+      before = s.table[blockIdx.x * BUCKETS + threadIdx.x];
+    }
+  } else if (threadIdx.x < BUCKETS) {
     // 16 loads ahead of their additions: one at a time, beside the clearing, a
     // table of 32 blocks took 50 us to add
     for (int b = 0; b < s.nblock; b += 16) {
@@ -541,7 +576,7 @@ Space space(long long N, long long V, long long D) {
   s.key1 = s.pos0 + up4(N);
   s.pos1 = s.key1 + (N > ONE ? up4(N) : 0);
   s.table = s.pos1 + (N > ONE ? up4(N) : 0);
-  s.owners = s.table + (N > ONE ? (long long)s.nblock * BUCKETS : 0);
+  s.owners = s.table + (N > ONE ? (s.nblock + 1LL) * BUCKETS : 0);
   s.parts = s.owners + up4(s.nseg + 1);
   s.all = s.parts + (s.nseg > 1 ? 2LL * s.nseg * D : 0);
   return s;
@@ -631,6 +666,7 @@ hipError_t bwd(const EmbedArgs& a, hipStream_t st) {
       r.shift = p / 2 * r.bits;
       if (p % 2 == 0) {
         hipLaunchKernelGGL(embed_count, dim3(s.nblock + clears), dim3(ST), 0, st, r);
+        if (s.nblock > MANY) hipLaunchKernelGGL(embed_offsets, dim3(BUCKETS / WAVE), dim3(ST), 0, st, r);
       } else {
         hipLaunchKernelGGL(embed_scatter, dim3(s.nblock + clears), dim3(ST), 0, st, r);
         std::swap(r.key[0], r.key[1]);

@@ -399,8 +399,21 @@ def test_sums_are_whole(N, V, D, hot):
     p = 1.0 / torch.arange(1, V + 1)
     ids = torch.multinomial(p, N, replacement=True, generator=g)
     ids[torch.randperm(N, generator=g)[:int(N * hot)]] = V // 2
-    ids, dy = ids.cuda(), torch.randint(-8, 9, (N, D), generator=g).float().cuda()
+    dy = torch.randint(-8, 9, (N, D), generator=g).float()
     w = torch.zeros(V, D, device="cuda", requires_grad=True)
-    dw, = torch.autograd.grad(embedding(ids, w), w, dy)
-    want = torch.zeros(V, D, dtype=torch.float64, device="cuda").index_add_(0, ids, dy.double())
-    assert torch.equal(dw.double(), want)
+    dw, = torch.autograd.grad(embedding(ids.cuda(), w), w, dy.cuda())
+    assert torch.equal(dw.cpu(), torch.zeros(V, D).index_add_(0, ids, dy))
+
+
+@pytest.mark.parametrize("N,V,D", [(528385, 40000, 3), ((1 << 22) + 7, 70001, 2), (1 << 24, 300, 1)])
+def test_sums_of_millions_of_tokens(N, V, D):
+    """More blocks of ids than are counted again by each: whole numbers, exact."""
+    g = torch.Generator(device="cuda").manual_seed(N)
+    ids = torch.randint(-1, V + 1, (N,), generator=g, device="cuda")
+    ids[::3] = V // 3
+    dy = torch.randint(-2, 3, (N, D), generator=g, device="cuda").float()
+    w = torch.zeros(V, D, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(embedding(ids, w, padding_idx=1), w, dy)
+    ok = (ids >= 0) & (ids < V) & (ids != 1)
+    want = torch.zeros(V, D).index_add_(0, ids[ok].cpu(), dy[ok].cpu())
+    assert torch.equal(dw.cpu(), want)
