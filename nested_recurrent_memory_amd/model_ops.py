@@ -59,6 +59,7 @@ def _compute_dtype(x):
 
 # ---------------------------------------------------------------- embedding
 
+_functorch = torch._C._functorch
 _EMBED = (torch.bfloat16, torch.float32)                     # the kernels' types
 _TABLES = (torch.bfloat16, torch.float16, torch.float32)     # fp16 runs in fp32
 _EMBED_MOST = 1 << 24                                        # ids, and rows of the table
@@ -89,6 +90,13 @@ def _lookup(ids, weight, scale, ydt):
 
 
 def _lookup_grad(ids, dy, scale, padding_idx, V, wdt):
+    if _functorch.is_functorch_wrapped_tensor(dy) or _functorch.is_legacy_batchedtensor(dy):
+        # many gradients at once (is_grads_batched): torch's operations have a batched form
+        keep = (ids >= 0) & (ids < V)
+        if padding_idx is not None:
+            keep &= ids != padding_idx
+        g = torch.where(keep.unsqueeze(-1), dy.float(), 0.0)
+        return (torch.ops.aten.embedding_dense_backward(g, ids.clamp(0, V - 1), V, -1, False) * scale).to(wdt)
     g = _embed(dy)
     N, D = ids.numel(), dy.shape[-1]
     dw = g.new_empty((V, D), dtype=wdt if wdt in _EMBED else torch.float32)

@@ -417,3 +417,17 @@ def test_sums_of_millions_of_tokens(N, V, D):
     ok = (ids >= 0) & (ids < V) & (ids != 1)
     want = torch.zeros(V, D).index_add_(0, ids[ok].cpu(), dy[ok].cpu())
     assert torch.equal(dw.cpu(), want)
+
+
+def test_a_batch_of_gradients():
+    """is_grads_batched (a vmap over the backward), as nn.Embedding takes it."""
+    ids = torch.tensor([0, 3, -1, 3, 4, 5, 2])
+    w, dys = torch.randn(5, 12), torch.randn(3, 7, 12)
+    wg = w.cuda().requires_grad_(True)
+    y = embedding(ids.cuda(), wg, scale=2.0, padding_idx=4)
+    dw, = torch.autograd.grad(y, wg, dys.cuda(), is_grads_batched=True)
+    m = Embedding(5, 12).cuda()
+    dm, = torch.autograd.grad(m(ids.clamp(0, 4).cuda()), m.weight, dys.cuda(), is_grads_batched=True)
+    for i in range(3):
+        check_grad(dw[i], ids, dys[i], 5, 2.0, 4)
+        check_grad(dm[i], ids.clamp(0, 4), dys[i], 5, 1.0)
