@@ -124,6 +124,27 @@ def lib():
     return _lib
 
 
+_nodes = None
+
+
+def node():
+    """The autograd node in C++ (csrc/node.cpp, built beside the library).
+    Raises if it has not been built."""
+    global _nodes
+    if _nodes is None:
+        lib()
+        try:
+            from . import _node
+        except ImportError as e:
+            raise NgdnError(f"the package's _node.so cannot be loaded ({e}): build it as the library, with "
+                            "this torch") from e
+        if _node.version != VERSION:
+            raise NgdnError(f"_node.so was built for interface version {_node.version}, this package calls "
+                            f"version {VERSION}: rebuild it")
+        _nodes = _node
+    return _nodes
+
+
 # When set to a dict, every entry point call is bracketed by two timing events
 # recorded on the stream it launches on: TIMING[name] collects (start, end)
 # event pairs. SIDE collects the names launched on a side stream (their

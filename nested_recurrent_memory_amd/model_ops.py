@@ -107,8 +107,27 @@ def _lookup_grad(ids, dy, scale, padding_idx, V, wdt):
     return dw if dw.dtype == wdt else dw.to(wdt)
 
 
+def _grad(ids, dy, scale, padding_idx, V, wdt):
+    # a graph is only wanted where the gradient is differentiated again
+    f = _EmbeddingGradFn.apply if torch.is_grad_enabled() else _lookup_grad
+    return f(ids, dy, scale, padding_idx, V, wdt)
+
+
+_cpp = None
+
+
+def _node():
+    global _cpp
+    if _cpp is None:
+        n = _lib.node()
+        n.setup(_grad, _lib.NgdnError)
+        _cpp = n
+    return _cpp
+
+
 class _EmbeddingFn(torch.autograd.Function):
-    """Linear in the table: the gradient is _EmbeddingGradFn, whose own is this."""
+    """Linear in the table: the gradient is _EmbeddingGradFn, whose own is this. In C++
+    for the kernels' types (csrc/node.cpp)."""
 
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx, ydt):
@@ -119,9 +138,7 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
-        # a graph is only wanted where the gradient is differentiated again
-        grad = _EmbeddingGradFn.apply if torch.is_grad_enabled() else _lookup_grad
-        return None, grad(ids, dy, *ctx.cfg), None, None, None
+        return None, _grad(ids, dy, *ctx.cfg), None, None, None
 
 
 class _EmbeddingGradFn(torch.autograd.Function):
@@ -142,6 +159,19 @@ class _EmbeddingGradFn(torch.autograd.Function):
         # an id outside the table, whose lookup is NaN, was in no sum
         g = g.masked_fill(((ids < 0) | (ids >= ddw.shape[0])).unsqueeze(-1), 0)
         return None, g, None, None, None, None
+
+
+def _whole(ids):
+    if ids.dtype != torch.int64:
+        ids = ids.to(torch.int64)
+    return ids if ids.is_contiguous() else ids.contiguous()
+
+
+def _differentiable(ids, weight, scale, padding_idx, ydt):
+    ids = _whole(ids)
+    if weight.dtype in _EMBED and ydt in _EMBED and _lib.TIMING is None:
+        return _node().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx, ydt)
+    return _EmbeddingFn.apply(ids, weight, scale, padding_idx, ydt)
 
 
 def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
@@ -167,13 +197,9 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     if max(weight.shape) > (1 << 31) - 1:
         raise ValueError(f"embedding: weight {tuple(weight.shape)} (sizes up to 2^31 - 1)")
     _on_gpu("embedding", weight, ids)
-    if ids.dtype != torch.int64:
-        ids = ids.to(torch.int64)
-    if not ids.is_contiguous():
-        ids = ids.contiguous()
     if not (weight.requires_grad and torch.is_grad_enabled()) and forward_ad._current_level < 0:
-        return _lookup(ids, weight.detach(), float(scale), ydt)
-    return _EmbeddingFn.apply(ids, weight, float(scale), padding_idx, ydt)
+        return _lookup(_whole(ids), weight.detach(), float(scale), ydt)
+    return _differentiable(ids, weight, float(scale), padding_idx, ydt)
 
 
 class Embedding(nn.Embedding):
@@ -188,19 +214,20 @@ class Embedding(nn.Embedding):
     id outside the table, where ``embedding`` gives NaN.)"""
 
     def forward(self, ids):
-        w = self.weight
+        w, pad = self.weight, self.padding_idx
         plain = (type(ids) is torch.Tensor and type(w) in (torch.Tensor, nn.Parameter)
                  and w.requires_grad and torch.is_grad_enabled() and w.is_cuda
                  and ids.device == w.device and w.dim() == 2 and w.numel() > 0
                  and w.dtype in _EMBED and ids.dtype in (torch.int32, torch.int64)
                  and w.shape[0] < _EMBED_MOST and w.shape[1] <= _EMBED_WIDTH
                  and ids.numel() <= min(_EMBED_MOST, _EMBED_VALUES // w.shape[1])
+                 and (pad is None or 0 <= pad < w.shape[0])
                  and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse)
         if (not plain or torch.compiler.is_compiling() or torch.jit.is_tracing()
                 or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
                 or torch._C._are_functorch_transforms_active()):
             return super().forward(ids)
-        return embedding(ids, w, padding_idx=self.padding_idx)
+        return _differentiable(ids, w, 1.0, pad, w.dtype)
 
 
 # ---------------------------------------------------------------- RMSNorm

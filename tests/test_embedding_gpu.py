@@ -431,3 +431,48 @@ def test_a_batch_of_gradients():
     for i in range(3):
         check_grad(dw[i], ids, dys[i], 5, 2.0, 4)
         check_grad(dm[i], ids.clamp(0, 4), dys[i], 5, 1.0)
+
+
+def test_autograds_node():
+    """In C++, and what autograd does with any: kept graphs, graphs gone, ids changed
+    under it, saved tensors elsewhere, checkpoints, forward mode, sizes refused."""
+    from torch.autograd import forward_ad
+    from torch.utils.checkpoint import checkpoint
+    from nested_recurrent_memory_amd import _lib
+    ids, w, dy = make(40, 9, 16, torch.float32, torch.float32)
+    want, _ = oracle.embedding_grad(ids, dy, 9, 3.0, 2)
+    ids, w, dy = ids.cuda(), w.cuda().requires_grad_(True), dy.cuda()
+
+    def lookup(w):
+        return embedding(ids, w, scale=3.0, padding_idx=-7)
+
+    y = lookup(w)
+    assert type(y.grad_fn).__name__ == "_EmbeddingFnBackward"
+    assert not isinstance(y.grad_fn, torch.autograd.function.BackwardCFunction)
+    first, = torch.autograd.grad(y, w, dy, retain_graph=True)
+    check_grad(first, ids.cpu(), dy.cpu(), 9, 3.0, 2)
+    assert torch.allclose(first.double().cpu(), want, atol=1e-4)
+    assert torch.equal(torch.autograd.grad(y, w, dy)[0], first)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, w, dy)
+    y = lookup(w)
+    ids.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, w, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = lookup(w)
+    assert torch.equal(torch.autograd.grad(y, w, dy)[0], first)
+    for reentrant in (False, True):
+        y = checkpoint(lookup, w, use_reentrant=reentrant)
+        w.grad = None
+        y.backward(dy)
+        assert torch.equal(w.grad, first)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError):
+        embedding(ids, forward_ad.make_dual(w, torch.ones_like(w)))
+    one = torch.zeros(1, 1, device="cuda", requires_grad=True)
+    with pytest.raises(_lib.NgdnError, match="2\\^24"):
+        embedding(torch.zeros((1 << 24) + 1, dtype=torch.long, device="cuda"), one)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        y = lookup(w)
+        assert torch.equal(torch.autograd.grad(y, w, dy)[0], first)
+        torch.cuda.current_stream().synchronize()
