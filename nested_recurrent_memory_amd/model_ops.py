@@ -66,6 +66,10 @@ _EMBED_MOST = 1 << 24                                        # ids, and rows of 
 _EMBED_WIDTH, _EMBED_VALUES = 1 << 20, 1 << 35               # and its columns, ids times columns
 
 
+def _fits(N, V, D):
+    return 0 < V < _EMBED_MOST and 0 < D <= _EMBED_WIDTH and N <= _EMBED_MOST and N * D <= _EMBED_VALUES
+
+
 def _embed(t):
     if t.dtype not in _EMBED:
         t = t.float()
@@ -167,10 +171,12 @@ def _whole(ids):
     return ids if ids.is_contiguous() else ids.contiguous()
 
 
-def _differentiable(ids, weight, scale, padding_idx, ydt):
+def _apply(ids, weight, scale, padding_idx, ydt):
     ids = _whole(ids)
     if weight.dtype in _EMBED and ydt in _EMBED and _lib.TIMING is None:
         return _node().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx, ydt)
+    if not (weight.requires_grad and torch.is_grad_enabled()) and forward_ad._current_level < 0:
+        return _lookup(ids, weight.detach(), scale, ydt)
     return _EmbeddingFn.apply(ids, weight, scale, padding_idx, ydt)
 
 
@@ -197,37 +203,30 @@ def embedding(ids, weight, scale=1.0, padding_idx=None, out_dtype=None):
     if max(weight.shape) > (1 << 31) - 1:
         raise ValueError(f"embedding: weight {tuple(weight.shape)} (sizes up to 2^31 - 1)")
     _on_gpu("embedding", weight, ids)
-    if not (weight.requires_grad and torch.is_grad_enabled()) and forward_ad._current_level < 0:
-        return _lookup(_whole(ids), weight.detach(), float(scale), ydt)
-    return _differentiable(ids, weight, float(scale), padding_idx, ydt)
+    return _apply(ids, weight, float(scale), padding_idx, ydt)
 
 
 class Embedding(nn.Embedding):
-    """nn.Embedding whose lookup in training on the GPU and its gradient are
-    kernels of the library: sums in fp32 whatever the type, in an order that the
-    ids fix. A lookup that needs no gradient is nn.Embedding's, as fast on the
-    card and with 2 us less host work; so is one with max_norm,
-    scale_grad_by_freq or sparse, off the GPU, in other types than bfloat16 and
-    float32, beyond the kernels' sizes, of tensor subclasses and under functorch,
-    forward-mode differentiation, tracing or any dispatch mode (a tracer sees
-    torch's operations, not the kernels). (nn.Embedding ends the process on an
-    id outside the table, where ``embedding`` gives NaN.)"""
+    """nn.Embedding whose lookup on the GPU and its gradient are kernels of the
+    library: sums in fp32 whatever the type, in an order that the ids fix, and a
+    row of NaN for an id outside the table (what torch's lookup reads there
+    depends on whether its build checks). nn.Embedding's own are a call with
+    max_norm, scale_grad_by_freq or sparse, off the GPU, in other types than
+    bfloat16 and float32, beyond the kernels' sizes, of tensor subclasses and
+    under functorch, forward-mode differentiation, tracing or any dispatch mode
+    (a tracer sees torch's operations, not the kernels)."""
 
     def forward(self, ids):
         w, pad = self.weight, self.padding_idx
-        plain = (type(ids) is torch.Tensor and type(w) in (torch.Tensor, nn.Parameter)
-                 and w.requires_grad and torch.is_grad_enabled() and w.is_cuda
-                 and ids.device == w.device and w.dim() == 2 and w.numel() > 0
-                 and w.dtype in _EMBED and ids.dtype in (torch.int32, torch.int64)
-                 and w.shape[0] < _EMBED_MOST and w.shape[1] <= _EMBED_WIDTH
-                 and ids.numel() <= min(_EMBED_MOST, _EMBED_VALUES // w.shape[1])
-                 and (pad is None or 0 <= pad < w.shape[0])
-                 and self.max_norm is None and not self.scale_grad_by_freq and not self.sparse)
-        if (not plain or torch.compiler.is_compiling() or torch.jit.is_tracing()
-                or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
-                or torch._C._are_functorch_transforms_active()):
+        if (torch.compiler.is_compiling() or type(ids) is not torch.Tensor or type(w) not in (nn.Parameter, torch.Tensor) or not w.is_cuda
+                or ids.device != w.device or w.dtype not in _EMBED or ids.dtype not in (torch.int64, torch.int32)
+                or w.dim() != 2 or not _fits(ids.numel(), *w.shape)
+                or not (pad is None or 0 <= pad < w.shape[0])
+                or self.max_norm is not None or self.scale_grad_by_freq or self.sparse
+                or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
+                or torch._C._len_torch_dispatch_stack() > 0 or torch._C._are_functorch_transforms_active()):
             return super().forward(ids)
-        return _differentiable(ids, w, 1.0, pad, w.dtype)
+        return _apply(ids, w, 1.0, pad, w.dtype)
 
 
 # ---------------------------------------------------------------- RMSNorm

@@ -476,3 +476,19 @@ def test_autograds_node():
         y = lookup(w)
         assert torch.equal(torch.autograd.grad(y, w, dy)[0], first)
         torch.cuda.current_stream().synchronize()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_module_outside_the_table(dtype):
+    """The same in training and without a gradient: rows of NaN, nothing read there."""
+    m = Embedding(5, 12).cuda().to(dtype)
+    ids = torch.tensor([[0, -1, 5], [3, 1 << 40, 4]], device="cuda")
+    bad = (ids < 0) | (ids >= 5)
+    trained = m(ids)
+    with torch.no_grad():
+        y = m(ids)
+    with torch.inference_mode():
+        z = m(ids)
+    for t in (trained, y, z, m.requires_grad_(False)(ids)):
+        assert torch.isnan(t[bad]).all() and torch.equal(t[~bad], m.weight[ids[~bad]])
+    assert trained.requires_grad and not y.requires_grad and not z.requires_grad
