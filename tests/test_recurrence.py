@@ -240,3 +240,20 @@ def test_step_refuses_forward_mode():
                 step_gated_recurrence(*a)
         with pytest.raises(ValueError, match="no CPU path"):
             step_gated_recurrence(*args)
+
+
+def test_a_node_of_another_interface_is_refused(monkeypatch):
+    """The C++ node describes one interface, as the library does; without it the
+    message says what to build."""
+    import sys
+    import nested_recurrent_memory_amd as package
+    _lib.node()
+    monkeypatch.setattr(_lib, "_nodes", None)
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "VERSION", 1)
+        with pytest.raises(_lib.NgdnError, match="rebuild"):
+            _lib.node()
+    monkeypatch.delattr(package, "_node")
+    monkeypatch.setitem(sys.modules, package.__name__ + "._node", None)
+    with pytest.raises(_lib.NgdnError, match="build it"):
+        _lib.node()
