@@ -45,7 +45,8 @@ __device__ __forceinline__ void put(E* p, const float* x) {
 
 // 2^lg lanes a row (the least that hold it in one pass, at most a wave), each
 // taking VEC values at a time. Bound by HBM: 32768 x 1024 from fp32 to bf16 20 us
-// (102 MB with the distinct rows of the table), 131072 x 2048 175 us (870 MB).
+// (102 MB with the distinct rows of the table), 131072 x 2048 182 us (870 MB; 196 in a
+// training pass, behind the gradient of the one before).
 template <typename W, typename Y, int VEC>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(EmbedArgs a, int lg) {
   // loads before the first store: 131072 x 2048 from fp32 to bf16 184 us one at a

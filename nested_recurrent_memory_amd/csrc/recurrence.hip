@@ -506,7 +506,7 @@ __global__ __launch_bounds__(64 * W, 4) void rec_fwd_kernel(RecArgs a, Sync sy) 
 // ki_t g_t, needs no second array: with G_t = a_t G_(t-1) + k_t it is
 // sum dy_t G_t + c_in G_last.
 // Four values of a token and channel are read, three written: 4 x 8192 x 2048 in
-// bf16 195 us, 4.8 TB/s. Its 69 vector instructions a token are issued 3/4 of the
+// bf16 195 us, 4.8 TB/s. Its 71 vector instructions a token are issued 3/4 of the
 // time; a tenth fewer (sigmoid(z) from its logarithm, df summed as it is formed)
 // took 1 % off. A branch a token where a row or sequence may end: straight code for
 // rows of whole runs was no faster, and two copies of the loop spill.

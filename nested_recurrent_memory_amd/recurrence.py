@@ -10,8 +10,9 @@ prologue (``NestedGDN2Attention.A_log``, ``dt_bias``):
     h_t = exp(g_t) h_(t-1) + sqrt(1 - exp(2 g_t)) sigmoid(wz_t) x_t
     y_t = h_t
 
-* ``gated_recurrence``: whole sequences, forward and backward, padded batches
-  or packed sequences, a state in and out.
+* ``gated_recurrence``: whole sequences, forward and backward, rows of one
+  length (the padding of a shorter one is tokens like the others) or packed
+  sequences, a state in and out.
 * ``step_gated_recurrence``: one token, for decoding. Forward only.
 
 Inputs all in bfloat16 or all in float32 run on the kernels as they are, float16
@@ -192,8 +193,9 @@ def gated_recurrence(x, f, wz, A_log, dt_bias, initial_state=None, output_final_
     channels h D/H .. (h + 1) D/H - 1 (H = D: a decay for every channel).
     Returns (y [B,T,D] in x's dtype, the final state fp32 or None).
 
-    Without cu_seqlens every row of the batch is a sequence; initial_state and
-    the final state are [B,D]. With cu_seqlens (int tensor [S+1] on the GPU,
+    Without cu_seqlens every row of the batch is a sequence of all T tokens (one
+    padded behind its end has a final state behind the padding); initial_state
+    and the final state are [B,D]. With cu_seqlens (int tensor [S+1] on the GPU,
     0 <= cu_seqlens[0] <= ... <= cu_seqlens[S] <= T; its values are not
     checked) B is 1 and tokens cu_seqlens[s] .. cu_seqlens[s+1] - 1 are
     sequence s; the states are [S,D], and an empty sequence keeps its state.

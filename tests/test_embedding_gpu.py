@@ -449,8 +449,12 @@ def test_autograds_node():
     y = lookup(w)
     assert type(y.grad_fn).__name__ == "_EmbeddingFnBackward"
     assert not isinstance(y.grad_fn, torch.autograd.function.BackwardCFunction)
+    assert [f is not None and f.variable is w for f, _ in y.grad_fn.next_functions if f is not None] == [True]
+    seen = []
+    y.grad_fn.register_hook(lambda given, taken: seen.append(taken[0].shape))
     first, = torch.autograd.grad(y, w, dy, retain_graph=True)
     check_grad(first, ids.cpu(), dy.cpu(), 9, 3.0, 2)
+    assert seen == [dy.shape]
     assert torch.allclose(first.double().cpu(), want, atol=1e-4)
     assert torch.equal(torch.autograd.grad(y, w, dy)[0], first)
     with pytest.raises(RuntimeError, match="second time"):
