@@ -69,7 +69,7 @@ const char* ngdn_last_error(void);
  * 0.5.0 took W and U out of ngdn_l0_bwd; 0.6.0 moved the upper levels'
  * lower-state gradients from ngdn_probe_bwd's d_below to an injection that
  * ngdn_upper_scan_bwd adds. */
-#define NGDN_VERSION 1200
+#define NGDN_VERSION 1300
 int32_t ngdn_version(void);
 /* Offload architecture the library was built for ("gfx950"). */
 const char* ngdn_arch(void);
@@ -649,6 +649,79 @@ int64_t ngdn_recurrence_ws(int32_t B, int32_t T, int32_t D, int32_t backward);
 /* One token of B sequences: the state h0 [B,D] in, final_state [B,D] out (may be
  * the same array), y [B,D]; T, S, cu and the token strides are not read. */
 int32_t ngdn_recurrence_step(int32_t dtype, const ngdn_recurrence_args* r, void* stream);
+
+/* ---- Dropout, the residual norm and the sampler (no counterpart kernels in the
+ * reference, whose blocks add x + sublayer(norm(x)) without dropout,
+ * models/modeling_nested_gdn2.py:59-68, and whose tokens transformers draws). */
+
+/* y[i] = kept(i) ? keep x[i] : 0 for i < n, x and y in dtype, any alignment of
+ * their values; y may be x. kept(i): word i % 4 of the generator's block i / 4 is
+ * at least threshold, 1 <= threshold <= 2^32 (p 2^32; 2^32 drops everything). The
+ * generator: Philox4x32 with seven rounds, counter (block, offset), key seed, each
+ * two words, low word first. seed_ptr, if set, is a device int64 that takes the
+ * place of seed. The gradient is the same call on dy. */
+int32_t ngdn_dropout(int32_t dtype, int64_t n, int64_t threshold, float keep, int64_t seed,
+                     const int64_t* seed_ptr, int64_t offset, const void* x, void* y, void* stream);
+
+/* Rows of D:
+ *   z = branch rstd(branch) post_weight     (post_weight NULL: z = branch)
+ *   h = residual_scale x + branch_scale drop(gate z)
+ *   y = h rstd(h) weight                    (weight NULL: no y)
+ *   rstd(v) = 1 / sqrt(mean(v^2) + eps)
+ * in fp32, h and y each rounded once. x, h in x_dtype; branch, y, weight,
+ * post_weight and gate in their own types; types of (x, branch, y): bf16
+ * throughout, or x fp32 and the others either. The gate by gate_kind: 0 none, 1
+ * [D], 2 [rows / seq, D] (one for each seq rows, rows a multiple of seq), 3
+ * [rows], 4 [rows, D]. drop is ngdn_dropout's over the index row D + column
+ * (threshold 0: nothing is dropped). rstd_h, rstd_b [rows] fp32: what the backward
+ * reads (NULL: not written). 1 <= D <= 16384, contiguous rows, any alignment of
+ * their values.
+ * The backward takes the forward's inputs, rstd_h, rstd_b (where their norm is), dh
+ * (NULL: zeros) and dy (NULL: zeros), and writes those of dx, dbranch (in x's and
+ * branch's types), dweight, dpost_weight and dgate (in their parameters') that are
+ * not NULL. ws: ngdn_residual_norm_ws fp32, no initial contents. Sums over
+ * rows are fp32 in a fixed order: the same inputs give the same bits. */
+typedef struct ngdn_residual_args {
+  int64_t rows, seq;
+  int32_t D, gate_kind;
+  int32_t x_dtype, branch_dtype, y_dtype, w_dtype, pw_dtype, gate_dtype;
+  float residual_scale, branch_scale, eps, keep;
+  int64_t threshold, seed, offset;
+  const int64_t* seed_ptr;
+  const void *x, *branch, *weight, *post_weight, *gate;
+  void *h, *y;
+  float *rstd_h, *rstd_b;
+  const void *dh, *dy;
+  void *dx, *dbranch, *dweight, *dpost_weight, *dgate;
+  float* ws;
+} ngdn_residual_args;
+int32_t ngdn_residual_norm_fwd(const ngdn_residual_args* r, void* stream);
+int32_t ngdn_residual_norm_bwd(const ngdn_residual_args* r, void* stream);
+int64_t ngdn_residual_norm_ws(const ngdn_residual_args* r);
+
+/* A token for each row of logits [rows, V] in dtype (rows stride values apart),
+ * from u [rows] in [0, 1] (fp32, or fp64 with u_wide): with w_i = exp((l_i - max l)
+ * / temperature), kept are the top_k largest (below 1: all), of those, largest
+ * first, the ones before which less than top_p of their sum lies (1: all; the
+ * first always), of those the ones with w_i >= min_p; equal logits rank by index.
+ * The token is the first in index order with the kept weights up to and with it
+ * above u times their sum. temperature 0: the first of the largest. A row whose
+ * largest logit is not finite, that holds a NaN, or whose settings are outside
+ * their ranges (temperature finite and >= 0, top_p >= 0, 0 <= min_p <= 1) gives
+ * -1. Each setting is a scalar, or one a row where its _ptr is set (fp32; top_k
+ * int32, or int64 with top_k_wide). 1 <= V <= 2^20. The same inputs give the same
+ * token. */
+typedef struct ngdn_sample_args {
+  int64_t rows, stride;
+  int32_t V, u_wide, top_k_wide;
+  float temperature, top_p, min_p;
+  int64_t top_k;
+  const void *logits, *u;
+  const float *temperature_ptr, *top_p_ptr, *min_p_ptr;
+  const void* top_k_ptr;
+  int64_t* token;
+} ngdn_sample_args;
+int32_t ngdn_sample(int32_t dtype, const ngdn_sample_args* r, void* stream);
 
 #ifdef __cplusplus
 }

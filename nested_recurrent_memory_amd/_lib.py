@@ -20,7 +20,7 @@ NGDN_BF16 = 1
 # NGDN_VERSION of include/ngdn.h: the interface the signatures below describe.
 # The loader refuses a library of another version (working-tensor layouts and
 # argument meanings changed between versions under unchanged signatures).
-VERSION = 1200
+VERSION = 1300
 
 
 class Dims(ctypes.Structure):
@@ -90,9 +90,15 @@ SIGNATURES = {
     "ngdn_recurrence_bwd": [I32, P, P],
     "ngdn_recurrence_step": [I32, P, P],
     "ngdn_recurrence_ws": [I32, I32, I32, I32],
+    "ngdn_dropout": [I32, I64, I64, ctypes.c_float, I64, P, I64, P, P, P],
+    "ngdn_residual_norm_fwd": [P, P],
+    "ngdn_residual_norm_bwd": [P, P],
+    "ngdn_residual_norm_ws": [P],
+    "ngdn_sample": [I32, P, P],
 }
 _RESTYPES = {"ngdn_last_error": ctypes.c_char_p, "ngdn_arch": ctypes.c_char_p,
-             "ngdn_embedding_ws": ctypes.c_int64, "ngdn_recurrence_ws": ctypes.c_int64}
+             "ngdn_embedding_ws": ctypes.c_int64, "ngdn_recurrence_ws": ctypes.c_int64,
+             "ngdn_residual_norm_ws": ctypes.c_int64}
 
 _lib = None
 _fns = {}             # entry point name -> the loaded library's function

@@ -1194,4 +1194,83 @@ int32_t ngdn_recurrence_step(int32_t dtype, const ngdn_recurrence_args* r, void*
   return launched(ngdn::rec_step(*r, dtype, (hipStream_t)stream), "ngdn_recurrence_step");
 }
 
+namespace {
+
+int32_t drop_check(int64_t threshold, const char* what) {
+  if (threshold < 0 || threshold > (1LL << 32))
+    return fail(NGDN_EINVAL, "%s: threshold %lld (0 to 2^32)", what, (long long)threshold);
+  return NGDN_OK;
+}
+
+int32_t residual_check(const ngdn_residual_args* r, const char* what) {
+  if (!r) return fail(NGDN_EINVAL, "%s: args is NULL", what);
+  if (r->rows < 0 || r->D < 1 || r->D > ngdn::RESIDUAL_MOST || r->rows > (1LL << 31) - 1)
+    return fail(NGDN_EINVAL, "%s: rows=%lld D=%d (0 <= rows < 2^31, 1 <= D <= %d)", what, (long long)r->rows,
+                r->D, ngdn::RESIDUAL_MOST);
+  if (!ngdn::residual_types(r->x_dtype, r->branch_dtype, r->y_dtype))
+    return fail(NGDN_EINVAL, "%s: dtypes %d, %d, %d (bf16 throughout, or x fp32)", what, r->x_dtype,
+                r->branch_dtype, r->y_dtype);
+  for (int32_t d : {r->w_dtype, r->pw_dtype, r->gate_dtype})
+    if (d != NGDN_F32 && d != NGDN_BF16) return fail(NGDN_EINVAL, "%s: parameter dtype %d", what, d);
+  if (r->gate_kind < 0 || r->gate_kind > 4) return fail(NGDN_EINVAL, "%s: gate_kind %d", what, r->gate_kind);
+  // a workgroup for each sequence at least: work-items below 2^32
+  if (r->gate_kind == 2 && r->rows > 0 && (r->seq < 1 || r->rows % r->seq || r->rows / r->seq > (1LL << 22) - 1))
+    return fail(NGDN_EINVAL, "%s: rows=%lld seq=%lld (a multiple; fewer than 2^22 sequences)", what,
+                (long long)r->rows, (long long)r->seq);
+  if (r->rows > 0 && (!r->branch || !r->x || (r->gate_kind && !r->gate)))
+    return fail(NGDN_EINVAL, "%s: NULL tensor", what);
+  return drop_check(r->threshold, what);
+}
+
+}  // namespace
+
+int32_t ngdn_dropout(int32_t dtype, int64_t n, int64_t threshold, float keep, int64_t seed,
+                     const int64_t* seed_ptr, int64_t offset, const void* x, void* y, void* stream) {
+  g_err[0] = 0;
+  if (dtype != NGDN_F32 && dtype != NGDN_BF16) return fail(NGDN_EINVAL, "ngdn_dropout: dtype %d", dtype);
+  if (n < 0) return fail(NGDN_EINVAL, "ngdn_dropout: n=%lld", (long long)n);
+  if (int32_t e = drop_check(threshold, "ngdn_dropout")) return e;
+  if (threshold == 0) return fail(NGDN_EINVAL, "ngdn_dropout: threshold 0 (1 to 2^32)");
+  if (n > 0 && (!x || !y)) return fail(NGDN_EINVAL, "ngdn_dropout: NULL tensor");
+  ngdn::DropoutArgs a{};
+  a.x = x; a.y = y; a.n = n; a.threshold = threshold; a.seed = seed; a.offset = offset;
+  a.seed_ptr = seed_ptr; a.keep = keep;
+  return launched(ngdn::dropout(a, dtype, (hipStream_t)stream), "ngdn_dropout");
+}
+
+int64_t ngdn_residual_norm_ws(const ngdn_residual_args* r) {
+  g_err[0] = 0;
+  if (residual_check(r, "ngdn_residual_norm_ws")) return -1;
+  return ngdn::residual_ws(*r);
+}
+
+int32_t ngdn_residual_norm_fwd(const ngdn_residual_args* r, void* stream) {
+  g_err[0] = 0;
+  if (int32_t e = residual_check(r, "ngdn_residual_norm_fwd")) return e;
+  if (r->rows > 0 && (!r->h || (r->weight && !r->y))) return fail(NGDN_EINVAL, "ngdn_residual_norm_fwd: NULL tensor");
+  return launched(ngdn::residual_fwd(*r, (hipStream_t)stream), "ngdn_residual_norm_fwd");
+}
+
+int32_t ngdn_residual_norm_bwd(const ngdn_residual_args* r, void* stream) {
+  g_err[0] = 0;
+  if (int32_t e = residual_check(r, "ngdn_residual_norm_bwd")) return e;
+  if ((r->dy && !r->weight) || (r->dweight && !r->weight) || (r->dpost_weight && !r->post_weight) ||
+      (r->dgate && !r->gate_kind))
+    return fail(NGDN_EINVAL, "ngdn_residual_norm_bwd: a gradient without its parameter");
+  if (r->rows > 0 && ((r->dy && !r->rstd_h) || (r->post_weight && !r->rstd_b) || !r->ws))
+    return fail(NGDN_EINVAL, "ngdn_residual_norm_bwd: NULL tensor");
+  return launched(ngdn::residual_bwd(*r, (hipStream_t)stream), "ngdn_residual_norm_bwd");
+}
+
+int32_t ngdn_sample(int32_t dtype, const ngdn_sample_args* r, void* stream) {
+  g_err[0] = 0;
+  if (!r) return fail(NGDN_EINVAL, "ngdn_sample: args is NULL");
+  if (dtype != NGDN_F32 && dtype != NGDN_BF16) return fail(NGDN_EINVAL, "ngdn_sample: dtype %d", dtype);
+  // a workgroup of 1024 a row: work-items below 2^32
+  if (r->rows < 0 || r->rows > (1LL << 22) - 1 || r->V < 1 || r->V > (1 << 20))
+    return fail(NGDN_EINVAL, "ngdn_sample: rows=%lld V=%d (0 <= rows < 2^22, 1 <= V <= 2^20)", (long long)r->rows, r->V);
+  if (r->rows > 0 && (!r->logits || !r->u || !r->token)) return fail(NGDN_EINVAL, "ngdn_sample: NULL tensor");
+  return launched(ngdn::sample(*r, dtype, (hipStream_t)stream), "ngdn_sample");
+}
+
 }  // extern "C"

@@ -517,4 +517,22 @@ int64_t embed_ws(int64_t N, int64_t V, int64_t D);
 hipError_t embed_fwd(const EmbedArgs& a, int w_dtype, int y_dtype, hipStream_t st);
 hipError_t embed_bwd(const EmbedArgs& a, int dy_dtype, int w_dtype, hipStream_t st);
 
+// Dropout and the residual norm (residual.hip, residual_bwd.hip), the sampler
+// (sample.hip); what each field holds is in ngdn.h.
+struct DropoutArgs {
+  const void* x; void* y;
+  long long n, threshold, seed, offset;
+  const int64_t* seed_ptr;
+  float keep;
+};
+hipError_t dropout(const DropoutArgs& a, int dtype, hipStream_t st);
+using ResidualArgs = ngdn_residual_args;
+constexpr int RESIDUAL_MOST = 16384;        // columns
+bool residual_types(int xd, int rd, int yd);
+int64_t residual_ws(const ResidualArgs& a);
+hipError_t residual_fwd(const ResidualArgs& a, hipStream_t st);
+hipError_t residual_bwd(const ResidualArgs& a, hipStream_t st);
+using SampleArgs = ngdn_sample_args;
+hipError_t sample(const SampleArgs& a, int dtype, hipStream_t st);
+
 }  // namespace ngdn

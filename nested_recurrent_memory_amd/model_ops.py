@@ -15,6 +15,16 @@ points in include/ngdn.h):
 * ``Embedding``: torch's nn.Embedding with the lookup and its gradient on
   kernels (``embedding``, which also takes a scale and an output type).
 
+Beside them, without a counterpart in the reference (csrc/residual.hip,
+csrc/residual_bwd.hip, csrc/sample.hip):
+
+* ``residual_norm``: a block's output into its residual stream, with a norm after
+  the block, a gate, scales, dropout and the norm before the next block.
+* ``dropout``: from a counter-based generator, its mask formed again in the
+  backward.
+* ``sample_tokens``: a token a row of logits, by temperature, top-k, top-p and min-p
+  from given random numbers.
+
 Under autocast the GEMMs run in the autocast dtype (bfloat16), as
 nn.Linear's would; the kernels compute in fp32. There is no fallback: without
 the library, or on tensors off the GPU, the calls raise.
@@ -32,7 +42,8 @@ from . import _lib
 from .layer_ops import fanout
 
 __all__ = ["RMSNorm", "GatedMLP", "FusedLinearCrossEntropyLoss", "Embedding", "rms_norm",
-           "add_rms_norm", "swiglu", "fused_linear_cross_entropy", "embedding"]
+           "add_rms_norm", "swiglu", "fused_linear_cross_entropy", "embedding", "residual_norm",
+           "dropout", "sample_tokens"]
 
 
 def _code(t):
@@ -329,6 +340,63 @@ class RMSNorm(nn.Module):
 
     def forward(self, x):
         return rms_norm(x, self.weight, self.eps)
+
+
+# ---------------------------------------------------------------- the residual path
+
+def residual_norm(x, branch, weight=None, post_weight=None, gate=None, residual_scale=1.0, branch_scale=1.0,
+                  p=0.0, seed=0, offset=0, eps=1e-5, out_dtype=None):
+    """A block's output (``branch``) added to its residual stream ``x``, both
+    [..., D], with the norms on both sides of the sum, in one pass:
+
+        h = residual_scale x + branch_scale dropout(gate N(branch, post_weight))
+        y = N(h, weight),    N(v, w) = v / sqrt(mean(v^2) + eps) w
+
+    Returns (h, y), or h alone without ``weight``. Without ``post_weight`` the
+    branch is not normalised. ``gate`` is one value a channel [D], a token
+    [..., 1], a value (x's shape), or a channel of each sequence (x's shape with
+    ones in some of the dimensions before the last, from one of them on). ``p``, ``seed``
+    and ``offset`` are ``dropout``'s, over the values of x in row-major order.
+
+    h is in x's dtype, y in ``out_dtype`` (x's if None); bf16, fp16 and fp32, any
+    1 <= D <= 16384. y is formed from h before h is rounded (``add_rms_norm``
+    normalises the rounded sum). Differentiable once, in every tensor; sums over
+    rows are fp32 in an order that the shapes fix."""
+    return _node().residual_norm(x, branch, weight, post_weight, gate, residual_scale, branch_scale, p, seed,
+                                 offset, eps, out_dtype)
+
+
+def dropout(x, p, seed, offset=0):
+    """x with each value 0 with probability p and 1 / (1 - p) of itself otherwise;
+    x itself where p is 0 (below 2^-33). Which values are dropped is a function
+    of their row-major index, p, ``seed`` and ``offset`` alone (integers, modulo
+    2^64): value i is kept where word i % 4 of Philox4x32-7 at counter (i // 4,
+    offset) and key seed is at least p 2^32. Calls that are to drop different
+    values differ in seed or offset. ``seed`` may be an int64 tensor of one
+    element on x's GPU, which is read when the kernel runs: a captured graph
+    drops other values after it has changed. No mask is stored; a dropped value
+    is 0 whatever it was, and so is its gradient. Differentiable to any order."""
+    return _node().dropout(x, p, seed, offset)
+
+
+# ---------------------------------------------------------------- sampling
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """One token (int64) for each row of logits [..., V] from the random numbers
+    u [...] in [0, 1). With w_i = exp((l_i - max l) / temperature), kept are the
+    ``top_k`` largest (below 1: all), of those, largest first, the ones before
+    which less than ``top_p`` of their sum lies (the first always), of those the
+    ones with w_i >= ``min_p``; equal logits rank by index. The token is the
+    first in index order with the kept weights up to and with it above u times
+    their sum. A temperature of 0 takes the first of the largest logits. A row
+    that is all -inf, whose largest logit is +inf, or that holds a NaN gives -1.
+
+    logits are bf16, fp16 or fp32, rows of any stride, V up to 2^20; u fp32 or
+    fp64. Each setting is a number or a tensor of one a row on the same GPU (fp32;
+    top_k int32 or int64), of which values outside their ranges give -1. The sums
+    have no rounding: a row's token depends on nothing but its own inputs. No
+    host synchronisation: the call can be captured into a graph."""
+    return _node().sample_tokens(logits, u, temperature, top_k, top_p, min_p)
 
 
 # ---------------------------------------------------------------- SwiGLU MLP
