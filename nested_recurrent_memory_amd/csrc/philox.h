@@ -17,6 +17,10 @@ struct PhiloxKey {
       : k0((uint32_t)seed), k1((uint32_t)(seed >> 32)), c2((uint32_t)offset), c3((uint32_t)(offset >> 32)) {}
 };
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);
+}
+
 // the words of counter (block, offset)
 __device__ __forceinline__ void philox(const PhiloxKey& key, uint64_t block, uint32_t* out) {
   uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32), c2 = key.c2, c3 = key.c3;
@@ -24,8 +28,8 @@ __device__ __forceinline__ void philox(const PhiloxKey& key, uint64_t block, uin
 #pragma unroll
   for (int r = 0; r < 7; ++r) {
     const uint64_t a = (uint64_t)0xD2511F53u * c0, b = (uint64_t)0xCD9E8D57u * c2;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c0 = xor3((uint32_t)(b >> 32), c1, k0);
+    c2 = xor3((uint32_t)(a >> 32), c3, k1);
     c1 = (uint32_t)b;
     c3 = (uint32_t)a;
     k0 += 0x9E3779B9u;
@@ -45,11 +49,12 @@ __device__ __forceinline__ void philox8(const PhiloxKey& key, uint64_t i, bool a
     for (int e = 0; e < 8; ++e) w[e] = t[e];
   } else {
     philox(key, (i >> 2) + 2, t + 8);
-    const bool one = i & 1, two = i & 2;
+    // by masks: chosen by a condition, the words would become an array in memory
+    const uint32_t one = 0u - (uint32_t)(i & 1), two = 0u - (uint32_t)(i >> 1 & 1);
 #pragma unroll
-    for (int e = 0; e < 11; ++e) t[e] = one ? t[e + 1] : t[e];
+    for (int e = 0; e < 11; ++e) t[e] ^= (t[e] ^ t[e + 1]) & one;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = two ? t[e + 2] : t[e];
+    for (int e = 0; e < 8; ++e) w[e] = t[e] ^ ((t[e] ^ t[e + 2]) & two);
   }
 }
 

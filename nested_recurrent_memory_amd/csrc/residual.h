@@ -66,14 +66,50 @@ __device__ __forceinline__ void widen(const Raw8<bf16>& r, float* o) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = (float)r.a[e];
 }
-// a parameter's or gate's eight values, in either type
+// a parameter's or gate's eight values as they lie, in either type: no conversion, so a
+// load may be in flight where it is branched over
+struct RawParam { f4 a, b; };
+template <bool TINY>
+__device__ __forceinline__ void raw_param(const void* p, int dtype, long long at, const Chunk& c, RawParam& r) {
+  if (dtype == NGDN_BF16) {
+    const Raw8<bf16> t = raw8<TINY>(static_cast<const bf16*>(p) + at, c);
+    r.a = __builtin_bit_cast(f4, t.a);
+  } else {
+    const Raw8<float> t = raw8<TINY>(static_cast<const float*>(p) + at, c);
+    r.a = t.a; r.b = t.b;
+  }
+}
+__device__ __forceinline__ void widen(const RawParam& r, int dtype, float* o) {
+  if (dtype == NGDN_BF16) widen(Raw8<bf16>{__builtin_bit_cast(bf16x8, r.a)}, o);
+  else widen(Raw8<float>{r.a, r.b}, o);
+}
 template <bool TINY>
 __device__ __forceinline__ void load_param(const void* p, int dtype, long long at, const Chunk& c, float* o) {
-  if (dtype == NGDN_BF16) widen(raw8<TINY>(static_cast<const bf16*>(p) + at, c), o);
-  else widen(raw8<TINY>(static_cast<const float*>(p) + at, c), o);
+  RawParam r{};
+  raw_param<TINY>(p, dtype, at, c, r);
+  widen(r, dtype, o);
 }
 __device__ __forceinline__ float load_one(const void* p, int dtype, long long at) {
   return dtype == NGDN_BF16 ? (float)static_cast<const bf16*>(p)[at] : static_cast<const float*>(p)[at];
+}
+// post_weight and a gate of channels (its row from gate_at on) times scale, one where
+// there is none
+template <bool TINY>
+__device__ __forceinline__ void branch_factor(const ResidualArgs& a, bool sequence, long long gate_at, const Chunk& c, float scale,
+                                              float* o) {
+  float t[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = scale;
+  if (a.post_weight) {
+    load_param<TINY>(a.post_weight, a.pw_dtype, 0, c, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= t[e];
+  }
+  if (a.gate_kind == GATE_CHANNEL || (sequence && a.gate_kind == GATE_SEQUENCE)) {
+    load_param<TINY>(a.gate, a.gate_dtype, gate_at, c, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= t[e];
+  }
 }
 template <bool TINY, typename E>
 __device__ __forceinline__ void put8(E* row, const Chunk& c, const float* x) {
@@ -94,31 +130,69 @@ __device__ __forceinline__ void put8(E* row, const Chunk& c, const float* x) {
   }
 }
 
+// v of another lane of the row, by the vector unit's own lane moves (no trip through LDS)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+// the sum over a wave, in a scalar register
+__device__ __forceinline__ float wave_sum_uniform(float v) {
+  v += moved<0x111, 0xf>(v);      // row_shr 1, 2, 4, 8: the sum of 16 lanes in their last
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);      // row_bcast 15 into rows 1 and 3, row_bcast 31 into 2 and 3
+  v += moved<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), WAVE - 1));
+}
+
 // sums over a row of N values a lane, the same in each of its lanes. A row over
 // several waves goes through s [2][32], its halves in turn: a half is written again
 // only behind the next sum's barrier, so one barrier a sum is enough
 template <int G, int N>
 __device__ __forceinline__ void row_sum(float* v, int waves, float* s, int& side) {
+  if constexpr (G < WAVE) {
 #pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1)
+    for (int o = G / 2; o > 0; o >>= 1)
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] += __shfl_xor(v[j], o, WAVE);
-  if (G == WAVE && waves > 1) {
-    float* t = s + side * 32;
-    side ^= 1;
-    const int w = wave_id(), w0 = w - w % waves;
-    if (lane_id() == 0) {
+      for (int j = 0; j < N; ++j) v[j] += __shfl_xor(v[j], o, WAVE);
+  } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j) t[w * N + j] = v[j];
+    for (int j = 0; j < N; ++j) v[j] = wave_sum_uniform(v[j]);
+    if (waves > 1) {
+      float* t = s + side * 32;
+      side ^= 1;
+      const int w = wave_id(), w0 = w - w % waves;
+      if (lane_id() == 0) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) t[w * N + j] = v[j];
+      }
+      lds_barrier();
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = 0.f;
+      for (int i = 0; i < waves; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] += t[(w0 + i) * N + j];
     }
-    lds_barrier();
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = 0.f;
-    for (int i = 0; i < waves; ++i)
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[j] += t[(w0 + i) * N + j];
   }
 }
+
+// a sum over a lane's values p(e) that count. Where D is a multiple of eight (uniform)
+// a lane's count all or none
+template <bool TINY, typename F>
+__device__ __forceinline__ float lane_sum(const Chunk& c, bool eights, F p) {
+  float s = 0.f;
+  if (!TINY && eights) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += p(e);
+    return c.first == 0 ? s : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s += counts<TINY>(c, e) ? p(e) : 0.f;
+  return s;
+}
+// 1 / sqrt(mean + eps), within two units of the last place
+__device__ __forceinline__ float inverse_root(float sum, float inv, float eps) { return rsqrtf(sum * inv + eps); }
 
 // which of the values i ... i + 7 of the stream are kept: word >= threshold (1 to 2^32)
 __device__ __forceinline__ void drop8(const ResidualArgs& a, const PhiloxKey& key, uint64_t i, bool* kept) {

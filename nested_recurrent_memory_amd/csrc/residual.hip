@@ -58,95 +58,132 @@ hipError_t dropout(const DropoutArgs& a, int dtype, hipStream_t st) {
 
 // ---------------------------------------------------------------- the residual norm
 
-template <typename X, typename R, typename Y, int G, int V, bool TINY>
+// A row of G < 64 lanes, of one wave (four rows a workgroup, each wave on its own)
+// or of a workgroup. A workgroup stays and takes rows in steps of the grid, its
+// parameters in registers; the next row's values are in flight while a row is worked
+// on, in two sets of registers in turn (a copy from one into the other would wait
+// for them).
+//
+// HBM-bound: 4 x 4096 rows of 2048, fp32 stream and bf16 branch, 403 MB in 77-78 us
+// (5.2 TB/s, a copy's rate); 4 x 8192 rows of 2048, bf16, with dropout, 537 MB in 113
+// us (4.75 TB/s). A workgroup a row with its parameters loaded each time took 111 and
+// 226 us, and 12 us for 128 rows, the latencies of four loads in a row, where this takes
+// 4.5. Of the second case's 226 us the generator and the sums' arithmetic were as much as
+// the loads: xor of three in one instruction, wave sums by lane moves instead of through
+// LDS and one factor for post_weight, gate and scales took it from 157 to 113.
+template <typename X, typename R, typename Y, int G, int V, bool PRE, bool TINY>
 __global__ __launch_bounds__(1024) void residual_fwd_kernel(ResidualArgs a, int waves) {
   __shared__ float s_sum[2 * 32];
   int side = 0;
   const int lanes = G < WAVE ? G : waves * WAVE, slots = blockDim.x / lanes;
   const int slot = G < WAVE ? threadIdx.x / G : wave_id() / waves, li = threadIdx.x - slot * lanes;
   const PhiloxKey key = residual_key(a);
+  const float inv = 1.f / (float)a.D;
+  const bool eights = (a.D & 7) == 0;
+  const bool rows_gate = a.gate_kind == GATE_SEQUENCE || a.gate_kind == GATE_FULL;
   Chunk c[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) c[v] = chunk_of<TINY>(v * lanes + li, a.D);
-  const float inv = 1.f / (float)a.D;
-  for (long long r0 = (long long)blockIdx.x * slots; r0 < a.rows; r0 += (long long)gridDim.x * slots) {
-    const bool live = r0 + slot < a.rows;
-    const long long row = live ? r0 + slot : a.rows - 1, at = row * a.D;
-    Raw8<X> rx[V];
-    Raw8<R> rb[V];
-    float z[V][8], t[8];
+
+  struct Row {
+    Raw8<X> x[V];
+    Raw8<R> b[V];
+  };
+  auto fetch = [&](long long row, Row& r) __attribute__((always_inline)) {
+    const long long at = row * a.D;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      rx[v] = raw8<TINY>(static_cast<const X*>(a.x) + at, c[v]);
-      rb[v] = raw8<TINY>(static_cast<const R*>(a.branch) + at, c[v]);
+      r.b[v] = raw8<TINY>(static_cast<const R*>(a.branch) + at, c[v]);
+      r.x[v] = raw8<TINY>(static_cast<const X*>(a.x) + at, c[v]);
     }
+  };
+  const long long step = (long long)gridDim.x * slots;
+  long long row = (long long)blockIdx.x * slots + slot;
+  // the rows of a wave under 64 lanes end together
+  const long long last = a.rows - 1;
+  Row r0, r1;
+  if (G < WAVE || row <= last) fetch(row < last ? row : last, r0);
+  // pg: what a normalised value of the branch is multiplied by
+  float w[V][8], pg[V][8];
+  const float scale = a.branch_scale * (a.threshold ? a.keep : 1.f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) widen(rb[v], z[v]);
+  for (int v = 0; v < V; ++v) {
+    if (PRE) load_param<TINY>(a.weight, a.w_dtype, 0, c[v], w[v]);
+    branch_factor<TINY>(a, false, 0, c[v], scale, pg[v]);
+  }
+
+  auto work = [&](Row& r, Row& next) __attribute__((always_inline)) {
+    const bool live = row <= last;
+    const long long at = (live ? row : last) * a.D;
+    if (G < WAVE || row + step <= last) fetch(row + step < last ? row + step : last, next);
+    float z[V][8], t[8], rstd_b = 1.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) widen(r.b[v], z[v]);
     if (a.post_weight) {
       float ss = 0.f;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss += counts<TINY>(c[v], e) ? z[v][e] * z[v][e] : 0.f;
+      for (int v = 0; v < V; ++v) ss += lane_sum<TINY>(c[v], eights, [&](int e) { return z[v][e] * z[v][e]; });
       row_sum<G, 1>(&ss, waves, s_sum, side);
-      const float rstd = 1.f / sqrtf(ss * inv + a.eps);
-      if (a.rstd_b && live && li == 0) a.rstd_b[row] = rstd;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        load_param<TINY>(a.post_weight, a.pw_dtype, 0, c[v], t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[v][e] *= rstd * t[e];
-      }
+      rstd_b = inverse_root(ss, inv, a.eps);
     }
-    if (a.gate_kind == GATE_TOKEN) {
-      const float g = load_one(a.gate, a.gate_dtype, row);
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[v][e] *= g;
-    } else if (a.gate_kind != GATE_NONE) {
-      const long long ga = a.gate_kind == GATE_FULL ? at : a.gate_kind == GATE_SEQUENCE ? row / a.seq * a.D : 0;
+    if (rows_gate) {
+      const long long ga = a.gate_kind == GATE_FULL ? at : (long long)((uint32_t)(live ? row : last) / (uint32_t)a.seq) * a.D;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         load_param<TINY>(a.gate, a.gate_dtype, ga, c[v], t);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[v][e] *= t[e];
+        for (int e = 0; e < 8; ++e) z[v][e] *= rstd_b * (pg[v][e] * t[e]);
       }
+    } else {
+      const float one = a.gate_kind == GATE_TOKEN ? rstd_b * load_one(a.gate, a.gate_dtype, live ? row : last) : rstd_b;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[v][e] *= one * pg[v][e];
     }
-    float scale = a.branch_scale;
     if (a.threshold) {
-      scale *= a.keep;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         bool kept[8];
         drop8(a, key, (uint64_t)at + c[v].base, kept);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[v][e] = kept[e] ? z[v][e] * scale : 0.f;
+        for (int e = 0; e < 8; ++e) z[v][e] = kept[e] ? z[v][e] : 0.f;
       }
-      scale = 1.f;
     }
     float ss = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      widen(rx[v], t);
+      widen(r.x[v], t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        z[v][e] = a.residual_scale * t[e] + scale * z[v][e];      // h
-        ss += counts<TINY>(c[v], e) ? z[v][e] * z[v][e] : 0.f;
-      }
-      if (live) put8<TINY>(static_cast<X*>(a.h) + at, c[v], z[v]);
+      for (int e = 0; e < 8; ++e) z[v][e] += a.residual_scale * t[e];      // h
+      if (PRE) ss += lane_sum<TINY>(c[v], eights, [&](int e) { return z[v][e] * z[v][e]; });
+      if (G == WAVE || live) put8<TINY>(static_cast<X*>(a.h) + at, c[v], z[v]);
     }
-    if (a.weight) {
+    if (PRE) {
       row_sum<G, 1>(&ss, waves, s_sum, side);
-      const float rstd = 1.f / sqrtf(ss * inv + a.eps);
-      if (a.rstd_h && live && li == 0) a.rstd_h[row] = rstd;
+      const float rstd = inverse_root(ss, inv, a.eps);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        load_param<TINY>(a.weight, a.w_dtype, 0, c[v], t);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[v][e] *= rstd * t[e];
-        if (live) put8<TINY>(static_cast<Y*>(a.y) + at, c[v], z[v]);
+        for (int e = 0; e < 8; ++e) z[v][e] *= rstd * w[v][e];
+        if (G == WAVE || live) put8<TINY>(static_cast<Y*>(a.y) + at, c[v], z[v]);
       }
+      if (a.rstd_h && live && li == 0) a.rstd_h[row] = rstd;
+    }
+    if (a.rstd_b && a.post_weight && live && li == 0) a.rstd_b[row] = rstd_b;
+    row += step;
+  };
+  // lanes of a wave and waves of a row end together: rows in one step differ by less than slots
+  if constexpr (G < WAVE) {
+    for (long long first = (long long)blockIdx.x * slots; first <= last; first += 2 * step) {
+      work(r0, r1);
+      work(r1, r0);
+    }
+  } else {
+    while (row <= last) {
+      work(r0, r1);
+      if (row > last) break;
+      work(r1, r0);
     }
   }
 }
@@ -159,23 +196,31 @@ bool residual_types(int xd, int rd, int yd) {
 
 namespace {
 
-template <typename X, typename R, typename Y>
+// As many waves as run at once, four a SIMD: 12 and 20 a CU instead of 16 take 77 and
+// 86 us where 16 take 77 (fp32 stream), 139 and 143 where 16 take 126 (dropout).
+constexpr long long FWD_WAVES = 256 * 16;
+
+template <typename X, typename R, typename Y, bool PRE>
 hipError_t launch_fwd(const ResidualArgs& a, hipStream_t st) {
   const int D = a.D;
-  // work-items below 2^32; a workgroup takes further rows in steps of the grid
   auto go = [&](auto kernel, int threads, int slots, int waves) {
-    const long long want = (a.rows + slots - 1) / slots, most = 1 << 21;
+    const long long want = (a.rows + slots - 1) / slots, most = FWD_WAVES * 64 / threads;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(want < most ? want : most)), dim3(threads), 0, st, a, waves);
     return hipGetLastError();
   };
-  if (D < 8) return go(residual_fwd_kernel<X, R, Y, 8, 1, true>, 256, 32, 1);
-  if (D <= 64) return go(residual_fwd_kernel<X, R, Y, 8, 1, false>, 256, 32, 1);
-  if (D <= 128) return go(residual_fwd_kernel<X, R, Y, 16, 1, false>, 256, 16, 1);
-  if (D <= 256) return go(residual_fwd_kernel<X, R, Y, 32, 1, false>, 256, 8, 1);
+  if (D < 8) return go(residual_fwd_kernel<X, R, Y, 8, 1, PRE, true>, 256, 32, 1);
+  if (D <= 64) return go(residual_fwd_kernel<X, R, Y, 8, 1, PRE, false>, 256, 32, 1);
+  if (D <= 128) return go(residual_fwd_kernel<X, R, Y, 16, 1, PRE, false>, 256, 16, 1);
+  if (D <= 256) return go(residual_fwd_kernel<X, R, Y, 32, 1, PRE, false>, 256, 8, 1);
   const int waves = (D + 511) / 512;
-  if (waves <= 2) return go(residual_fwd_kernel<X, R, Y, 64, 1, false>, 256, 4 / waves, waves);
-  if (waves <= 16) return go(residual_fwd_kernel<X, R, Y, 64, 1, false>, waves * 64, 1, waves);
-  return go(residual_fwd_kernel<X, R, Y, 64, 2, false>, (waves + 1) / 2 * 64, 1, (waves + 1) / 2);
+  if (waves == 1) return go(residual_fwd_kernel<X, R, Y, 64, 1, PRE, false>, 256, 4, 1);
+  if (waves <= 16) return go(residual_fwd_kernel<X, R, Y, 64, 1, PRE, false>, waves * 64, 1, waves);
+  return go(residual_fwd_kernel<X, R, Y, 64, 2, PRE, false>, (waves + 1) / 2 * 64, 1, (waves + 1) / 2);
+}
+
+template <typename X, typename R, typename Y>
+hipError_t launch_fwd(const ResidualArgs& a, hipStream_t st) {
+  return a.weight ? launch_fwd<X, R, Y, true>(a, st) : launch_fwd<X, R, X, false>(a, st);
 }
 
 }  // namespace

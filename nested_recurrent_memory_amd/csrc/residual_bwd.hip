@@ -8,7 +8,9 @@
 //   dbranch = rstd_b (dz post_weight - bn mean(dz post_weight bn))
 //
 // z and h are formed again from branch and x with the forward's statistics, the
-// mask from its counter. Sums over rows are kept in registers by a workgroup for
+// mask from its counter. With q the kept part of dH (times the gate where it is a
+// token's or a value's) the sums over rows of post_weight and of a gate of channels
+// are one: sum q bn, times branch_scale and the other parameter. Sums over rows are kept in registers by a workgroup for
 // the rows that it takes, written once as its partial row, and added in a second
 // launch in the order of the workgroups: the same inputs give the same bits.
 #include "residual.h"
@@ -17,14 +19,18 @@ namespace ngdn {
 
 namespace {
 
-// Workgroups of a pass: for sums over rows, few partial rows; each group (the
-// rows that share a gate of a sequence; one group else) has its own.
+// Workgroups of a pass: each leaves one partial row of every sum over rows; each group
+// (the rows that share a gate of a sequence; one group else) has its own.
 struct Plan {
   int lanes, threads, slots, waves, V;
   long long groups, per, blocks;     // rows of a group, workgroups a group
 };
 
-constexpr long long BWD_BLOCKS = 1024;
+// As many waves as run at once, three a SIMD at the registers that a row takes: more
+// would leave more partial rows. Two rows a slot at least, which halves those of a
+// small batch.
+constexpr long long BWD_WAVES = 256 * 12;
+constexpr int BWD_ROWS = 2;
 
 Plan plan_bwd(const ResidualArgs& a) {
   Plan p;
@@ -35,15 +41,15 @@ Plan plan_bwd(const ResidualArgs& a) {
     p.threads = 256; p.waves = 1;
   } else {
     p.waves = (D + 511) / 512;
-    if (p.waves > 16) { p.V = 2; p.waves = (p.waves + 1) / 2; }
+    if (p.waves > 8) { p.V = 2; p.waves = (p.waves + 1) / 2; }
     p.lanes = p.waves * 64;
-    p.threads = p.waves <= 2 ? 256 : p.lanes;
+    p.threads = p.waves == 1 ? 256 : p.lanes;
   }
   p.slots = p.threads / p.lanes;
   p.groups = a.gate_kind != GATE_SEQUENCE ? 1 : a.rows > 0 ? a.rows / a.seq : 0;
   p.per = a.gate_kind == GATE_SEQUENCE ? a.seq : a.rows;
-  const long long want = (p.per + p.slots - 1) / p.slots;
-  const long long most = p.groups > 0 && BWD_BLOCKS / p.groups > 1 ? BWD_BLOCKS / p.groups : 1;
+  const long long want = (p.per + p.slots * BWD_ROWS - 1) / (p.slots * BWD_ROWS), all = BWD_WAVES * 64 / p.threads;
+  const long long most = p.groups > 0 && all / p.groups > 1 ? all / p.groups : 1;
   p.blocks = want < most ? want : most;
   return p;
 }
@@ -56,9 +62,19 @@ int64_t residual_ws(const ResidualArgs& a) {
   return 3 * p.groups * p.blocks * a.D;
 }
 
-template <typename X, typename R, typename Y, int G, int V, bool TINY>
-__global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a, int waves, long long per,
-                                                            long long blocks) {
+// A row's layout is the forward's. A workgroup stays, its parameters and its sums over
+// rows in registers.
+// USUAL: both outputs have a gradient and both inputs want one, so no load or store
+// lies under a branch (behind one the compiler waits for every store before it).
+//
+// HBM-bound: 4 x 8192 rows of 2048, bf16, a gate a channel and dropout move 805 MB (x
+// and branch read again, dh, dy, dx, dbranch) in 167-171 us, 4.8 TB/s of the 4.9-5.2
+// that a copy reaches; the sum over partial rows takes 5. Of the arithmetic, 42 full-rate
+// operations a value (17 of them the generator's), one sum for post_weight and gate
+// instead of two took the pass from 181 to 170 us. The next row's values in flight in a
+// second set of registers, as in the forward, changed nothing (167).
+template <typename X, typename R, typename Y, int G, int V, int TH, bool USUAL, bool TINY>
+__global__ __launch_bounds__(TH) void residual_bwd_kernel(ResidualArgs a, int waves, long long per, long long blocks) {
   extern __shared__ float s_row[];          // [slots][D]
   __shared__ float s_sum[2 * 32];
   int side = 0;
@@ -66,26 +82,28 @@ __global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a, int 
   const int slot = G < WAVE ? threadIdx.x / G : wave_id() / waves, li = threadIdx.x - slot * lanes;
   const PhiloxKey key = residual_key(a);
   const float inv = 1.f / (float)a.D;
+  const bool eights = (a.D & 7) == 0;
   const bool cols = a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SEQUENCE;
+  const bool norm = USUAL || (a.weight && a.dy), has_dh = USUAL || a.dh;
+  const float scale = a.branch_scale * (a.threshold ? a.keep : 1.f);
   // the group's rows, from its block-th run of slots in steps of its workgroups
   const long long group = blockIdx.x / blocks, block = blockIdx.x - group * blocks;
-  const long long g0 = group * per, g1 = g0 + per < a.rows ? g0 + per : a.rows;
+  const long long g0 = group * per, last = (g0 + per < a.rows ? g0 + per : a.rows) - 1;
+  const long long step = blocks * slots;
   Chunk c[V];
-  float sw[V][8], sp[V][8], sg[V][8];
+  float sw[V][8], sb[V][8], w[V][8], pg[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     c[v] = chunk_of<TINY>(v * lanes + li, a.D);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sw[v][e] = sp[v][e] = sg[v][e] = 0.f;
+    for (int e = 0; e < 8; ++e) sw[v][e] = sb[v][e] = 0.f;
   }
-  for (long long r0 = g0 + block * slots; r0 < g1; r0 += blocks * slots) {
-    const bool live = r0 + slot < g1;
-    const long long row = live ? r0 + slot : g1 - 1, at = row * a.D;
+
+  auto work = [&](long long row, bool live) __attribute__((always_inline)) {
+    const long long at = row * a.D;
     Raw8<X> rx[V], rh[V];
     Raw8<R> rb[V];
     Raw8<Y> ry[V];
-    float z[V][8], u[V][8], d[V][8], t[8];
-    const bool norm = a.weight != nullptr && a.dy != nullptr;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       rb[v] = raw8<TINY>(static_cast<const R*>(a.branch) + at, c[v]);
@@ -93,62 +111,50 @@ __global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a, int 
         rx[v] = raw8<TINY>(static_cast<const X*>(a.x) + at, c[v]);
         ry[v] = raw8<TINY>(static_cast<const Y*>(a.dy) + at, c[v]);
       }
-      if (a.dh) rh[v] = raw8<TINY>(static_cast<const X*>(a.dh) + at, c[v]);
+      if (has_dh) rh[v] = raw8<TINY>(static_cast<const X*>(a.dh) + at, c[v]);
     }
-    const float rstd_b = a.post_weight ? a.rstd_b[row] : 1.f;
-    const float one = a.gate_kind == GATE_TOKEN ? load_one(a.gate, a.gate_dtype, row) : 1.f;
-    const long long ga = a.gate_kind == GATE_FULL ? at : a.gate_kind == GATE_SEQUENCE ? group * a.D : 0;
-    const bool wide = a.gate_kind != GATE_NONE && a.gate_kind != GATE_TOKEN;
-    unsigned kept[V];
+    const float rstd_h = norm ? a.rstd_h[row] : 0.f, rstd_b = a.post_weight ? a.rstd_b[row] : 1.f;
+    const bool full = a.gate_kind == GATE_FULL, token = a.gate_kind == GATE_TOKEN;
+    const float one = token ? load_one(a.gate, a.gate_dtype, row) : 1.f;
+    // bn; hn, then what dz is of the kept dH; dH, then dz post_weight
+    float b[V][8], u[V][8], d[V][8], t[8];
+    bool kept[V][8];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      kept[v] = 0xff;
-      if (a.threshold) {
-        bool k[8];
-        drop8(a, key, (uint64_t)at + c[v].base, k);
-        kept[v] = 0;
+      widen(rb[v], b[v]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) kept[v] |= (unsigned)k[e] << e;
-      }
-    }
-    const float scale = a.branch_scale * (a.threshold ? a.keep : 1.f);
-    // z, and the sum over the row for the norm of h
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      widen(rb[v], z[v]);
-      if (a.post_weight) {
-        load_param<TINY>(a.post_weight, a.pw_dtype, 0, c[v], t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[v][e] *= rstd_b * t[e];
-      }
+      for (int e = 0; e < 8; ++e) { b[v][e] *= rstd_b; kept[v][e] = true; }
+      if (a.threshold) drop8(a, key, (uint64_t)at + c[v].base, kept[v]);
     }
     if (norm) {
-      const float rstd = a.rstd_h[row];
       float dot = 0.f;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        float g[8], x[8], dy[8];
+        float x[8];
+        if (full) {
+          load_param<TINY>(a.gate, a.gate_dtype, at, c[v], t);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = one;
-        if (wide) load_param<TINY>(a.gate, a.gate_dtype, ga, c[v], g);
+          for (int e = 0; e < 8; ++e) u[v][e] = b[v][e] * (pg[v][e] * t[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) u[v][e] = b[v][e] * (one * pg[v][e]);
+        }
         widen(rx[v], x);
-        widen(ry[v], dy);
-        load_param<TINY>(a.weight, a.w_dtype, 0, c[v], t);
+        widen(ry[v], t);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float b = kept[v] >> e & 1 ? z[v][e] * g[e] * scale : 0.f;
-          u[v][e] = (a.residual_scale * x[e] + b) * rstd;          // hn
-          if (live) sw[v][e] += dy[e] * u[v][e];
-          d[v][e] = dy[e] * t[e];
-          dot += counts<TINY>(c[v], e) ? d[v][e] * u[v][e] : 0.f;
+          u[v][e] = (a.residual_scale * x[e] + (kept[v][e] ? u[v][e] : 0.f)) * rstd_h;
+          if (G == WAVE || live) sw[v][e] += t[e] * u[v][e];
+          d[v][e] = t[e] * w[v][e];
         }
+        dot += lane_sum<TINY>(c[v], eights, [&](int e) { return d[v][e] * u[v][e]; });
       }
       row_sum<G, 1>(&dot, waves, s_sum, side);
       dot *= inv;
 #pragma unroll
       for (int v = 0; v < V; ++v)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[v][e] = rstd * (d[v][e] - u[v][e] * dot);
+        for (int e = 0; e < 8; ++e) d[v][e] = rstd_h * (d[v][e] - u[v][e] * dot);
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v)
@@ -158,83 +164,117 @@ __global__ __launch_bounds__(1024) void residual_bwd_kernel(ResidualArgs a, int 
     float sums[2] = {0.f, 0.f};       // dz post_weight bn, and the token gate's
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float g[8];
-      if (a.dh) {
+      if (has_dh) {
         widen(rh[v], t);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[v][e] += t[e];               // dH
+        for (int e = 0; e < 8; ++e) d[v][e] += t[e];
       }
-      if (a.dx && live) {
+      if ((USUAL || a.dx) && (G == WAVE || live)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[e] = a.residual_scale * d[v][e];
         put8<TINY>(static_cast<X*>(a.dx) + at, c[v], t);
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = one;
-      if (wide) load_param<TINY>(a.gate, a.gate_dtype, ga, c[v], g);
+      for (int e = 0; e < 8; ++e) d[v][e] = kept[v][e] ? d[v][e] : 0.f;
+      if (full) {
+        float g[8];
+        load_param<TINY>(a.gate, a.gate_dtype, at, c[v], g);
+        if (a.dgate && (G == WAVE || live)) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) t[e] = d[v][e] * (b[v][e] * pg[v][e]);
+          if (a.gate_dtype == NGDN_BF16) put8<TINY>(static_cast<bf16*>(a.dgate) + at, c[v], t);
+          else put8<TINY>(static_cast<float*>(a.dgate) + at, c[v], t);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[v][e] *= g[e];
+      } else if (token) {
+        sums[1] += lane_sum<TINY>(c[v], eights, [&](int e) { return d[v][e] * (b[v][e] * pg[v][e]); });
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[v][e] *= one;
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        d[v][e] = kept[v] >> e & 1 ? d[v][e] * scale : 0.f;        // du
-        z[v][e] *= d[v][e];                                        // du z
-        d[v][e] *= g[e];                                           // dz
-        if (counts<TINY>(c[v], e)) sums[1] += z[v][e];
+        if (G == WAVE || live) sb[v][e] += d[v][e] * b[v][e];
+        d[v][e] *= pg[v][e];
       }
-      if (a.gate_kind == GATE_FULL && a.dgate && live) {
-        if (a.gate_dtype == NGDN_BF16) put8<TINY>(static_cast<bf16*>(a.dgate) + at, c[v], z[v]);
-        else put8<TINY>(static_cast<float*>(a.dgate) + at, c[v], z[v]);
-      }
-      if (cols && live) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sg[v][e] += z[v][e];
-      }
-      if (a.post_weight) {
-        widen(rb[v], u[v]);
-        load_param<TINY>(a.post_weight, a.pw_dtype, 0, c[v], t);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          u[v][e] *= rstd_b;                                       // bn
-          if (live) sp[v][e] += d[v][e] * u[v][e];
-          d[v][e] *= t[e];
-          if (counts<TINY>(c[v], e)) sums[0] += d[v][e] * u[v][e];
-        }
-      }
+      if (a.post_weight) sums[0] += lane_sum<TINY>(c[v], eights, [&](int e) { return d[v][e] * b[v][e]; });
     }
-    const bool token = a.gate_kind == GATE_TOKEN && a.dgate;
-    if (a.post_weight || token) {
-      row_sum<G, 2>(sums, waves, s_sum, side);
-      if (token && live && li == 0) {
-        if (a.gate_dtype == NGDN_BF16) static_cast<bf16*>(a.dgate)[row] = (bf16)sums[1];
-        else static_cast<float*>(a.dgate)[row] = sums[1];
-      }
-    }
-    if (a.dbranch && live) {
-      const float mean = sums[0] * inv;
+    if (a.post_weight || (token && a.dgate)) row_sum<G, 2>(sums, waves, s_sum, side);
+    if (USUAL || a.dbranch) {
+      const float mean = sums[0] * inv;      // 0 without a norm on the branch
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (a.post_weight) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[v][e] = rstd_b * (d[v][e] - u[v][e] * mean);
+          for (int e = 0; e < 8; ++e) d[v][e] = rstd_b * (d[v][e] - b[v][e] * mean);
         }
-        put8<TINY>(static_cast<R*>(a.dbranch) + at, c[v], d[v]);
+        if (G == WAVE || live) put8<TINY>(static_cast<R*>(a.dbranch) + at, c[v], d[v]);
       }
     }
+    if (token && a.dgate && live && li == 0) {
+      if (a.gate_dtype == NGDN_BF16) static_cast<bf16*>(a.dgate)[row] = (bf16)sums[1];
+      else static_cast<float*>(a.dgate)[row] = sums[1];
+    }
+  };
+
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (norm) load_param<TINY>(a.weight, a.w_dtype, 0, c[v], w[v]);
+    branch_factor<TINY>(a, true, group * a.D, c[v], scale, pg[v]);
   }
+  if constexpr (G < WAVE) {
+    // the rows of a wave: those behind the last are the last again, and leave nothing
+    for (long long first = g0 + block * slots; first <= last; first += step) {
+      const bool live = first + slot <= last;
+      work(live ? first + slot : last, live);
+    }
+  } else {
+    for (long long row = g0 + block * slots + slot; row <= last; row += step) work(row, true);
+  }
+
   // the workgroup's sums over rows: its slots in their order
-  for (int k = 0; k < 3; ++k) {
-    const bool wanted = k == 0 ? a.dweight && a.dy : k == 1 ? a.dpost_weight != nullptr : cols && a.dgate;
-    if (!wanted) continue;
+  auto leave = [&](int k, float (&s)[V][8]) __attribute__((always_inline)) {
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (counts<TINY>(c[v], e)) s_row[slot * a.D + c[v].base + e] = k == 0 ? sw[v][e] : k == 1 ? sp[v][e] : sg[v][e];
+        if (counts<TINY>(c[v], e)) s_row[slot * a.D + c[v].base + e] = s[v][e];
     __syncthreads();
+    float* out = a.ws + ((long long)k * gridDim.x + blockIdx.x) * a.D;
     for (int j = threadIdx.x; j < a.D; j += blockDim.x) {
-      float s = 0.f;
-      for (int i = 0; i < slots; ++i) s += s_row[i * a.D + j];
-      a.ws[((long long)k * gridDim.x + blockIdx.x) * a.D + j] = s;
+      float t = 0.f;
+      for (int i = 0; i < slots; ++i) t += s_row[i * a.D + j];
+      out[j] = t;
     }
+  };
+  if (a.dweight && norm) leave(0, sw);
+  float t[8];
+  if (a.dpost_weight) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[v][e] = sb[v][e] * scale;
+      if (cols) {
+        load_param<TINY>(a.gate, a.gate_dtype, group * a.D, c[v], t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[v][e] *= t[e];
+      }
+    }
+    leave(1, w);
+  }
+  if (cols && a.dgate) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[v][e] = sb[v][e] * scale;
+      if (a.post_weight) {
+        load_param<TINY>(a.post_weight, a.pw_dtype, 0, c[v], t);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[v][e] *= t[e];
+      }
+    }
+    leave(2, w);
   }
 }
 
@@ -260,6 +300,7 @@ __global__ __launch_bounds__(1024) void residual_sum_kernel(RowSumArgs a) {
     const float* ws = a.ws[k] + g * a.parts[k] * a.D;
     float v = 0.f;
     if (j < a.D)
+#pragma unroll 8
       for (long long p = slice; p < a.parts[k]; p += SUM_SLICES) v += ws[p * a.D + j];
     __syncthreads();
     s[slice][col] = v;
@@ -280,15 +321,18 @@ template <typename X, typename R, typename Y>
 hipError_t launch_bwd(const ResidualArgs& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.groups * p.blocks));
   const size_t lds = (size_t)p.slots * a.D * 4;
-#define NGDN_GO(G, V, TINY)                                                                              \
-  hipLaunchKernelGGL((residual_bwd_kernel<X, R, Y, G, V, TINY>), grid, dim3(p.threads), lds, st, a, p.waves, \
-                     p.per, p.blocks)
-  if (a.D < 8) NGDN_GO(8, 1, true);
-  else if (p.lanes == 8) NGDN_GO(8, 1, false);
-  else if (p.lanes == 16) NGDN_GO(16, 1, false);
-  else if (p.lanes == 32) NGDN_GO(32, 1, false);
-  else if (p.V == 1) NGDN_GO(64, 1, false);
-  else NGDN_GO(64, 2, false);
+#define NGDN_GO(G, V, TH, USUAL, TINY)                                                                     \
+  hipLaunchKernelGGL((residual_bwd_kernel<X, R, Y, G, V, TH, USUAL, TINY>), grid, dim3(p.threads), lds, st, a, \
+                     p.waves, p.per, p.blocks)
+  const bool usual = a.weight && a.dy && a.dh && a.dx && a.dbranch;
+  if (a.D < 8) NGDN_GO(8, 1, 256, false, true);
+  else if (p.lanes == 8) NGDN_GO(8, 1, 256, false, false);
+  else if (p.lanes == 16) NGDN_GO(16, 1, 256, false, false);
+  else if (p.lanes == 32) NGDN_GO(32, 1, 256, false, false);
+  else if (p.V == 1 && usual) NGDN_GO(64, 1, 512, true, false);
+  else if (p.V == 1) NGDN_GO(64, 1, 512, false, false);
+  else if (p.waves <= 8) NGDN_GO(64, 2, 512, false, false);
+  else NGDN_GO(64, 2, 1024, false, false);
 #undef NGDN_GO
   return hipGetLastError();
 }
