@@ -10,6 +10,11 @@ ignore index -100, through the fused linear cross entropy when training.
 Registered with transformers' Auto classes under model_type "nested_gdn2",
 as the reference registers itself (nested_gdn2/__init__.py:17-23).
 
+Beyond the reference, each off unless set: norms after the blocks
+(``post_norm``), a gate for each channel of their outputs (``layer_scale``), a
+scale (``branch_scale``) and dropout (``resid_dropout``) before they are added to
+the stream, and ``NestedGDN2ForCausalLM.sample``, which draws tokens on the GPU.
+
 Decoding cache: ``NestedGDN2Cache``, a dict from layer index to the layer's
 entry (``recurrent_state`` = (state [B,H,L,K,V] fp32, position [B] int64),
 ``conv_state`` = fla-layout convolution caches) that also counts the tokens
@@ -29,7 +34,7 @@ from transformers.modeling_utils import PreTrainedModel
 from .layer import NestedGDN2Attention
 from .layer_ops import FusedRMSNormGated, ShortConvolution
 from .model_ops import (Embedding, FusedLinearCrossEntropyLoss, GatedMLP, RMSNorm, add_rms_norm,
-                        rms_norm)
+                        residual_norm, rms_norm, sample_tokens)
 
 __all__ = ["NestedGDN2Config", "NestedGDN2Cache", "NestedGDN2Block", "NestedGDN2Model",
            "NestedGDN2ForCausalLM", "NestedGDN2PreTrainedModel"]
@@ -37,7 +42,11 @@ __all__ = ["NestedGDN2Config", "NestedGDN2Cache", "NestedGDN2Block", "NestedGDN2
 
 class NestedGDN2Config(PretrainedConfig):
     """The reference's config (models/configuration_nested_gdn2.py:10-133):
-    same fields, defaults and checks."""
+    same fields, defaults and checks; and, without a counterpart there and off by
+    default, what happens to a block's output before it is added to the stream:
+    ``post_norm`` (an RMSNorm), ``layer_scale`` (the initial value of a learned gate
+    a channel; None: no gate), ``branch_scale`` and ``resid_dropout``. They need
+    ``fuse_norm``."""
     model_type = "nested_gdn2"
     keys_to_ignore_at_inference = ["past_key_values"]
 
@@ -47,7 +56,8 @@ class NestedGDN2Config(PretrainedConfig):
                  fuse_cross_entropy=True, use_cache=True, norm_eps=1e-5, initializer_range=0.02,
                  tie_word_embeddings=False, num_levels=2, firing_intervals=(1, 4),
                  n_queries_per_level=(64,), promotion="learned", read_mix="softmax",
-                 max_horizon=None, op_chunk_size=64, use_triton=True, **kwargs):
+                 max_horizon=None, op_chunk_size=64, use_triton=True, post_norm=False,
+                 layer_scale=None, branch_scale=1.0, resid_dropout=0.0, **kwargs):
         self.vocab_size = vocab_size
         self.hidden_size = hidden_size
         self.num_hidden_layers = num_hidden_layers
@@ -73,6 +83,14 @@ class NestedGDN2Config(PretrainedConfig):
         self.max_horizon = max_horizon
         self.op_chunk_size = op_chunk_size
         self.use_triton = use_triton
+        self.post_norm = post_norm
+        self.layer_scale = layer_scale
+        self.branch_scale = branch_scale
+        self.resid_dropout = resid_dropout
+        if not 0.0 <= resid_dropout <= 1.0:
+            raise ValueError(f"resid_dropout must be in [0, 1], got {resid_dropout}")
+        if not fuse_norm and (post_norm or layer_scale is not None or branch_scale != 1.0 or resid_dropout):
+            raise ValueError("post_norm, layer_scale, branch_scale and resid_dropout need fuse_norm")
         if len(self.firing_intervals) != num_levels:
             raise ValueError(f"firing_intervals must have length num_levels={num_levels}, "
                              f"got {len(self.firing_intervals)}")
@@ -143,9 +161,40 @@ class NestedGDN2Block(GradientCheckpointingLayer):
         self.mlp = GatedMLP(hidden_size=config.hidden_size, hidden_ratio=config.hidden_ratio,
                             intermediate_size=config.intermediate_size,
                             hidden_act=config.hidden_act, fuse_swiglu=config.fuse_swiglu)
+        # what happens to the two outputs before they are added
+        D = config.hidden_size
+        self.branch_scale, self.resid_dropout = config.branch_scale, config.resid_dropout
+        if config.post_norm:
+            self.attn_post_norm = RMSNorm(D, eps=config.norm_eps)
+            self.mlp_post_norm = RMSNorm(D, eps=config.norm_eps)
+        if config.layer_scale is not None:
+            self.attn_gate = nn.Parameter(torch.full((D,), float(config.layer_scale)))
+            self.mlp_gate = nn.Parameter(torch.full((D,), float(config.layer_scale)))
+        self.plain = not (config.post_norm or config.layer_scale is not None
+                          or config.branch_scale != 1.0 or config.resid_dropout)
+
+    def branch(self, which):
+        """The norm's weight and the gate of "attn" or "mlp" (None where there is none)."""
+        norm = getattr(self, which + "_post_norm", None)
+        return None if norm is None else norm.weight, getattr(self, which + "_gate", None)
+
+    def join(self, hidden_states, out, params, norm=None, out_dtype=None):
+        """The stream with a block's output ``out`` added (``params``: what
+        ``branch`` gives for it), and, with ``norm``, what that norm makes of it.
+        In training each call drops other values (a seed of torch's CPU generator,
+        which checkpointing sets back for its second forward)."""
+        if self.plain:
+            if norm is None:
+                return hidden_states + out
+            return add_rms_norm(hidden_states, out, norm.weight, norm.eps, out_dtype)
+        p = self.resid_dropout if self.training else 0.0
+        seed = int(torch.randint(1 << 62, ())) if p else 0
+        weight, eps = (None, self.attn_norm.eps) if norm is None else (norm.weight, norm.eps)
+        return residual_norm(hidden_states, out, weight, *params, branch_scale=self.branch_scale, p=p,
+                             seed=seed, eps=eps, out_dtype=out_dtype)
 
     def forward(self, hidden_states, residual=None, past_key_values=None, use_cache=False,
-                defer_residual=False):
+                defer_residual=False, residual_params=(None, None)):
         """Same values as norm -> attn -> add -> norm -> mlp -> add. The norms
         write the dtype their consumers compute in (bf16 under autocast: the
         cast the projections would make) and each residual add runs inside
@@ -153,7 +202,8 @@ class NestedGDN2Block(GradientCheckpointingLayer):
         ``residual`` (the previous block's deferred MLP output) the input is
         hidden_states + residual, added inside the first norm; with
         ``defer_residual`` the block returns (h, mlp_out, cache) for the next
-        norm to add instead of h + mlp_out."""
+        norm to add instead of h + mlp_out; ``residual_params`` is what the previous
+        block's ``branch`` gives for the output that it deferred."""
         if not self.fused:
             if residual is not None:
                 hidden_states = hidden_states + residual
@@ -171,14 +221,14 @@ class NestedGDN2Block(GradientCheckpointingLayer):
         if residual is None:
             y = rms_norm(hidden_states, an.weight, an.eps, cdt)
         else:
-            hidden_states, y = add_rms_norm(hidden_states, residual, an.weight, an.eps, cdt)
+            hidden_states, y = self.join(hidden_states, residual, residual_params, an, cdt)
         attn_out, _, past_key_values = self.attn(y, past_key_values=past_key_values,
                                                  use_cache=use_cache)
-        hidden_states, y = add_rms_norm(hidden_states, attn_out, mn.weight, mn.eps, cdt)
+        hidden_states, y = self.join(hidden_states, attn_out, self.branch("attn"), mn, cdt)
         mlp_out = self.mlp(y)
         if defer_residual:
             return hidden_states, mlp_out, past_key_values
-        return hidden_states + mlp_out, past_key_values
+        return self.join(hidden_states, mlp_out, self.branch("mlp")), past_key_values
 
 
 class NestedGDN2PreTrainedModel(PreTrainedModel):
@@ -195,6 +245,9 @@ class NestedGDN2PreTrainedModel(PreTrainedModel):
             for p in (module.A_log, module.dt_bias):
                 p._no_weight_decay = True
             return
+        if isinstance(module, NestedGDN2Block) and self.config.layer_scale is not None:
+            nn.init.constant_(module.attn_gate, self.config.layer_scale)
+            nn.init.constant_(module.mlp_gate, self.config.layer_scale)
         if isinstance(module, (nn.Linear, nn.Conv1d, ShortConvolution)):
             nn.init.normal_(module.weight, mean=0.0, std=self.config.initializer_range)
             if getattr(module, "bias", None) is not None:
@@ -235,21 +288,24 @@ class NestedGDN2Model(NestedGDN2PreTrainedModel):
         if use_cache and not isinstance(past_key_values, NestedGDN2Cache):
             past_key_values = NestedGDN2Cache.from_legacy_cache(past_key_values)
         all_hidden_states = () if output_hidden_states else None
-        residual = None     # each block's MLP output, added inside the next norm
+        # each block's MLP output, added inside the next norm, the block, and what it
+        # says of that output
+        residual, last, params = None, None, (None, None)
         for layer in self.layers:
             if output_hidden_states:
                 if residual is not None:
-                    hidden_states, residual = hidden_states + residual, None
+                    hidden_states, residual = last.join(hidden_states, residual, params), None
                 all_hidden_states += (hidden_states,)
             # the tensors positionally, as checkpointing with use_reentrant
             # needs them
             hidden_states, residual, past_key_values = layer(
                 hidden_states, residual, past_key_values=past_key_values, use_cache=use_cache,
-                defer_residual=True)
+                defer_residual=True, residual_params=params)
+            last, params = layer, layer.branch("mlp")
         if use_cache:
             past_key_values.seen_tokens += hidden_states.shape[1]
         if residual is not None and self.config.fuse_norm:
-            _, hidden_states = add_rms_norm(hidden_states, residual, self.norm.weight, self.norm.eps)
+            _, hidden_states = last.join(hidden_states, residual, params, self.norm)
         else:
             if residual is not None:
                 hidden_states = hidden_states + residual
@@ -302,6 +358,36 @@ class NestedGDN2ForCausalLM(NestedGDN2PreTrainedModel, GenerationMixin):
         if seen:
             input_ids = input_ids[:, seen:]
         return {"input_ids": input_ids, "past_key_values": past_key_values, "use_cache": use_cache}
+
+    @torch.no_grad()
+    def sample(self, input_ids, max_new_tokens, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, u=None,
+               generator=None, eos_token_id=None):
+        """input_ids [B,T] continued by up to max_new_tokens tokens each, drawn by
+        ``model_ops.sample_tokens``: the settings are numbers, or tensors [B] of one
+        a request. ``u`` [B, max_new_tokens] are the random numbers (torch.rand's,
+        from ``generator``, if None): the same ones give the same tokens. With
+        ``eos_token_id`` a sequence that has ended goes on with it, and the call
+        ends with the last sequence (a host synchronisation a token; without it
+        there is none). A sequence whose logits are not finite goes on with -1."""
+        B = input_ids.shape[0]
+        if u is None:
+            u = torch.rand(B, max_new_tokens, device=input_ids.device, generator=generator)
+        if u.shape != (B, max_new_tokens):
+            raise ValueError(f"sample: u {tuple(u.shape)} for {B} sequences and {max_new_tokens} tokens")
+        u, cache, token = u.t().contiguous(), None, input_ids
+        ended = torch.zeros(B, dtype=torch.bool, device=input_ids.device)
+        for i in range(max_new_tokens):
+            out = self.model(input_ids=token, past_key_values=cache, use_cache=True, return_dict=True)
+            cache = out.past_key_values
+            token = sample_tokens(self.lm_head(out.last_hidden_state[:, -1]), u[i], temperature, top_k, top_p, min_p)
+            if eos_token_id is not None:
+                token = torch.where(ended, eos_token_id, token)
+                ended |= token == eos_token_id
+            token = token.unsqueeze(1)
+            input_ids = torch.cat((input_ids, token), 1)
+            if eos_token_id is not None and bool(ended.all()):
+                break
+        return input_ids
 
     def forward(self, input_ids=None, attention_mask=None, inputs_embeds=None, labels=None,
                 output_hidden_states=None, return_dict=None, past_key_values=None, use_cache=None,
