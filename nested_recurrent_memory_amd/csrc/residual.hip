@@ -196,15 +196,16 @@ bool residual_types(int xd, int rd, int yd) {
 
 namespace {
 
-// As many waves as run at once, four a SIMD: 12 and 20 a CU instead of 16 take 77 and
-// 86 us where 16 take 77 (fp32 stream), 139 and 143 where 16 take 126 (dropout).
-constexpr long long FWD_WAVES = 256 * 16;
-
 template <typename X, typename R, typename Y, bool PRE>
 hipError_t launch_fwd(const ResidualArgs& a, hipStream_t st) {
   const int D = a.D;
+  // As many whole workgroups as 16 waves a CU hold (four a SIMD, at the registers that a
+  // row takes): 12 and 20 waves take 77 and 86 us where 16 take 77 (fp32 stream), 139 and
+  // 143 where 16 take 126 (dropout); part of a round more, 47 where 37 (2816 columns).
+  // Rows of up to 8192 by eight values a lane: sixteen take 62 us where eight take 47 (8192
+  // columns), and 24.5 where 20 (768 columns, one wave where two)
   auto go = [&](auto kernel, int threads, int slots, int waves) {
-    const long long want = (a.rows + slots - 1) / slots, most = FWD_WAVES * 64 / threads;
+    const long long want = (a.rows + slots - 1) / slots, most = 256LL * (threads < 1024 ? 1024 / threads : 1);
     hipLaunchKernelGGL(kernel, dim3((unsigned)(want < most ? want : most)), dim3(threads), 0, st, a, waves);
     return hipGetLastError();
   };

@@ -26,10 +26,7 @@ struct Plan {
   long long groups, per, blocks;     // rows of a group, workgroups a group
 };
 
-// As many waves as run at once, three a SIMD at the registers that a row takes: more
-// would leave more partial rows. Two rows a slot at least, which halves those of a
-// small batch.
-constexpr long long BWD_WAVES = 256 * 12;
+// Two rows a slot at least, which halves the partial rows of a small batch.
 constexpr int BWD_ROWS = 2;
 
 Plan plan_bwd(const ResidualArgs& a) {
@@ -41,14 +38,17 @@ Plan plan_bwd(const ResidualArgs& a) {
     p.threads = 256; p.waves = 1;
   } else {
     p.waves = (D + 511) / 512;
-    if (p.waves > 8) { p.V = 2; p.waves = (p.waves + 1) / 2; }
+    if (p.waves > 16) { p.V = 2; p.waves = (p.waves + 1) / 2; }
     p.lanes = p.waves * 64;
     p.threads = p.waves == 1 ? 256 : p.lanes;
   }
   p.slots = p.threads / p.lanes;
   p.groups = a.gate_kind != GATE_SEQUENCE ? 1 : a.rows > 0 ? a.rows / a.seq : 0;
   p.per = a.gate_kind == GATE_SEQUENCE ? a.seq : a.rows;
-  const long long want = (p.per + p.slots * BWD_ROWS - 1) / (p.slots * BWD_ROWS), all = BWD_WAVES * 64 / p.threads;
+  // a CU's share: 12 waves in small workgroups (16 are no faster and leave more partial
+  // rows), else as many workgroups as 16 waves hold
+  const long long want = (p.per + p.slots * BWD_ROWS - 1) / (p.slots * BWD_ROWS);
+  const long long all = 256LL * (p.threads <= 256 ? 768 / p.threads : 1024 / p.threads);
   const long long most = p.groups > 0 && all / p.groups > 1 ? all / p.groups : 1;
   p.blocks = want < most ? want : most;
   return p;
@@ -329,9 +329,8 @@ hipError_t launch_bwd(const ResidualArgs& a, const Plan& p, hipStream_t st) {
   else if (p.lanes == 8) NGDN_GO(8, 1, 256, false, false);
   else if (p.lanes == 16) NGDN_GO(16, 1, 256, false, false);
   else if (p.lanes == 32) NGDN_GO(32, 1, 256, false, false);
-  else if (p.V == 1 && usual) NGDN_GO(64, 1, 512, true, false);
-  else if (p.V == 1) NGDN_GO(64, 1, 512, false, false);
-  else if (p.waves <= 8) NGDN_GO(64, 2, 512, false, false);
+  else if (p.V == 1 && usual) NGDN_GO(64, 1, 1024, true, false);
+  else if (p.V == 1) NGDN_GO(64, 1, 1024, false, false);
   else NGDN_GO(64, 2, 1024, false, false);
 #undef NGDN_GO
   return hipGetLastError();
