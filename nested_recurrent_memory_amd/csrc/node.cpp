@@ -178,7 +178,20 @@ Stream stream_from(const char* name, double p, const py::object& seed, const py:
   return s;
 }
 
-const int64_t* seed_of(const Tensor& t) { return t.defined() ? t.const_data_ptr<int64_t>() : nullptr; }
+// A pointer for a kernel: of memory on the GPU, which tensors of function transforms, fake
+// ones and other subclasses with a dispatch of their own do not hold. Null where undefined.
+const void* raw(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  if (!t.has_storage() || t.key_set().has(c10::DispatchKey::Python))
+    throw std::runtime_error("the library's kernels take plain tensors: function transforms, tracers and tensor "
+                             "subclasses are not supported");
+  return t.const_data_ptr();
+}
+void* raw_out(const Tensor& t) {
+  return raw(t) ? t.mutable_data_ptr() : nullptr;
+}
+
+const int64_t* seed_of(const Tensor& t) { return static_cast<const int64_t*>(raw(t)); }
 
 void plain_gradient(const char* name, const Tensor& g) {
   if (g.defined() && !g.has_storage())
@@ -190,7 +203,7 @@ Tensor drop(const Tensor& x, const Stream& s) {
   const Tensor c = x.contiguous();
   Tensor y = at::empty_like(c);
   done(ngdn_dropout(code(c), c.numel(), s.threshold, s.keep(), s.seed, seed_of(s.seed_tensor), s.offset,
-                    c.const_data_ptr(), y.mutable_data_ptr(), stream(c)),
+                    raw(c), raw_out(y), stream(c)),
        "ngdn_dropout");
   return y;
 }
@@ -226,6 +239,7 @@ Tensor dropout(const Tensor& x, double p, const py::object& seed, const py::obje
   on_gpu("dropout", x, x);
   if (s.seed_tensor.defined()) on_gpu("dropout", s.seed_tensor, x);
   if (s.threshold == 0) return x;
+  const py::gil_scoped_release free;        // a launch may wait for room in the queue
   const Tensor w = widened(x);
   Tensor y;
   if (wants_grad({w})) {
@@ -251,9 +265,8 @@ struct Seed {       // a tensor that autograd does not take for an input
 };
 
 void point(ngdn_residual_args& a, const Parts& t) {
-  const auto ptr = [](const Tensor& v) { return v.defined() ? v.const_data_ptr() : nullptr; };
-  a.x = ptr(t[0]); a.branch = ptr(t[1]); a.weight = ptr(t[2]); a.post_weight = ptr(t[3]);
-  a.gate = ptr(t[4]); a.seed_ptr = seed_of(t[5]);
+  a.x = raw(t[0]); a.branch = raw(t[1]); a.weight = raw(t[2]); a.post_weight = raw(t[3]);
+  a.gate = raw(t[4]); a.seed_ptr = seed_of(t[5]);
 }
 
 Tensor whole(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
@@ -269,14 +282,14 @@ void residual_forward(const Parts& t, const Residual& r, Tensor* out, bool saved
   ngdn_residual_args a = r.a;
   point(a, t);
   out[0] = at::empty_like(t[0]);
-  a.h = out[0].mutable_data_ptr();
+  a.h = raw_out(out[0]);
   if (t[2].defined()) {
     out[1] = at::empty_like(t[0], t[0].options().dtype(r.y_type));
-    a.y = out[1].mutable_data_ptr();
+    a.y = raw_out(out[1]);
   }
   if (saved) {
     out[2] = at::empty({2, a.rows}, t[0].options().dtype(at::kFloat));
-    a.rstd_h = static_cast<float*>(out[2].mutable_data_ptr());
+    a.rstd_h = static_cast<float*>(raw_out(out[2]));
     a.rstd_b = a.rstd_h + a.rows;
   }
   done(ngdn_residual_norm_fwd(&a, stream(t[0])), "ngdn_residual_norm_fwd");
@@ -325,14 +338,13 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
         if (which >> i & 1 && ctx->needs_input_grad(j++)) out[i] = at::empty_like(t[i]);
       ngdn_residual_args a = r->a;
       point(a, t);
-      const auto ptr = [](const Tensor& v) { return v.defined() ? v.mutable_data_ptr() : nullptr; };
-      a.rstd_h = static_cast<float*>(ptr(saved.back()));
+      a.rstd_h = static_cast<float*>(raw_out(saved.back()));
       a.rstd_b = a.rstd_h + a.rows;
-      a.dh = ptr(dh); a.dy = ptr(dy);
-      a.dx = ptr(out[0]); a.dbranch = ptr(out[1]); a.dweight = ptr(out[2]); a.dpost_weight = ptr(out[3]);
-      a.dgate = ptr(out[4]);
+      a.dh = raw(dh); a.dy = raw(dy);
+      a.dx = raw_out(out[0]); a.dbranch = raw_out(out[1]); a.dweight = raw_out(out[2]); a.dpost_weight = raw_out(out[3]);
+      a.dgate = raw_out(out[4]);
       const Tensor ws = at::empty({ngdn_residual_norm_ws(&a)}, t[0].options().dtype(at::kFloat));
-      a.ws = static_cast<float*>(ws.mutable_data_ptr());
+      a.ws = static_cast<float*>(raw_out(ws));
       done(ngdn_residual_norm_bwd(&a, stream(t[0])), "ngdn_residual_norm_bwd");
     }
     if (at::GradMode::is_enabled()) {
@@ -421,6 +433,7 @@ py::object residual_norm(const Tensor& x0, const Tensor& branch0, const Optional
   a.residual_scale = (float)residual_scale; a.branch_scale = (float)branch_scale; a.eps = (float)eps;
   a.threshold = s.threshold; a.keep = s.keep(); a.seed = s.seed; a.offset = s.offset;
   Tensor out[3];
+  auto free = std::make_unique<py::gil_scoped_release>();        // a launch may wait for room in the queue
   if (wants_grad({t[0], t[1], t[2], t[3], t[4]})) {
     std::vector<Tensor> there;
     unsigned which = 0;
@@ -436,8 +449,9 @@ py::object residual_norm(const Tensor& x0, const Tensor& branch0, const Optional
     residual_forward(whole(t), *r, out, false);
   }
   if (out[0].scalar_type() != h_type) out[0] = out[0].to(h_type);
+  if (t[2].defined() && out[1].scalar_type() != y_type) out[1] = out[1].to(y_type);
+  free.reset();
   if (!t[2].defined()) return py::cast(out[0]);
-  if (out[1].scalar_type() != y_type) out[1] = out[1].to(y_type);
   return py::make_tuple(out[0], out[1]);
 }
 
@@ -473,7 +487,7 @@ struct Setting {
     if (!rows.defined()) return nullptr;
     if (!whole_number && rows.scalar_type() != at::kFloat) rows = rows.to(at::kFloat);
     rows = rows.dim() == 0 ? rows.expand(u.sizes()).contiguous() : rows.contiguous();
-    return rows.const_data_ptr();
+    return raw(rows);
   }
 };
 
@@ -492,6 +506,7 @@ Tensor sample_tokens(const Tensor& logits0, const Tensor& u0, const py::object& 
   on_gpu(name, logits0, logits0);
   for (const Tensor& v : {u0, t.rows, k.rows, p.rows, m.rows})
     if (v.defined()) on_gpu(name, v, logits0);
+  const py::gil_scoped_release free;
   const at::NoGradGuard off;
   const c10::DeviceGuard guard(logits0.device());
   const Tensor u = u0.detach().contiguous();
@@ -510,8 +525,8 @@ Tensor sample_tokens(const Tensor& logits0, const Tensor& u0, const py::object& 
   a.min_p_ptr = static_cast<const float*>(m.ptr(u, false));
   a.top_k_ptr = k.ptr(u, true);
   a.top_k_wide = k.rows.defined() && k.rows.scalar_type() == at::kLong;
-  a.logits = logits.const_data_ptr(); a.u = u.const_data_ptr();
-  a.token = token.mutable_data_ptr<int64_t>();
+  a.logits = raw(logits); a.u = raw(u);
+  a.token = static_cast<int64_t*>(raw_out(token));
   done(ngdn_sample(code(logits), &a, stream(logits)), "ngdn_sample");
   return token;
 }

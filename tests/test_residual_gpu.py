@@ -421,3 +421,79 @@ def test_the_gradient_is_the_differences():
         want = (g.double() * v.double()).sum().item()
         scale = (g.double().norm() * v.double().norm()).item()
         assert abs((up - down) / 2e-2 - want) <= 1e-2 * scale, n
+
+
+def test_function_transforms_fake_tensors_and_subclasses_are_refused():
+    a, _, _ = make((3, 20), TYPES[0])
+    x, b, w = a["x"].cuda(), a["branch"].cuda(), a["weight"].cuda()
+    for f in (lambda t: residual_norm(t, b, w)[1], lambda t: dropout(t, 0.3, 1)):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: f(t).sum())(x)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(lambda t: f(t))(torch.stack((x, x)))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (x,))
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        fake = mode.from_tensor(x)
+        for f in (lambda: residual_norm(fake, fake), lambda: dropout(fake, 0.3, 1), lambda: residual_norm(x, b, w),
+                  lambda: dropout(x, 0.3, 1)):
+            with pytest.raises((RuntimeError, AssertionError)):       # the mode's own for tensors not of it
+                f()
+
+
+def test_more_than_2_to_31_values():
+    """The last rows of 2^31 values and more: places, and the generator's blocks."""
+    rows, D = (1 << 20) + 3, 2048
+    x = torch.zeros(rows, D, dtype=BF16, device="cuda")
+    b = torch.zeros(rows, D, dtype=BF16, device="cuda")
+    g = torch.Generator().manual_seed(0)
+    tx, tb, w = (torch.randn(s, generator=g) for s in ((3, D), (3, D), (D,)))
+    x[-3:], b[-3:] = tx.cuda(), tb.cuda()
+    first = (rows - 3) * D
+    keep = torch.tensor(oracle.words(first, 3 * D, 77, 5), dtype=torch.int64).view(3, D) >= round(0.25 * 2 ** 32)
+    h, y = residual_norm(x, b, w.cuda(), p=0.25, seed=77, offset=5)
+    tx, tb = tx.to(BF16), tb.to(BF16)
+    want = oracle.residual_norm(tx, torch.where(keep, tb.double() / 0.75, 0.0), w)
+    for n, t in (("h", h), ("y", y)):
+        value, bound = want[n]
+        # the branch's factor rounds once more than the oracle knows of
+        close(n, t[-3:], (value, bound + 4 * 2.0 ** -24 * value.abs()), BF16)
+    assert (h[:-3] == 0).all()
+    del h, y
+    got = dropout(x, 0.25, 77, 5)[-3:]
+    assert torch.equal(got.cpu(), torch.where(keep, tx.float() * (1 / 0.75), 0.0).to(BF16))
+    xg = x.requires_grad_(True)
+    h, y = residual_norm(xg, b, w.cuda(), p=0.25, seed=77, offset=5)
+    dy = torch.zeros_like(b)
+    dy[-3:] = tb.cuda()
+    dx, = torch.autograd.grad(y, xg, dy)
+    want = oracle.residual_norm(tx, torch.where(keep, tb.double() / 0.75, 0.0), w, dy=tb)["dx"]
+    close("dx", dx[-3:], (want[0], 1.01 * want[1] + 2.0 ** -20 * want[0].abs().max()), BF16)
+
+
+def test_threads_and_streams_at_once():
+    """Four threads, a stream each, both passes: the bits of one alone."""
+    import threading
+    cases = [make((50 + i, 640), TYPES[1], "channel", seed=i) for i in range(4)]
+
+    def work(a, dh, dy):
+        cu = {n: t.cuda().requires_grad_(True) for n, t in a.items()}
+        h, y = residual_norm(**cu, p=0.1, seed=2)
+        return [h, y, *torch.autograd.grad([h, y], list(cu.values()), [dh.cuda(), dy.cuda()])]
+
+    want = [work(*c) for c in cases]
+    got = [None] * 4
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i] = work(*cases[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(p, q) for a, b in zip(got, want) for p, q in zip(a, b))

@@ -219,3 +219,31 @@ def test_a_token_after_a_block():
     y = oracle.residual_norm(x, b, w, pw, gate)["y"][0]
     # a dot product of 64 fp32 terms and the norm's own error, on logits of order 10
     assert (logits.cpu().double() - y @ head.double().t()).abs().max() < 1e-3
+
+
+def test_rows_far_apart():
+    """Rows 2^31 values and more from each other."""
+    l, u = make(3, 1000, BF16, "peaked")
+    x = torch.empty(2 * ((1 << 31) + 77) + 1000, dtype=BF16, device="cuda")
+    rows = x.as_strided((3, 1000), ((1 << 31) + 77, 1))
+    rows.copy_(l)
+    assert torch.equal(sample_tokens(rows, u.cuda(), top_k=30, top_p=0.9).cpu(), oracle.sample(l, u, top_k=30, top_p=0.9))
+
+
+def test_tensors_of_transforms_are_refused():
+    l, u = torch.randn(3, 40, device="cuda"), torch.rand(3, device="cuda")
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.func.vmap(lambda a, b: sample_tokens(a, b))(l, u)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode() as mode:
+        with pytest.raises(RuntimeError):
+            sample_tokens(mode.from_tensor(l), mode.from_tensor(u))
+        with pytest.raises((RuntimeError, AssertionError)):           # the mode's own for tensors not of it
+            sample_tokens(l, u)
+
+
+def test_logits_that_require_a_gradient():
+    l, u = make(4, 300)
+    x = l.cuda().requires_grad_(True)
+    token = sample_tokens(x, u.cuda())
+    assert not token.requires_grad and torch.equal(token.cpu(), oracle.sample(l, u))
