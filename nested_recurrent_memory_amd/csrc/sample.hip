@@ -431,9 +431,11 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
       if (threadIdx.x < s.listed) atomicMin(&s.lo, ~(uint32_t)s.place[threadIdx.x]);
     } else {
       __syncthreads();
+      uint32_t first = 0xffffffffu;
       visit(s, row, is_top, [&](float l, int i) {
-        if (l == top) atomicMin(&s.lo, (uint32_t)i);
+        if (l == top && (uint32_t)i < first) first = (uint32_t)i;
       });
+      atomicMin(&s.lo, first);
     }
     __syncthreads();
     if (threadIdx.x == 0) a.token[r] = s.lo;
@@ -533,12 +535,13 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
         return s.best;
       }
       spoilt = true;
-      // the range of the logits in this bin
+      // the range of the logits in this bin; near the last bins some of them weigh nothing
+      const bool live_bin = bin < NB - 2 * NB / (s_bits + 2);
       if (threadIdx.x == 0) { s.lo = 0xffffffffu; s.hi = 0; }
       __syncthreads();
       uint32_t lo = 0xffffffffu, hi = 0;
       visit(s, row, [&](float m) { return bin_of(m) <= bin; }, [&](float l, int) {
-        if (bin_of(l) == bin && weigh(l)) {
+        if (bin_of(l) == bin && (live_bin || weigh(l))) {
           const uint32_t key = key_of(l);
           lo = key < lo ? key : lo;
           hi = key > hi ? key : hi;
@@ -548,35 +551,42 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
       atomicMax(&s.hi, hi);
       __syncthreads();
       lo = s.lo; hi = s.hi;
+      // a bf16's key is its upper half: the lower is 0, or all ones below zero
+      constexpr int LOW = sizeof(E) == 2 ? 16 : 0;
+      auto value_of = [](uint32_t k) { return logit_of(LOW ? k << LOW | (k >> 15 ? 0u : 0xffffu) : k); };
+      lo >>= LOW;
+      hi >>= LOW;
       for (;;) {
         const uint32_t width = hi - lo;
         const int bits = width ? 32 - __clz(width) : 0, shift = bits > 11 ? bits - 11 : 0;
-        const float least = logit_of(lo);
+        const bool single = shift == 0;                // a bin for each value: counts are enough
+        const float least = value_of(lo);
         clear_bins(s);
         visit(s, row, [&](float m) { return m >= least; }, [&](float l, int) {
-          const uint32_t key = key_of(l);
+          const uint32_t key = key_of(l) >> LOW;
           if (key >= lo && key <= hi) {
             atomicAdd(&s.count[(hi - key) >> shift], 1u);
-            atomicAdd(&s.weight[(hi - key) >> shift], weigh(l));
+            if (!single) atomicAdd(&s.weight[(hi - key) >> shift], weigh(l));
           }
         });
+        __syncthreads();
+        if (single)
+          for (uint32_t i = threadIdx.x; i <= width; i += TH) s.weight[i] = s.count[i] * weigh(value_of(hi - i));
         find_bin(s, by_weight, target, before_c, before_w);
         const uint32_t b = (uint32_t)s.bin, in_c = s.in_c;
         const u64 in_w = s.in_w;
         before_c = s.before_c; before_w = s.before_w;
         hi -= b << shift;
-        if (shift == 0) {
-          const u64 each = in_w / in_c;            // equal logits have equal weights
+        if (single) {
+          const u64 each = in_w / in_c;                // equal logits have equal weights
           const u64 kept = by_weight ? (target - before_w + each - 1) / each : target - before_c;
+          const float value = value_of(hi);
           sum = before_w + kept * each;
-          int last = row.V;                        // every index
-          if (kept < in_c) {
-            const uint32_t key = hi;
-            const float value = logit_of(key);
+          int last = row.V;                            // every index
+          if (kept < in_c)
             last = select_index(s, row, [&](float m) { return m >= value; },
-                                [&](float l, int) -> u64 { return key_of(l) == key; }, [&](u64) { return kept - 1; });
-          }
-          return (u64)hi << 32 | (uint32_t)~last;
+                                [&](float l, int) -> u64 { return l == value; }, [&](u64) { return kept - 1; });
+          return (u64)key_of(value) << 32 | (uint32_t)~last;
         }
         const uint32_t span = (1u << shift) - 1;
         lo = hi - lo > span ? hi - span : lo;

@@ -134,6 +134,21 @@ def test_zeros_of_both_signs_are_equal():
         check(l, torch.tensor([0.0, 0.3, 0.6, 0.99]), **kw)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_many_equal_logits_of_both_signs(dtype):
+    """More equal ones than a list holds in the bin where the last one kept is, on
+    either side of zero, and few values in all."""
+    g = torch.Generator().manual_seed(9)
+    for V in (3000, 40000):
+        l = (1e-3 * torch.randint(-3, 4, (5, V), generator=g)).to(dtype)
+        l[3] = l[3].abs()
+        l[4] = -l[4].abs() - 1
+        for kw in (dict(top_k=V // 3), dict(top_k=V // 2), dict(top_k=6 * V // 7), dict(top_p=0.1), dict(top_p=0.45),
+                   dict(top_p=0.6), dict(top_p=0.95), dict(top_k=V // 2, top_p=0.9), dict(temperature=0.0)):
+            for u in (torch.rand(5, generator=g), torch.zeros(5), torch.full((5,), 1 - 2.0 ** -24)):
+                check(l, u, **kw)
+
+
 def test_strided_rows():
     """The last position of prompts, a vocabulary padded in memory, a row that
     starts at an odd value, columns, more dimensions, none."""
