@@ -181,14 +181,18 @@ class NestedGDN2Block(GradientCheckpointingLayer):
     def join(self, hidden_states, out, params, norm=None, out_dtype=None):
         """The stream with a block's output ``out`` added (``params``: what
         ``branch`` gives for it), and, with ``norm``, what that norm makes of it.
-        In training each call drops other values (a seed of torch's CPU generator,
-        which checkpointing sets back for its second forward)."""
+        In training each call drops other values: by a seed of torch's CPU generator,
+        which checkpointing sets back for its second forward, or, captured into a
+        graph, one that each replay draws on the GPU."""
         if self.plain:
             if norm is None:
                 return hidden_states + out
             return add_rms_norm(hidden_states, out, norm.weight, norm.eps, out_dtype)
         p = self.resid_dropout if self.training else 0.0
-        seed = int(torch.randint(1 << 62, ())) if p else 0
+        seed = 0
+        if p:
+            seed = (torch.randint(1 << 62, (1,), device=hidden_states.device)
+                    if torch.cuda.is_current_stream_capturing() else int(torch.randint(1 << 62, (), device="cpu")))
         weight, eps = (None, self.attn_norm.eps) if norm is None else (norm.weight, norm.eps)
         return residual_norm(hidden_states, out, weight, *params, branch_scale=self.branch_scale, p=p,
                              seed=seed, eps=eps, out_dtype=out_dtype)

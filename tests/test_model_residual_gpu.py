@@ -103,6 +103,36 @@ def test_gradient_checkpointing_drops_the_same(reentrant):
         assert rel(got[n], want[n]) <= 1e-5, n
 
 
+def test_a_captured_join_drops_other_values_on_each_replay():
+    block = make(resid_dropout=0.25).train().model.layers[0]
+    x, out = torch.zeros(64, 128, device=DEV), torch.ones(64, 128, device=DEV)
+    params = block.branch("attn")
+
+    def work():
+        with torch.no_grad():
+            return block.join(x, out, params, block.mlp_norm)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        h, y = work()
+    seen = []
+    for _ in range(4):
+        g.replay()
+        torch.cuda.synchronize()
+        kept = h != 0
+        assert torch.equal(h[kept], torch.full_like(h[kept], 1 / 0.75))
+        # 8192 draws: five standard deviations are 0.024
+        assert abs(kept.double().mean().item() - 0.75) < 0.024
+        seen.append(kept.clone())
+        work()
+    assert all(not torch.equal(a, b) for i, a in enumerate(seen) for b in seen[:i])
+
+
 @pytest.mark.parametrize("autocast", [False, True])
 def test_bf16(autocast):
     """Autocast (an fp32 stream) and a bf16 model: a finite loss, close to fp32's."""
