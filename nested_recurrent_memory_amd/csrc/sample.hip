@@ -223,17 +223,22 @@ __device__ __forceinline__ void clear_bins(Shared& s) {
   __syncthreads();
 }
 
-// the first bin with which the count (by_weight: the weight) reaches target >= 1,
-// which lies within the bins' whole; base_c and base_w lie before bin 0
-__device__ __forceinline__ void find_bin(Shared& s, bool by_weight, u64 target, uint32_t base_c, u64 base_w) {
+// the first bin with which the count (by_weight: the weight) reaches target_of(the bins'
+// whole), 1 at least; none where the whole does not reach it. base_c and base_w lie before
+// bin 0. Gives the whole
+struct Whole { uint32_t count; u64 weight; };
+template <typename T>
+__device__ __forceinline__ Whole find_bin(Shared& s, bool by_weight, T target_of, uint32_t base_c, u64 base_w) {
   __syncthreads();
   const int i = threadIdx.x * 2;
   const uint32_t ca = s.count[i], cb = s.count[i + 1];
   const u64 wa = s.weight[i], wb = s.weight[i + 1];
-  uint32_t c, ct;
-  u64 w, wt;
-  scan_block(s, ca + cb, wa + wb, c, w, ct, wt);
+  uint32_t c;
+  u64 w;
+  Whole all;
+  scan_block(s, ca + cb, wa + wb, c, w, all.count, all.weight);
   c += base_c; w += base_w;
+  const u64 target = target_of(all);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const uint32_t cj = j ? cb : ca;
@@ -245,6 +250,7 @@ __device__ __forceinline__ void find_bin(Shared& s, bool by_weight, u64 target, 
     c += cj; w += wj;
   }
   __syncthreads();
+  return all;
 }
 
 // the first index with f(l, i) summed up to and with it above target(whole sum): sums over
@@ -478,7 +484,7 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
     clear_bins(s);
     if (mine > -INFINITY) atomicAdd(&s.count[bin_of(mine)], 1u);
     if (threadIdx.x == 0) s.bin = NB - 1;           // fewer than k lanes have one
-    find_bin(s, false, (u64)k, 0, 0);
+    find_bin(s, false, [&](Whole) { return (u64)k; }, 0, 0);
     const int bin = s.bin;
     auto there = [&](float l) { return l > -INFINITY && bin_of(l) <= bin; };
     if (gather(s, row, false, there, there)) {
@@ -503,17 +509,14 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
   u64 cut = 0;                                      // the place of the last that is kept
   if (some || top_p < 1.f) {
     histogram();
-    uint32_t c, live;
-    u64 w, whole;
-    {
-      const int i = threadIdx.x * 2;
-      scan_block(s, s.count[i] + s.count[i + 1], s.weight[i] + s.weight[i + 1], c, w, live, whole);
-    }
+    // the bin in which top_k ends, or without it top_p
+    const Whole all = find_bin(s, !some, [&](Whole v) { return some ? (u64)k : part_of(v.weight, top_p); }, 0, 0);
+    u64 whole = all.weight;
     bool spoilt = false;
     // the last that is kept when target of the count (or the weight) is to be reached, and
     // in sum the weight up to it; found: its bin is known
     auto search = [&](bool by_weight, u64 target, bool found, u64& sum) -> u64 {
-      if (!found) find_bin(s, by_weight, target, 0, 0);
+      if (!found) find_bin(s, by_weight, [&](Whole) { return target; }, 0, 0);
       const int bin = s.bin;
       uint32_t before_c = s.before_c;
       u64 before_w = s.before_w;
@@ -572,7 +575,7 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
         __syncthreads();
         if (single)
           for (uint32_t i = threadIdx.x; i <= width; i += TH) s.weight[i] = s.count[i] * weigh(value_of(hi - i));
-        find_bin(s, by_weight, target, before_c, before_w);
+        find_bin(s, by_weight, [&](Whole) { return target; }, before_c, before_w);
         const uint32_t b = (uint32_t)s.bin, in_c = s.in_c;
         const u64 in_w = s.in_w;
         before_c = s.before_c; before_w = s.before_w;
@@ -592,15 +595,15 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
         lo = hi - lo > span ? hi - span : lo;
       }
     };
-    if (some && (u64)k < live) {
-      cut = search(false, (u64)k, false, whole);
+    if (some && (u64)k < all.count) {
+      cut = search(false, (u64)k, true, whole);
       if (top_p < 1.f && spoilt) histogram();
     }
     if (top_p < 1.f) {
       const u64 target = part_of(whole, top_p);
       const bool first = !cut;
       if (first) {
-        find_bin(s, true, target, 0, 0);
+        if (some) find_bin(s, true, [&](Whole) { return target; }, 0, 0);
         const int bin = s.bin;
         auto there = [&](float l) { return l > -INFINITY && bin_of(l) <= bin; };
         if (gather(s, row, false, there, there)) {
