@@ -680,7 +680,8 @@ int32_t ngdn_dropout(int32_t dtype, int64_t n, int64_t threshold, float keep, in
  * (NULL: zeros) and dy (NULL: zeros), and writes those of dx, dbranch (in x's and
  * branch's types), dweight, dpost_weight and dgate (in their parameters') that are
  * not NULL. ws: ngdn_residual_norm_ws fp32, no initial contents. Sums over
- * rows are fp32 in a fixed order: the same inputs give the same bits. */
+ * rows are fp32 in a fixed order: the same inputs give the same bits. Outputs are
+ * arrays of their own (no input, and none of each other). */
 typedef struct ngdn_residual_args {
   int64_t rows, seq;
   int32_t D, gate_kind;

@@ -66,37 +66,20 @@ __device__ __forceinline__ void widen(const Raw8<bf16>& r, float* o) {
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = (float)r.a[e];
 }
-// a parameter's or gate's eight values as they lie, in either type: no conversion, so a
-// load may be in flight where it is branched over
-struct RawParam { f4 a, b; };
-template <bool TINY>
-__device__ __forceinline__ void raw_param(const void* p, int dtype, long long at, const Chunk& c, RawParam& r) {
-  if (dtype == NGDN_BF16) {
-    const Raw8<bf16> t = raw8<TINY>(static_cast<const bf16*>(p) + at, c);
-    r.a = __builtin_bit_cast(f4, t.a);
-  } else {
-    const Raw8<float> t = raw8<TINY>(static_cast<const float*>(p) + at, c);
-    r.a = t.a; r.b = t.b;
-  }
-}
-__device__ __forceinline__ void widen(const RawParam& r, int dtype, float* o) {
-  if (dtype == NGDN_BF16) widen(Raw8<bf16>{__builtin_bit_cast(bf16x8, r.a)}, o);
-  else widen(Raw8<float>{r.a, r.b}, o);
-}
+// a parameter's or gate's eight values, in either type
 template <bool TINY>
 __device__ __forceinline__ void load_param(const void* p, int dtype, long long at, const Chunk& c, float* o) {
-  RawParam r{};
-  raw_param<TINY>(p, dtype, at, c, r);
-  widen(r, dtype, o);
+  if (dtype == NGDN_BF16) widen(raw8<TINY>(static_cast<const bf16*>(p) + at, c), o);
+  else widen(raw8<TINY>(static_cast<const float*>(p) + at, c), o);
 }
 __device__ __forceinline__ float load_one(const void* p, int dtype, long long at) {
   return dtype == NGDN_BF16 ? (float)static_cast<const bf16*>(p)[at] : static_cast<const float*>(p)[at];
 }
-// post_weight and a gate of channels (its row from gate_at on) times scale, one where
-// there is none
+// scale times post_weight and times a gate of channels (with sequence, one of a sequence too,
+// whose row begins at gate_at), where there are such
 template <bool TINY>
-__device__ __forceinline__ void branch_factor(const ResidualArgs& a, bool sequence, long long gate_at, const Chunk& c, float scale,
-                                              float* o) {
+__device__ __forceinline__ void branch_factor(const ResidualArgs& a, bool sequence, long long gate_at, const Chunk& c,
+                                              float scale, float* o) {
   float t[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = scale;

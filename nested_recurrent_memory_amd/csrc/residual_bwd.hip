@@ -64,16 +64,15 @@ int64_t residual_ws(const ResidualArgs& a) {
 
 // A row's layout is the forward's. A workgroup stays, its parameters and its sums over
 // rows in registers.
-// USUAL: both outputs have a gradient and both inputs want one, so no load or store
-// lies under a branch (behind one the compiler waits for every store before it).
 //
 // HBM-bound: 4 x 8192 rows of 2048, bf16, a gate a channel and dropout move 805 MB (x
 // and branch read again, dh, dy, dx, dbranch) in 167-171 us, 4.8 TB/s of the 4.9-5.2
 // that a copy reaches; the sum over partial rows takes 5. Of the arithmetic, 42 full-rate
 // operations a value (17 of them the generator's), one sum for post_weight and gate
 // instead of two took the pass from 181 to 170 us. The next row's values in flight in a
-// second set of registers, as in the forward, changed nothing (167).
-template <typename X, typename R, typename Y, int G, int V, int TH, bool USUAL, bool TINY>
+// second set of registers, as in the forward, changed nothing (167), nor did a variant
+// without a branch over any load or store.
+template <typename X, typename R, typename Y, int G, int V, int TH, bool TINY>
 __global__ __launch_bounds__(TH) void residual_bwd_kernel(ResidualArgs a, int waves, long long per, long long blocks) {
   extern __shared__ float s_row[];          // [slots][D]
   __shared__ float s_sum[2 * 32];
@@ -84,7 +83,7 @@ __global__ __launch_bounds__(TH) void residual_bwd_kernel(ResidualArgs a, int wa
   const float inv = 1.f / (float)a.D;
   const bool eights = (a.D & 7) == 0;
   const bool cols = a.gate_kind == GATE_CHANNEL || a.gate_kind == GATE_SEQUENCE;
-  const bool norm = USUAL || (a.weight && a.dy), has_dh = USUAL || a.dh;
+  const bool norm = a.weight && a.dy, has_dh = a.dh;
   const float scale = a.branch_scale * (a.threshold ? a.keep : 1.f);
   // the group's rows, from its block-th run of slots in steps of its workgroups
   const long long group = blockIdx.x / blocks, block = blockIdx.x - group * blocks;
@@ -169,7 +168,7 @@ __global__ __launch_bounds__(TH) void residual_bwd_kernel(ResidualArgs a, int wa
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[v][e] += t[e];
       }
-      if ((USUAL || a.dx) && (G == WAVE || live)) {
+      if (a.dx && (G == WAVE || live)) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) t[e] = a.residual_scale * d[v][e];
         put8<TINY>(static_cast<X*>(a.dx) + at, c[v], t);
@@ -200,7 +199,7 @@ __global__ __launch_bounds__(TH) void residual_bwd_kernel(ResidualArgs a, int wa
       if (a.post_weight) sums[0] += lane_sum<TINY>(c[v], eights, [&](int e) { return d[v][e] * b[v][e]; });
     }
     if (a.post_weight || (token && a.dgate)) row_sum<G, 2>(sums, waves, s_sum, side);
-    if (USUAL || a.dbranch) {
+    if (a.dbranch) {
       const float mean = sums[0] * inv;      // 0 without a norm on the branch
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -321,17 +320,15 @@ template <typename X, typename R, typename Y>
 hipError_t launch_bwd(const ResidualArgs& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)(p.groups * p.blocks));
   const size_t lds = (size_t)p.slots * a.D * 4;
-#define NGDN_GO(G, V, TH, USUAL, TINY)                                                                     \
-  hipLaunchKernelGGL((residual_bwd_kernel<X, R, Y, G, V, TH, USUAL, TINY>), grid, dim3(p.threads), lds, st, a, \
-                     p.waves, p.per, p.blocks)
-  const bool usual = a.weight && a.dy && a.dh && a.dx && a.dbranch;
-  if (a.D < 8) NGDN_GO(8, 1, 256, false, true);
-  else if (p.lanes == 8) NGDN_GO(8, 1, 256, false, false);
-  else if (p.lanes == 16) NGDN_GO(16, 1, 256, false, false);
-  else if (p.lanes == 32) NGDN_GO(32, 1, 256, false, false);
-  else if (p.V == 1 && usual) NGDN_GO(64, 1, 1024, true, false);
-  else if (p.V == 1) NGDN_GO(64, 1, 1024, false, false);
-  else NGDN_GO(64, 2, 1024, false, false);
+#define NGDN_GO(G, V, TH, TINY)                                                                             \
+  hipLaunchKernelGGL((residual_bwd_kernel<X, R, Y, G, V, TH, TINY>), grid, dim3(p.threads), lds, st, a, p.waves, \
+                     p.per, p.blocks)
+  if (a.D < 8) NGDN_GO(8, 1, 256, true);
+  else if (p.lanes == 8) NGDN_GO(8, 1, 256, false);
+  else if (p.lanes == 16) NGDN_GO(16, 1, 256, false);
+  else if (p.lanes == 32) NGDN_GO(32, 1, 256, false);
+  else if (p.V == 1) NGDN_GO(64, 1, 1024, false);
+  else NGDN_GO(64, 2, 1024, false);
 #undef NGDN_GO
   return hipGetLastError();
 }

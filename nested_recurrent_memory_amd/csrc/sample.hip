@@ -14,7 +14,7 @@
 // A workgroup of 1024 threads has a row, each wave a run of it. What bounds it is the one
 // CU that a row has: 256 rows of 131072 fp32, top_k 50 and top_p 0.95, 38 us, of which 26 to
 // 29 read the 134 MB (4.6 to 5.2 TB/s) and the rest are latencies; a row of 32000 bf16 with
-// top_p 0.9 20 us: 2.6 to read, 8 the weights by bins (5.7 of them fp64 arithmetic), 4 to
+// top_p 0.9 19 us: 2.6 to read, 8 the weights by bins (5.7 of them fp64 arithmetic), 3 to
 // find the bin, 4 for the candidates.
 //
 // The row is read once for its maximum, and the largest value of each lane's groups of
