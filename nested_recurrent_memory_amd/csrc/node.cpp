@@ -185,6 +185,13 @@ const void* raw(const Tensor& t) {
   if (!t.has_storage() || t.key_set().has(c10::DispatchKey::Python))
     throw std::runtime_error("the library's kernels take plain tensors: function transforms, tracers and tensor "
                              "subclasses are not supported");
+  if (t.numel() > 0) {
+    // a parameter whose memory has been taken back for now (sharded training) still has its shape
+    int64_t end = t.storage_offset() + 1;
+    for (int64_t d = 0; d < t.dim(); ++d) end += (t.size(d) - 1) * t.stride(d);
+    if ((size_t)end * t.element_size() > t.storage().nbytes())
+      throw std::runtime_error("a tensor's memory does not hold it (released, or not yet there)");
+  }
   return t.const_data_ptr();
 }
 void* raw_out(const Tensor& t) {

@@ -497,3 +497,46 @@ def test_threads_and_streams_at_once():
     for t in threads:
         t.join()
     assert all(torch.equal(p, q) for a, b in zip(got, want) for p, q in zip(a, b))
+
+
+def test_one_tensor_in_several_places():
+    """x as the branch too, one weight for both norms: their gradients add."""
+    a, dh, dy = make((4, 56), TYPES[0], post=False)
+    x, w = a["x"].cuda().requires_grad_(True), a["weight"].cuda().requires_grad_(True)
+    h, y = residual_norm(x, x, w, post_weight=w, gate=x)
+    dx, dw = torch.autograd.grad([h, y], [x, w], [dh.cuda(), dy.cuda()])
+    o = oracle.residual_norm(a["x"], a["x"], a["weight"], a["weight"], a["x"], dh=dh, dy=dy)
+    add = lambda *n: tuple(sum(o[k][j] for k in n) for j in (0, 1))  # noqa: E731
+    # autograd adds them in fp32: a rounding each
+    for got, names in ((dx, ("dx", "dbranch", "dgate")), (dw, ("dweight", "dpost_weight"))):
+        value, bound = add(*names)
+        close(names[0], got, (value, bound + 2 * 2.0 ** -24 * sum(o[k][0].abs() for k in names)), F32)
+
+
+def test_backward_twice_expanded_gradients_and_inference_mode():
+    a, dh, dy = make((3, 7, 30), TYPES[1], "channel")
+    cu = {n: t.cuda().requires_grad_(True) for n, t in a.items()}
+    h, y = residual_norm(**cu, p=0.2, seed=6)
+    one = torch.ones(1, dtype=BF16)
+    grads = [torch.autograd.grad([h, y], list(cu.values()), [one.cuda().expand(3, 7, 30)] * 2, retain_graph=i == 0)
+             for i in range(2)]
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
+    want = oracle.residual_norm(**a, p=0.2, seed=6, dh=one.expand(3, 7, 30), dy=one.expand(3, 7, 30))
+    for n, t in zip(NAMES, grads[0]):
+        close("d" + n, t, want["d" + n], a[n].dtype)
+    with torch.inference_mode():
+        again = residual_norm(**{n: t.cuda() for n, t in a.items()}, p=0.2, seed=6)
+        assert torch.equal(h, again[0]) and torch.equal(y, again[1])
+        assert torch.equal(dropout(again[0], 0.3, 2), dropout(h.detach(), 0.3, 2))
+
+
+def test_tensors_whose_memory_was_released_are_refused():
+    """As sharded training leaves a parameter between its uses."""
+    a, _, _ = make((4, 56), TYPES[0])
+    x, b, w = a["x"].cuda(), a["branch"].cuda(), a["weight"].cuda()
+    big = torch.ones(200, device="cuda")
+    part = big[100:156]
+    big.untyped_storage().resize_(0)
+    for f in (lambda: residual_norm(x, b, part), lambda: residual_norm(x, b, w, gate=part), lambda: dropout(part, 0.5, 1)):
+        with pytest.raises(RuntimeError, match="memory does not hold it"):
+            f()
