@@ -235,6 +235,30 @@ class NestedGDN2Block(GradientCheckpointingLayer):
         return self.join(hidden_states, mlp_out, self.branch("mlp")), past_key_values
 
 
+def _joining(layer):
+    """The block in a layer (the layer itself, or inside a module that wraps it) that has a
+    norm, a gate, a scale or dropout for its outputs; None if they are plainly added."""
+    if not isinstance(layer, NestedGDN2Block):
+        layer = next((m for m in layer.modules() if isinstance(m, NestedGDN2Block)), None)
+    return None if layer is None or layer.plain else layer
+
+
+def _alike(a, b):
+    """Whether block b's first norm may add what block a left (each as _joining gives it)."""
+    if a is None or b is None:
+        return a is b
+    return (a.branch_scale, a.resid_dropout, a.training) == (b.branch_scale, b.resid_dropout, b.training)
+
+
+def _join(block, hidden_states, out, norm=None):
+    """The stream with an MLP output added, by the block that it is of."""
+    if block is not None:
+        return block.join(hidden_states, out, block.branch("mlp"), norm)
+    if norm is None:
+        return hidden_states + out
+    return add_rms_norm(hidden_states, out, norm.weight, norm.eps)
+
+
 class NestedGDN2PreTrainedModel(PreTrainedModel):
     config_class = NestedGDN2Config
     base_model_prefix = "model"
@@ -292,27 +316,29 @@ class NestedGDN2Model(NestedGDN2PreTrainedModel):
         if use_cache and not isinstance(past_key_values, NestedGDN2Cache):
             past_key_values = NestedGDN2Cache.from_legacy_cache(past_key_values)
         all_hidden_states = () if output_hidden_states else None
-        # each block's MLP output, added inside the next norm, the block, and what it
-        # says of that output
-        residual, last, params = None, None, (None, None)
+        # each block's MLP output, added inside the next norm, and the block, where it does
+        # more with that output than add it
+        residual, last = None, None
         for layer in self.layers:
+            block = _joining(layer)
+            if residual is not None and (output_hidden_states or not _alike(last, block)):
+                hidden_states, residual = _join(last, hidden_states, residual), None
             if output_hidden_states:
-                if residual is not None:
-                    hidden_states, residual = last.join(hidden_states, residual, params), None
                 all_hidden_states += (hidden_states,)
+            extra = {} if last is None or residual is None else {"residual_params": last.branch("mlp")}
             # the tensors positionally, as checkpointing with use_reentrant
             # needs them
             hidden_states, residual, past_key_values = layer(
                 hidden_states, residual, past_key_values=past_key_values, use_cache=use_cache,
-                defer_residual=True, residual_params=params)
-            last, params = layer, layer.branch("mlp")
+                defer_residual=True, **extra)
+            last = block
         if use_cache:
             past_key_values.seen_tokens += hidden_states.shape[1]
         if residual is not None and self.config.fuse_norm:
-            _, hidden_states = last.join(hidden_states, residual, params, self.norm)
+            _, hidden_states = _join(last, hidden_states, residual, self.norm)
         else:
             if residual is not None:
-                hidden_states = hidden_states + residual
+                hidden_states = _join(last, hidden_states, residual)
             hidden_states = self.norm(hidden_states)
         if output_hidden_states:
             all_hidden_states += (hidden_states,)
