@@ -116,6 +116,13 @@ class NestedGDN2Config(PretrainedConfig):
         super().__init__(tie_word_embeddings=tie_word_embeddings, **kwargs)
 
 
+def _options(config):
+    """post_norm, layer_scale, branch_scale, resid_dropout: unset where the config is of a
+    class without them (the reference's)."""
+    return (getattr(config, "post_norm", False), getattr(config, "layer_scale", None),
+            getattr(config, "branch_scale", 1.0), getattr(config, "resid_dropout", 0.0))
+
+
 class NestedGDN2Cache(dict):
     """Per-layer decoding state keyed by layer index, plus the count of tokens
     seen (``get_seq_length``)."""
@@ -163,15 +170,14 @@ class NestedGDN2Block(GradientCheckpointingLayer):
                             hidden_act=config.hidden_act, fuse_swiglu=config.fuse_swiglu)
         # what happens to the two outputs before they are added
         D = config.hidden_size
-        self.branch_scale, self.resid_dropout = config.branch_scale, config.resid_dropout
-        if config.post_norm:
+        post_norm, layer_scale, self.branch_scale, self.resid_dropout = _options(config)
+        if post_norm:
             self.attn_post_norm = RMSNorm(D, eps=config.norm_eps)
             self.mlp_post_norm = RMSNorm(D, eps=config.norm_eps)
-        if config.layer_scale is not None:
-            self.attn_gate = nn.Parameter(torch.full((D,), float(config.layer_scale)))
-            self.mlp_gate = nn.Parameter(torch.full((D,), float(config.layer_scale)))
-        self.plain = not (config.post_norm or config.layer_scale is not None
-                          or config.branch_scale != 1.0 or config.resid_dropout)
+        if layer_scale is not None:
+            self.attn_gate = nn.Parameter(torch.full((D,), float(layer_scale)))
+            self.mlp_gate = nn.Parameter(torch.full((D,), float(layer_scale)))
+        self.plain = not (post_norm or layer_scale is not None or self.branch_scale != 1.0 or self.resid_dropout)
 
     def branch(self, which):
         """The norm's weight and the gate of "attn" or "mlp" (None where there is none)."""
@@ -273,9 +279,10 @@ class NestedGDN2PreTrainedModel(PreTrainedModel):
             for p in (module.A_log, module.dt_bias):
                 p._no_weight_decay = True
             return
-        if isinstance(module, NestedGDN2Block) and self.config.layer_scale is not None:
-            nn.init.constant_(module.attn_gate, self.config.layer_scale)
-            nn.init.constant_(module.mlp_gate, self.config.layer_scale)
+        layer_scale = _options(self.config)[1]
+        if isinstance(module, NestedGDN2Block) and layer_scale is not None:
+            nn.init.constant_(module.attn_gate, layer_scale)
+            nn.init.constant_(module.mlp_gate, layer_scale)
         if isinstance(module, (nn.Linear, nn.Conv1d, ShortConvolution)):
             nn.init.normal_(module.weight, mean=0.0, std=self.config.initializer_range)
             if getattr(module, "bias", None) is not None:

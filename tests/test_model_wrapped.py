@@ -33,3 +33,20 @@ def test_replacement_layers(output_hidden_states):
     assert torch.equal(out.last_hidden_state, m.norm(want[-1]))
     if output_hidden_states:
         assert all(torch.equal(a, b) for a, b in zip(out.hidden_states, want[:3]))
+
+
+NEW = ("post_norm", "layer_scale", "branch_scale", "resid_dropout")
+
+
+def test_a_config_without_the_options():
+    """The reference's config, or one pickled before this package had them."""
+    cfg = NestedGDN2Config(vocab_size=64, hidden_size=64, num_hidden_layers=1, num_heads=1, head_dim=64,
+                           n_queries_per_level=(16,))
+    want = set(NestedGDN2Model(cfg).state_dict())
+    for n in NEW:
+        delattr(cfg, n)
+    m = NestedGDN2Model(cfg)
+    assert set(m.state_dict()) == want
+    assert m.layers[0].branch("attn") == m.layers[0].branch("mlp") == (None, None)
+    x, y = torch.randn(2, 3, 64), torch.randn(2, 3, 64)
+    assert torch.equal(m.layers[0].join(x, y, (None, None)), x + y)
