@@ -155,6 +155,9 @@ class NestedGDN2Block(GradientCheckpointingLayer):
     training forward keeps only the block's inputs and recomputes the rest in
     the backward (caching is switched off for it, as the base class does)."""
 
+    # of blocks pickled before they had options for their outputs
+    plain, branch_scale, resid_dropout = True, 1.0, 0.0
+
     def __init__(self, config, layer_idx):
         super().__init__()
         # fuse_norm=False: torch's nn.RMSNorm and plain residual adds, as the

@@ -50,3 +50,15 @@ def test_a_config_without_the_options():
     assert m.layers[0].branch("attn") == m.layers[0].branch("mlp") == (None, None)
     x, y = torch.randn(2, 3, 64), torch.randn(2, 3, 64)
     assert torch.equal(m.layers[0].join(x, y, (None, None)), x + y)
+
+
+def test_a_model_pickled_before_the_options(tmp_path):
+    """Its blocks have none of their attributes."""
+    m = NestedGDN2Model(NestedGDN2Config(vocab_size=64, hidden_size=64, num_hidden_layers=1, num_heads=1, head_dim=64,
+                                         n_queries_per_level=(16,)))
+    for n in ("plain", "branch_scale", "resid_dropout"):
+        del m.layers[0].__dict__[n]
+    torch.save(m, tmp_path / "model.pt")
+    block = torch.load(tmp_path / "model.pt", weights_only=False).layers[0]
+    x, y = torch.randn(2, 3, 64), torch.randn(2, 3, 64)
+    assert torch.equal(block.join(x, y, block.branch("mlp")), x + y)
