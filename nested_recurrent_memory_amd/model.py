@@ -408,25 +408,27 @@ class NestedGDN2ForCausalLM(NestedGDN2PreTrainedModel, GenerationMixin):
         from ``generator``, if None): the same ones give the same tokens. With
         ``eos_token_id`` a sequence that has ended goes on with it, and the call
         ends with the last sequence (a host synchronisation a token; without it
-        there is none). A sequence whose logits are not finite goes on with -1."""
+        there is none). A sequence goes on with -1 from where its logits have no answer."""
         B = input_ids.shape[0]
         if u is None:
             u = torch.rand(B, max_new_tokens, device=input_ids.device, generator=generator)
         if u.shape != (B, max_new_tokens):
             raise ValueError(f"sample: u {tuple(u.shape)} for {B} sequences and {max_new_tokens} tokens")
-        u, cache, token = u.t().contiguous(), None, input_ids
+        u, cache, given, token = u.t().contiguous(), None, input_ids, None
         ended = torch.zeros(B, dtype=torch.bool, device=input_ids.device)
         for i in range(max_new_tokens):
-            out = self.model(input_ids=token, past_key_values=cache, use_cache=True, return_dict=True)
+            out = self.model(input_ids=given, past_key_values=cache, use_cache=True, return_dict=True)
             cache = out.past_key_values
-            token = sample_tokens(self.lm_head(out.last_hidden_state[:, -1]), u[i], temperature, top_k, top_p, min_p)
+            drawn = sample_tokens(self.lm_head(out.last_hidden_state[:, -1]), u[i], temperature, top_k, top_p, min_p)
+            token = drawn if token is None else torch.where(token < 0, token, drawn)
             if eos_token_id is not None:
                 token = torch.where(ended, eos_token_id, token)
                 ended |= token == eos_token_id
-            token = token.unsqueeze(1)
-            input_ids = torch.cat((input_ids, token), 1)
+            input_ids = torch.cat((input_ids, token.unsqueeze(1)), 1)
             if eos_token_id is not None and bool(ended.all()):
                 break
+            # -1 is no id: a lookup may read outside the table for it
+            given = token.clamp(min=0).unsqueeze(1)
         return input_ids
 
     def forward(self, input_ids=None, attention_mask=None, inputs_embeds=None, labels=None,
