@@ -408,7 +408,12 @@ class NestedGDN2ForCausalLM(NestedGDN2PreTrainedModel, GenerationMixin):
         from ``generator``, if None): the same ones give the same tokens. With
         ``eos_token_id`` a sequence that has ended goes on with it, and the call
         ends with the last sequence (a host synchronisation a token; without it
-        there is none). A sequence goes on with -1 from where its logits have no answer."""
+        there is none). A sequence goes on with -1 from where its logits have no answer.
+        Blocks in training that drop values or keep no cache are refused."""
+        if any(b.training and (b.resid_dropout or b.gradient_checkpointing)
+               for b in self.modules() if isinstance(b, NestedGDN2Block)):
+            raise RuntimeError("sample: the model is in training mode with dropout or gradient checkpointing; "
+                               "call eval() first")
         B = input_ids.shape[0]
         if u is None:
             u = torch.rand(B, max_new_tokens, device=input_ids.device, generator=generator)

@@ -45,3 +45,38 @@ def test_a_sequence_without_a_token_goes_on_with_minus_one(stand, eos):
     assert len(given) == 4 and torch.equal(given[0], ids)
     assert all(t.shape == (3, 1) and (t >= 0).all() and (t < 64).all() for t in given[1:])
     assert [t[0].item() for t in given[1:]] == want[0][:3]
+
+
+def test_sampling_in_training_mode_is_refused_where_it_would_drop(stand):
+    """With dropout the same u would not give the same tokens, and checkpointing's
+    layers keep no cache. Without either, and in evaluation, the mode is no matter."""
+    m, given, tokens = stand
+    ids, u = torch.tensor([[1, 2]]), torch.rand(1, 1)
+
+    def tokens_of(**kw):
+        tokens[:] = [[5]]
+        return m.sample(ids, 1, u=u, **kw).tolist()
+
+    assert m.train() and tokens_of() == [[1, 2, 5]]
+    m.model.layers = nn.ModuleList([model_module.NestedGDN2Block(NestedGDN2Config(
+        vocab_size=64, hidden_size=64, num_hidden_layers=1, num_heads=1, head_dim=64, n_queries_per_level=(16,),
+        resid_dropout=0.1), 0)])
+    for mode in (m, m.model.layers[0]):
+        mode.train()
+        state = torch.get_rng_state()
+        with pytest.raises(RuntimeError, match="eval"):
+            tokens_of()
+        assert torch.equal(state, torch.get_rng_state()) and m.model.layers[0].training
+        m.eval()
+        assert tokens_of() == [[1, 2, 5]]
+    m.train()
+    m.model.layers[0].eval()
+    assert tokens_of() == [[1, 2, 5]]
+    m.model.layers[0].resid_dropout = 0.0
+    m.train()
+    assert tokens_of() == [[1, 2, 5]]
+    m.model.layers[0].gradient_checkpointing = True
+    with pytest.raises(RuntimeError, match="eval"):
+        tokens_of()
+    m.eval()
+    assert tokens_of() == [[1, 2, 5]]
