@@ -479,6 +479,7 @@ struct Setting {
     if (whole_number) {
       if (!PyIndex_Check(v.ptr())) refuse(std::string("sample_tokens: ") + which + " must be an integer");
       const py::object i = py::reinterpret_steal<py::object>(PyNumber_Index(v.ptr()));
+      if (!i) throw py::error_already_set();
       int over = 0;
       const long long n = PyLong_AsLongLongAndOverflow(i.ptr(), &over);
       value = over ? (over > 0 ? 1e9 : 0) : (double)(n > 1000000000 ? 1000000000 : n < 0 ? 0 : n);
