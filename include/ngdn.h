@@ -69,7 +69,7 @@ const char* ngdn_last_error(void);
  * 0.5.0 took W and U out of ngdn_l0_bwd; 0.6.0 moved the upper levels'
  * lower-state gradients from ngdn_probe_bwd's d_below to an injection that
  * ngdn_upper_scan_bwd adds. */
-#define NGDN_VERSION 1300
+#define NGDN_VERSION 1301
 int32_t ngdn_version(void);
 /* Offload architecture the library was built for ("gfx950"). */
 const char* ngdn_arch(void);
@@ -708,7 +708,7 @@ int64_t ngdn_residual_norm_ws(const ngdn_residual_args* r);
  * The token is the first in index order with the kept weights up to and with it
  * above u times their sum. temperature 0: the first of the largest. A row whose
  * largest logit is not finite, that holds a NaN, or whose settings are outside
- * their ranges (temperature finite and >= 0, top_p >= 0, 0 <= min_p <= 1) gives
+ * their ranges (temperature finite and >= 0, 0 <= top_p <= 1, 0 <= min_p <= 1) gives
  * -1. Each setting is a scalar, or one a row where its _ptr is set (fp32; top_k
  * int32, or int64 with top_k_wide). 1 <= V <= 2^20. The same inputs give the same
  * token. */

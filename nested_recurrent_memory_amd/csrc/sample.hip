@@ -425,7 +425,7 @@ __global__ __launch_bounds__(TH) void sample_kernel(SampleArgs a, int s_bits, fl
   __syncthreads();
   top = logit_of((uint32_t)s.best);
   const bool fits = !s.bad && top > -INFINITY && top < INFINITY && t >= 0.f && t < INFINITY && top_p >= 0.f &&
-                    min_p >= 0.f && min_p <= 1.f && u >= 0. && u <= 1.;
+                    top_p <= 1.f && min_p >= 0.f && min_p <= 1.f && u >= 0. && u <= 1.;
   if (!fits) {
     if (threadIdx.x == 0) a.token[r] = -1;
     return;

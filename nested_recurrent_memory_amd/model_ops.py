@@ -393,7 +393,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
     logits are bf16, fp16 or fp32, rows of any stride, V up to 2^20; u fp32 or
     fp64. Each setting is a number or a tensor of one a row on the same GPU (fp32;
-    top_k int32 or int64), of which values outside their ranges give -1. The sums
+    top_k int32 or int64). Their ranges: a finite temperature >= 0, top_p and min_p
+    in [0, 1]; a number outside is refused, a row whose value in a tensor is gives -1. The sums
     have no rounding: a row's token depends on nothing but its own inputs. No
     host synchronisation: the call can be captured into a graph."""
     return _node().sample_tokens(logits, u, temperature, top_k, top_p, min_p)

@@ -153,7 +153,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         top = l[i].max()
         if not np.isfinite(top):            # NaN too
             continue
-        if not (0 <= T[i] < np.inf and P[i] >= 0 and 0 <= least[i] <= 1 and 0 <= U01[i] <= 1):
+        if not (0 <= T[i] < np.inf and 0 <= P[i] <= 1 and 0 <= least[i] <= 1 and 0 <= U01[i] <= 1):
             continue
         if T[i] == 0:
             token[i] = int(np.argmax(l[i]))
