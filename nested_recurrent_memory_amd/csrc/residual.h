@@ -174,8 +174,15 @@ __device__ __forceinline__ float lane_sum(const Chunk& c, bool eights, F p) {
   for (int e = 0; e < 8; ++e) s += counts<TINY>(c, e) ? p(e) : 0.f;
   return s;
 }
-// 1 / sqrt(mean + eps), within two units of the last place
-__device__ __forceinline__ float inverse_root(float sum, float inv, float eps) { return rsqrtf(sum * inv + eps); }
+// 1 / sqrt(mean + eps): the hardware's, which is up to a unit off, and a Newton step on it, with
+// what the product loses, after which only the rounding is left (4 x 8192 rows of 2048, bf16, with
+// dropout, both passes: 271 us, as without; 275 by a root and a quotient). Zeros and infinities
+// as they are
+__device__ __forceinline__ float inverse_root(float sum, float inv, float eps) {
+  const float v = sum * inv + eps, r = rsqrtf(v), t = v * r;
+  const float e = fmaf(-t, r, 1.f) - fmaf(v, r, -t) * r;       // 1 - v r^2
+  return v > 0.f && v < INFINITY ? fmaf(0.5f * r, e, r) : r;
+}
 
 // which of the values i ... i + 7 of the stream are kept: word >= threshold (1 to 2^32)
 __device__ __forceinline__ void drop8(const ResidualArgs& a, const PhiloxKey& key, uint64_t i, bool* kept) {
