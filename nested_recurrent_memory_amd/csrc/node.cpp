@@ -178,6 +178,10 @@ Stream stream_from(const char* name, double p, const py::object& seed, const py:
   return s;
 }
 
+// t with its values in memory as they are read, row by row: contiguous, and not a view
+// that stands for their negatives (an imaginary part of a conjugate)
+Tensor whole(const Tensor& t) { return t.defined() ? t.contiguous().resolve_neg() : t; }
+
 // A pointer for a kernel: of memory on the GPU, which tensors of function transforms, fake
 // ones and other subclasses with a dispatch of their own do not hold. Null where undefined.
 const void* raw(const Tensor& t) {
@@ -207,7 +211,7 @@ void plain_gradient(const char* name, const Tensor& g) {
 
 Tensor drop(const Tensor& x, const Stream& s) {
   const c10::DeviceGuard guard(x.device());
-  const Tensor c = x.contiguous();
+  const Tensor c = whole(x);
   Tensor y = at::empty_like(c);
   done(ngdn_dropout(code(c), c.numel(), s.threshold, s.keep(), s.seed, seed_of(s.seed_tensor), s.offset,
                     raw(c), raw_out(y), stream(c)),
@@ -276,8 +280,6 @@ void point(ngdn_residual_args& a, const Parts& t) {
   a.gate = raw(t[4]); a.seed_ptr = seed_of(t[5]);
 }
 
-Tensor whole(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
-
 Parts whole(const Parts& t) {
   Parts c;
   for (int i = 0; i < 6; ++i) c[i] = whole(t[i]);
@@ -309,7 +311,7 @@ struct ResidualFn : torch::autograd::Function<ResidualFn> {
     const c10::DeviceGuard guard(given[0].device());
     Parts t;
     for (int i = 0, j = 0; i < 5; ++i)
-      if (which >> i & 1) t[i] = given[j++].contiguous();
+      if (which >> i & 1) t[i] = whole(given[j++]);
     t[5] = seed.t;
     Tensor out[3];
     residual_forward(t, *r, out, true);
@@ -494,7 +496,7 @@ struct Setting {
   const void* ptr(const Tensor& u, bool whole_number) {
     if (!rows.defined()) return nullptr;
     if (!whole_number && rows.scalar_type() != at::kFloat) rows = rows.to(at::kFloat);
-    rows = rows.dim() == 0 ? rows.expand(u.sizes()).contiguous() : rows.contiguous();
+    rows = whole(rows.dim() == 0 ? rows.expand(u.sizes()) : rows);
     return raw(rows);
   }
 };
@@ -517,12 +519,12 @@ Tensor sample_tokens(const Tensor& logits0, const Tensor& u0, const py::object& 
   const py::gil_scoped_release free;
   const at::NoGradGuard off;
   const c10::DeviceGuard guard(logits0.device());
-  const Tensor u = u0.detach().contiguous();
-  Tensor logits = widened(logits0.detach());
+  const Tensor u = whole(u0.detach());
+  Tensor logits = widened(logits0.detach()).resolve_neg();
   const int64_t V = logits.size(-1);
   int64_t step = V;
   if (logits.dim() == 2 && (logits.stride(1) == 1 || V == 1)) step = logits.stride(0);
-  else logits = logits.contiguous();
+  else logits = whole(logits);
   Tensor token = at::empty(u.sizes(), u.options().dtype(at::kLong));
   ngdn_sample_args a{};
   a.rows = u.numel(); a.stride = step; a.V = (int32_t)V;
