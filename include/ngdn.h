@@ -710,8 +710,9 @@ int64_t ngdn_residual_norm_ws(const ngdn_residual_args* r);
  * largest logit is not finite, that holds a NaN, or whose settings are outside
  * their ranges (temperature finite and >= 0, 0 <= top_p <= 1, 0 <= min_p <= 1) gives
  * -1. Each setting is a scalar, or one a row where its _ptr is set (fp32; top_k
- * int32, or int64 with top_k_wide). 1 <= V <= 2^20. The same inputs give the same
- * token. */
+ * int32, or int64 with top_k_wide). 1 <= V <= 2^20, rows < 2^22. Weights are rounded
+ * to units of 2^-s, s = 62 - ceil(log2 V), 51 at most; their sums are exact. The same
+ * inputs give the same token. */
 typedef struct ngdn_sample_args {
   int64_t rows, stride;
   int32_t V, u_wide, top_k_wide;

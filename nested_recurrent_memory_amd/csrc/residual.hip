@@ -8,8 +8,10 @@
 //
 // One pass: a row is read once into registers, both statistics are sums over
 // its lanes, and h and y are written from there. y is formed from h before h is
-// rounded to its type, so it carries one rounding; the backward forms the same h
-// from x and branch again, which costs no more bytes than reading h would.
+// rounded to its type, so it carries one rounding; the backward forms h again from
+// x and branch (the same up to fp32 roundings: its factors come in another order), which
+// costs no more bytes than reading h would where a norm or a gate on the branch needs
+// the branch anyway.
 // All arithmetic is in fp32.
 #include "residual.h"
 
@@ -67,8 +69,8 @@ hipError_t dropout(const DropoutArgs& a, int dtype, hipStream_t st) {
 // for them).
 //
 // HBM-bound: 4 x 4096 rows of 2048, fp32 stream and bf16 branch, 403 MB in 77-78 us
-// (5.2 TB/s, a copy's rate); 4 x 8192 rows of 2048, bf16, with dropout, 537 MB in 113
-// us (4.75 TB/s). A workgroup a row with its parameters loaded each time took 111 and
+// (5.2 TB/s, a copy's rate); 4 x 8192 rows of 2048, bf16, with dropout, 537 MB in 109
+// to 113 us (4.75 to 4.9 TB/s). A workgroup a row with its parameters loaded each time took 111 and
 // 226 us, and 12 us for 128 rows, the latencies of four loads in a row, where this takes
 // 4.5. Of the second case's 226 us the generator and the sums' arithmetic were as much as
 // the loads: xor of three in one instruction, wave sums by lane moves instead of through

@@ -359,9 +359,10 @@ def residual_norm(x, branch, weight=None, post_weight=None, gate=None, residual_
     and ``offset`` are ``dropout``'s, over the values of x in row-major order.
 
     h is in x's dtype, y in ``out_dtype`` (x's if None); bf16, fp16 and fp32, any
-    1 <= D <= 16384. y is formed from h before h is rounded (``add_rms_norm``
-    normalises the rounded sum). Differentiable once, in every tensor; sums over
-    rows are fp32 in an order that the shapes fix."""
+    1 <= D <= 16384, fewer than 2^31 rows (and 2^22 sequences with a gate of each). y
+    is formed from h before h is rounded (``add_rms_norm`` normalises the rounded
+    sum). Differentiable once, in every tensor; sums over rows are fp32 in an order
+    that the shapes fix."""
     return _node().residual_norm(x, branch, weight, post_weight, gate, residual_scale, branch_scale, p, seed,
                                  offset, eps, out_dtype)
 
@@ -391,12 +392,14 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     their sum. A temperature of 0 takes the first of the largest logits. A row
     that is all -inf, whose largest logit is +inf, or that holds a NaN gives -1.
 
-    logits are bf16, fp16 or fp32, rows of any stride, V up to 2^20; u fp32 or
-    fp64. Each setting is a number or a tensor of one a row on the same GPU (fp32;
-    top_k int32 or int64). Their ranges: a finite temperature >= 0, top_p and min_p
-    in [0, 1]; a number outside is refused, a row whose value in a tensor is gives -1. The sums
-    have no rounding: a row's token depends on nothing but its own inputs. No
-    host synchronisation: the call can be captured into a graph."""
+    logits are bf16, fp16 or fp32, fewer than 2^22 rows of any stride, V up to 2^20;
+    u fp32 or fp64. Each setting is a number or a tensor of one a row on the same GPU
+    (fp32; top_k int32 or int64). Their ranges: a finite temperature >= 0, top_p and
+    min_p in [0, 1]; a number outside is refused, a row whose value in a tensor is
+    gives -1. Weights are rounded to units of 2^-s, s = 62 - ceil(log2 V) and 51 at
+    most, so a token below half a unit of the largest (2^-46 at V = 131072) is never
+    drawn; their sums have no rounding: a row's token depends on nothing but its own
+    inputs. No host synchronisation: the call can be captured into a graph."""
     return _node().sample_tokens(logits, u, temperature, top_k, top_p, min_p)
 
 

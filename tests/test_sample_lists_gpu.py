@@ -13,7 +13,7 @@ such a one."""
 import pytest
 import torch
 
-import ngdn_residual_oracle as oracle
+from nested_recurrent_memory_amd.model_ops import sample_tokens
 from test_sample_gpu import BF16, F32, check, make
 
 pytestmark = pytest.mark.gpu
@@ -52,3 +52,14 @@ def test_more_than_256_pass_min_p_behind_a_cut():
         for floor in (0.02, 0.05, 0.06):
             for top_p in (1.0, 0.999, 0.9):
                 check(l, u, top_k=k, top_p=top_p, min_p=floor)
+
+
+@pytest.mark.parametrize("V,s", [(131072, 45), (131073, 44), (2048, 51), (9, 51)])
+def test_a_weight_is_rounded_to_its_unit(V, s):
+    """The random number 0 takes the first token that weighs anything: one of 0.6 units
+    weighs one, one of 0.4 none (a logit near -30 in fp32 holds its weight to 2^-19)."""
+    l = torch.full((2, V), -float("inf"), dtype=torch.float64)
+    l[:, 8] = 0.0
+    l[:, 3] = torch.tensor([0.6, 0.4], dtype=torch.float64).log() - s * torch.tensor(2.0, dtype=torch.float64).log()
+    got = sample_tokens(l.float().cuda(), torch.zeros(2, device="cuda"))
+    assert got.tolist() == [3, 8]
